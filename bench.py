@@ -715,7 +715,9 @@ def main():
 
     if a.train:
         return train_bench(a, rank, world, dev, dist)
-    graph_ok, graph_note = (False, "") if a.no_graph or a.graph_probe else graph_probe_child(a, local_dev)
+    # one probe per device: ranks that share a GPU with a lower one leave it to that rank (8 ranks and 8 probes on one card are 16 processes)
+    probes = int(os.environ.get("LOCAL_RANK", "0")) < torch.cuda.device_count()
+    graph_ok, graph_note = (False, "") if a.no_graph or a.graph_probe else graph_probe_child(a, local_dev) if probes else (True, "")
     if dist and not a.graph_probe:            # the leg's timing protocol is collective: every rank runs it, or none does
         t_ok = torch.tensor([1.0 if graph_ok else 0.0], dtype=torch.float64, device=dev if dist.get_backend() == "nccl" else "cpu")
         dist.all_reduce(t_ok, op=dist.ReduceOp.MIN)
