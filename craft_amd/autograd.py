@@ -1179,3 +1179,67 @@ def sequence_loss(flow_preds, flow_gt, valid, gamma: float = 0.8, max_flow: floa
     if defer_metrics:
         return loss, DeferredMetrics(m)
     return loss, DeferredMetrics(m).resolve()
+
+
+# ------------------------------------------------------------------------------------------------------------------
+# LayerNorm with weights; attention with a cap, a distance bias and causal / prefix / document masks
+# ------------------------------------------------------------------------------------------------------------------
+class LayerNorm(Function):
+    """ops.layer_norm with its gradients; keeps x and the two row statistics."""
+
+    @staticmethod
+    def forward(ctx, x, weight, bias, eps):
+        y, mean, rstd = ops._layer_norm(x, weight, bias, eps, None, True)
+        ctx.save_for_backward(x, weight, mean, rstd)
+        ctx.bias_type = None if bias is None else bias.dtype
+        return y
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, mean, rstd = ctx.saved_tensors
+        return (*ops.layer_norm_bwd(x, weight, ctx.bias_type, dy, mean, rstd, ctx.needs_input_grad[:3]), None)
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
+    """Differentiable ``ops.layer_norm`` (gradients of x, weight and bias; the weight's and bias' sums over the rows in fp32, in a fixed order)."""
+    return LayerNorm.apply(x, weight, bias, eps)
+
+
+class Attention(Function):
+    """ops.attention with its gradients; keeps q, k, v, the output and one log-sum per query."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, scale, cap, slopes, causal, prefix, docs, docs_k):
+        plan = ops.AttentionPlan(q, k, v, scale, cap, slopes, causal, prefix, docs, docs_k)
+        B, Nq, Nk, H, Hk, D = plan.dims
+        out = torch.empty(B, Nq, H, D, device=plan.device, dtype=q.dtype)
+        lse = torch.empty(B, H, Nq, device=plan.device, dtype=torch.float32)
+        if out.numel() and Nk:
+            plan.forward(out, lse)
+        else:
+            out.zero_()
+        ctx.save_for_backward(q, k, v, out, lse, slopes, prefix, docs, docs_k)
+        ctx.how = scale, cap, causal
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, go):
+        q, k, v, out, lse, slopes, prefix, docs, docs_k = ctx.saved_tensors
+        rest = (None,) * 7
+        if not out.numel() or not k.shape[1]:
+            return (torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), *rest)
+        scale, cap, causal = ctx.how
+        with torch.no_grad():
+            return (*ops.AttentionPlan(q, k, v, scale, cap, slopes, causal, prefix, docs, docs_k).backward(out, lse, go), *rest)
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optional[float] = None, cap: float = 0.0, slopes: Optional[torch.Tensor] = None,
+              causal: bool = False, prefix: Optional[torch.Tensor] = None, docs: Optional[torch.Tensor] = None,
+              docs_k: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """Differentiable ``ops.attention``: gradients of q, k and v (those of shared key heads summed over the heads that read them); the masks, slopes and
+    the cap have none.  The scores are computed again in the backward pass; no N x N tensor is kept."""
+    if slopes is not None and slopes.requires_grad:
+        raise hip.CraftHipError("attention: slopes have no gradient here")
+    return Attention.apply(q, k, v, scale, cap, slopes, causal, prefix, docs, docs_k)

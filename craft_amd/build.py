@@ -17,8 +17,9 @@ CSRC = os.path.join(HERE, "csrc")
 OBJ = os.path.join(CSRC, "build")
 LIB = os.path.join(HERE, "libcraft_hip.so")
 SOURCES = ["kernels_gemm.hip", "kernels_conv.hip", "kernels_conv_wf.hip", "kernels_conv_c64.hip", "kernels_stem.hip", "kernels_flash.hip", "kernels_attn.hip", "kernels_attn_d32.hip", "kernels_attn_d64.hip", "kernels_attn_d128.hip", "kernels_attn_w.hip",
-           "kernels_misc.hip", "kernels_convf1.hip", "kernels_gemm_gen.hip", "kernels_gemm_pk.hip", "kernels_gemm_pkb_tt.hip", "kernels_gemm_pkb_ct.hip", "kernels_gemm_pkb_cc.hip", "kernels_train.hip", "kernels_enc_train.hip", "kernels_augment.hip", "craft_hip.hip"]
-HEADERS = ["common.hpp", "gemm_engine.hpp", "launch.hpp", "attn_probs.inc.hpp", "conv_epilogue.hpp", "gemm_pkb.inc.hpp", os.path.join("..", "..", "include", "craft_hip.h")]
+           "kernels_misc.hip", "kernels_convf1.hip", "kernels_gemm_gen.hip", "kernels_gemm_pk.hip", "kernels_gemm_pkb_tt.hip", "kernels_gemm_pkb_ct.hip", "kernels_gemm_pkb_cc.hip", "kernels_train.hip", "kernels_enc_train.hip", "kernels_augment.hip", "kernels_layernorm.hip", "kernels_orthogonalize.hip",
+           "kernels_attention.hip"] + [f"kernels_attention_{t}_d{d}.hip" for t in ("f16", "bf16", "f32") for d in (32, 64, 128)] + ["craft_hip.hip"]
+HEADERS = ["common.hpp", "gemm_engine.hpp", "launch.hpp", "attn_probs.inc.hpp", "conv_epilogue.hpp", "gemm_pkb.inc.hpp", "attention_tile.hpp", "attention_fwd.inc.hpp", "attention_token.inc.hpp", "attention_bwd.inc.hpp", os.path.join("..", "..", "include", "craft_hip.h")]
 ARCH = "gfx950"
 
 
@@ -61,7 +62,7 @@ def build_extension(force: bool = False, extra_flags=()) -> str:
             os.remove(os.path.join(OBJ, f))
         if os.path.exists(LIB):
             os.remove(LIB)
-    with concurrent.futures.ThreadPoolExecutor(max_workers=len(SOURCES)) as ex:
+    with concurrent.futures.ThreadPoolExecutor(max_workers=os.cpu_count() or 8) as ex:
         objs = list(ex.map(lambda s: _compile(s, extra_flags), SOURCES))
     if _stale(LIB, objs):
         cmd = [_hipcc(), f"--offload-arch={ARCH}", "-shared", "-fPIC", "-o", LIB] + objs

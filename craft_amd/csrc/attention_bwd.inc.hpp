@@ -1,0 +1,399 @@
+// Backward attention.  With p = 2^(z - lse), delta_i = sum_d go_i o_i:
+//   dv_j = sum_i p_ij go_i;  dp_ij = go_i . v_j;  ds_ij = p_ij (dp_ij - delta_i) (1 - tanh^2);  dq_i = scale sum_j ds_ij k_j;  dk_j = scale sum_i ds_ij q_i
+// Two kernels, each the sole writer of its gradients (no atomics: the result does not depend on the order of the blocks): k_attention_dq owns 128
+// queries and walks over the keys, k_attention_dkv owns 128 keys and walks over the queries of every head that shares them.  Both recompute the scores.
+#pragma once
+#include "attention_tile.hpp"
+
+namespace craft {
+
+// delta, 16 lanes to a row
+template <typename T>
+__global__ __launch_bounds__(256) void k_attention_delta(AttentionParams p, float* delta) {
+  const long row = (long)blockIdx.x * 16 + (threadIdx.x >> 4), rows = (long)p.B * p.Nq * p.H;
+  if (row >= rows) return;                                                 // (whole 16-lane groups)
+  const int head = (int)(row % p.H);
+  const long bi = row / p.H, b = bi / p.Nq, i = bi - b * p.Nq;
+  const int c = 8 * (threadIdx.x & 15);
+  float s = 0.f;
+  if (c < p.D) {
+    typedef typename AtFrag<T>::type frag_t;
+    const frag_t o = *reinterpret_cast<const frag_t*>(reinterpret_cast<const T*>(p.o) + b * p.o_b + i * p.o_n + head * p.o_h + c);
+    const frag_t g = *reinterpret_cast<const frag_t*>(reinterpret_cast<const T*>(p.go) + b * p.go_b + i * p.go_n + head * p.go_h + c);
+#pragma unroll
+    for (int j = 0; j < 8; ++j) s += (float)o[j] * (float)g[j];
+  }
+#pragma unroll
+  for (int k = 8; k > 0; k >>= 1) s += __shfl_xor(s, k);
+  if ((threadIdx.x & 15) == 0) delta[(b * p.H + head) * p.Nq + i] = s;
+}
+
+template <typename T, int DP> struct BwdShape {
+  static constexpr int TR = sizeof(T) == 2 ? 64 : 32;                     // rows of a tile
+  static constexpr int TILE = TR * DP * (int)sizeof(T);
+  static constexpr int STAGE = 2 * TILE + 3 * 256;                        // two operands; lse, delta, documents of 64 rows
+  static constexpr int LDS = 2 * STAGE + 64;
+};
+
+// dq: lane = query
+template <typename T, int DP, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256) void k_attention_dq(AttentionParams p) {
+  typedef BwdShape<T, DP> S;
+  typedef typename AtFrag<T>::type frag_t;
+  constexpr int TK = S::TR, NB = TK / 32;
+  extern __shared__ __align__(16) unsigned char lds[];
+  const unsigned lds0 = (unsigned)(size_t)(CRAFT_LDS unsigned char*)lds;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int nqt = (p.Nq + 127) >> 7;
+  const int id = xcd_chunk(blockIdx.x, gridDim.x), bh = id / nqt, qt = nqt - 1 - (id - bh * nqt);
+  const int b = bh / p.H, head = bh - b * p.H, kvh = head / (p.H / p.Hk);
+  const int off = p.Nk - p.Nq, i0 = qt * 128, i_last = min(i0 + 127, p.Nq - 1);
+  const int prefix = p.prefix ? p.prefix[b] : 0;
+  const int i = min(i0 + wave * 32 + (lane & 31), p.Nq - 1), pos = i + off;
+  int lim = p.causal ? min(max(pos + 1, prefix), p.Nk) : p.Nk;
+  int mydoc = 0;
+  if (p.docq) { mydoc = p.docq[(long)b * p.Nq + i]; if (mydoc < 0) lim = 0; }
+  int lim_lo = lim, lim_hi = lim;
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) { lim_lo = min(lim_lo, __shfl_xor(lim_lo, o)); lim_hi = max(lim_hi, __shfl_xor(lim_hi, o)); }
+  lim_lo = __builtin_amdgcn_readfirstlane(lim_lo); lim_hi = __builtin_amdgcn_readfirstlane(lim_hi);
+
+  frag_t qf[DP / 16], gf[DP / 16];
+  load_own<T, DP>(reinterpret_cast<const T*>(p.q) + b * p.q_b + (long)i * p.q_n + head * p.q_h, p.D, h, qf);
+  load_own<T, DP>(reinterpret_cast<const T*>(p.go) + b * p.go_b + (long)i * p.go_n + head * p.go_h, p.D, h, gf);
+  const float lse = p.lse[(long)bh * p.Nq + i], delta = p.delta[(long)bh * p.Nq + i];
+
+  int t0 = 0, t1 = p.causal ? (max(min(max(i_last + off + 1, prefix), p.Nk), 0) + TK - 1) / TK : (p.Nk + TK - 1) / TK;
+  int4 qr = make_int4(0, 0, 0, 0), qrw = qr;
+  const int4* rk = nullptr;
+  const int kgroups = (p.Nk + 31) >> 5;
+  if (p.rq) {
+    const int qgroups = (p.Nq + 31) >> 5;
+    const int4* rq = p.rq + (long)b * qgroups;
+    rk = p.rk + (long)b * kgroups;
+    qr = join_ranges(rq, i0 >> 5, min((i0 >> 5) + 4, qgroups) - 1);
+    qrw = rq[min((i0 >> 5) + wave, qgroups - 1)];
+    tiles_of_documents<256>(rk, kgroups, NB, qr, t0, t1, tid, reinterpret_cast<int*>(lds + 2 * S::STAGE));
+  }
+  const int nchunk = p.D * (int)sizeof(T) / 16;
+  const unsigned kst = (unsigned)(p.k_n * (long)sizeof(T)), vst = (unsigned)(p.v_n * (long)sizeof(T));
+  TileCopy<T, DP, TK, 4> kc, vc;
+  kc.init(wave, lane, kst, nchunk);
+  vc.init(wave, lane, vst, nchunk);
+  const unsigned char* kb = reinterpret_cast<const unsigned char*>(p.k) + (b * p.k_b + kvh * p.k_h) * (long)sizeof(T);
+  const unsigned char* vb = reinterpret_cast<const unsigned char*>(p.v) + (b * p.v_b + kvh * p.v_h) * (long)sizeof(T);
+  auto range = [&](int t) { return join_ranges(rk, t * NB, min(t * NB + NB, kgroups) - 1); };
+  auto next = [&](int t) { if (rk) while (t < t1 && !ranges_meet(range(t), qr)) ++t; return t; };
+  auto stage = [&](int buf, int t) {
+    const int valid = p.Nk - t * TK;
+    const unsigned at = lds0 + (unsigned)buf * S::STAGE;
+    kc.issue(kb + (long)t * TK * kst, kst, nchunk, valid, at, wave, lane);
+    vc.issue(vb + (long)t * TK * vst, vst, nchunk, valid, at + S::TILE, wave, lane);
+    if (rk && wave == 0) copy_words(p.dock + (long)b * p.Nk, (long)t * TK, p.Nk - 1, at + 2 * S::TILE, lane);
+  };
+
+  f32x16 dq[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dq[d][r] = 0.f;
+  const float slope2 = BIAS ? p.slopes[head] * 1.44269504088896f : 0.f;
+
+  int t = next(t0), buf = 0;
+  if (t < t1) stage(0, t);
+  while (t < t1) {
+    wait_copies();
+    __syncthreads();
+    const int tn = next(t + 1);
+    if (tn < t1) stage(buf ^ 1, tn);
+    unsigned char* K = lds + buf * S::STAGE;
+    unsigned char* V = K + S::TILE;
+    const int* ids = reinterpret_cast<const int*>(V + S::TILE);
+    const int k0 = t * TK;
+    bool docmask = false, skip = k0 >= lim_hi;
+    if (rk) {
+      const int4 kr = range(t);
+      if (kr.z) { zero_rows<T, DP, TK>(K, ids, p.Nk - k0, tid, 256); __syncthreads(); }
+      docmask = !one_document(kr, qrw);
+      skip |= !ranges_meet(kr, qrw);
+    }
+    if (!skip) {
+      const bool masked = docmask || k0 + TK > lim_lo;
+#pragma unroll
+      for (int kbk = 0; kbk < NB; ++kbk) {
+        f32x16 x, y;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = y[r] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) at_mma(tile_row<T, DP>(K, 32 * kbk + (lane & 31), ks, h), qf[ks], x);
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) at_mma(tile_row<T, DP>(V, 32 * kbk + (lane & 31), ks, h), gf[ks], y);
+        const float away = BIAS ? (float)(pos - k0 - 32 * kbk - 4 * h) : 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          float th = 0.f;
+          float z = at_score<T, CAP>(p, x[r], th);
+          if constexpr (BIAS) z -= slope2 * fabsf(away - (float)acc_row(r));
+          float ds = __builtin_amdgcn_exp2f(z - lse) * (y[r] - delta);
+          if constexpr (CAP) ds *= 1.f - th * th;
+          x[r] = ds;
+        }
+        if (masked) {                                                     // a choice, not a product: what the mask hides may be inf or NaN
+          const int room = lim - k0 - 32 * kbk - 4 * h;
+#pragma unroll
+          for (int r = 0; r < 16; ++r) x[r] = acc_row(r) < room ? x[r] : 0.f;
+          if (docmask) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+              const int4 d = *reinterpret_cast<const int4*>(ids + 32 * kbk + 8 * g + 4 * h);
+              x[4 * g + 0] = d.x == mydoc ? x[4 * g + 0] : 0.f;
+              x[4 * g + 1] = d.y == mydoc ? x[4 * g + 1] : 0.f;
+              x[4 * g + 2] = d.z == mydoc ? x[4 * g + 2] : 0.f;
+              x[4 * g + 3] = d.w == mydoc ? x[4 * g + 3] : 0.f;
+            }
+          }
+        }
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2) {
+          const frag_t sf = at_pack<T>(x, s2);
+#pragma unroll
+          for (int d = 0; d < DP / 32; ++d) at_mma(tile_col<T, DP>(K, 32 * kbk + 16 * s2, d, lane), sf, dq[d]);
+        }
+      }
+    }
+    t = tn;
+    buf ^= 1;
+  }
+  if (i0 + wave * 32 + (lane & 31) < p.Nq) {
+    T* row = reinterpret_cast<T*>(p.dq) + (((long)b * p.Nq + i) * p.H + head) * p.D;
+    typedef T t4 __attribute__((ext_vector_type(4)));
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int c = 32 * d + 8 * g + 4 * h;
+        if (c < p.D) {
+          t4 w;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) w[j] = (T)(dq[d][4 * g + j] * p.scale);
+          *reinterpret_cast<t4*>(row + c) = w;
+        }
+      }
+  }
+}
+
+// dk, dv: lane = key
+template <typename T, int DP, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256) void k_attention_dkv(AttentionParams p) {
+  typedef BwdShape<T, DP> S;
+  typedef typename AtFrag<T>::type frag_t;
+  constexpr int TQ = S::TR, NB = TQ / 32;
+  extern __shared__ __align__(16) unsigned char lds[];
+  const unsigned lds0 = (unsigned)(size_t)(CRAFT_LDS unsigned char*)lds;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
+  const int nkt = (p.Nk + 127) >> 7, G = p.H / p.Hk;
+  // part_k: one block per query head, whose results a second kernel sums over the group; else one block walks over the heads of its group
+  const int heads = p.part_k ? p.H : p.Hk;
+  const int id = xcd_chunk(blockIdx.x, gridDim.x), bx = id / nkt, kt = id - bx * nkt;       // (the first keys of a causal row are the heaviest: first)
+  const int b = bx / heads, hx = bx - b * heads, kvh = p.part_k ? hx / G : hx;
+  const int head0 = p.part_k ? hx : hx * G, head1 = p.part_k ? hx + 1 : hx * G + G;
+  const int off = p.Nk - p.Nq, j0 = kt * 128, jw = j0 + wave * 32;
+  const int prefix = p.prefix ? p.prefix[b] : 0;
+  const int key = min(jw + (lane & 31), p.Nk - 1);
+  const int first = !p.causal || key < prefix ? -0x40000000 : key - off;  // the first query that sees this key
+  const int mydoc = p.dock ? p.dock[(long)b * p.Nk + key] : 0;
+
+  frag_t kf[DP / 16], vf[DP / 16];
+  load_own<T, DP>(reinterpret_cast<const T*>(p.k) + b * p.k_b + (long)key * p.k_n + kvh * p.k_h, p.D, h, kf);
+  load_own<T, DP>(reinterpret_cast<const T*>(p.v) + b * p.v_b + (long)key * p.v_n + kvh * p.v_h, p.D, h, vf);
+
+  int t0 = !p.causal || prefix > j0 ? 0 : min(max(j0 - off, 0), p.Nq) / TQ, t1 = (p.Nq + TQ - 1) / TQ;
+  int4 kr = make_int4(0, 0, 0, 0), krw = kr;
+  const int4* rq = nullptr;
+  const int qgroups = (p.Nq + 31) >> 5;
+  if (p.rq) {
+    const int kgroups = (p.Nk + 31) >> 5;
+    const int4* rk = p.rk + (long)b * kgroups;
+    rq = p.rq + (long)b * qgroups;
+    kr = join_ranges(rk, j0 >> 5, min((j0 >> 5) + 4, kgroups) - 1);
+    krw = rk[min((j0 >> 5) + wave, kgroups - 1)];
+    tiles_of_documents<256>(rq, qgroups, NB, kr, t0, t1, tid, reinterpret_cast<int*>(lds + 2 * S::STAGE));
+  }
+  const int nchunk = p.D * (int)sizeof(T) / 16;
+  const unsigned qst = (unsigned)(p.q_n * (long)sizeof(T)), gst = (unsigned)(p.go_n * (long)sizeof(T));
+  TileCopy<T, DP, TQ, 4> qc, gc;
+  qc.init(wave, lane, qst, nchunk);
+  gc.init(wave, lane, gst, nchunk);
+  auto range = [&](int t) { return join_ranges(rq, t * NB, min(t * NB + NB, qgroups) - 1); };
+  auto next = [&](int t) { if (rq) while (t < t1 && !ranges_meet(range(t), kr)) ++t; return t; };
+  auto stage = [&](int buf, int head, int t) {
+    const int valid = p.Nq - t * TQ;
+    const unsigned at = lds0 + (unsigned)buf * S::STAGE;
+    const unsigned char* qb = reinterpret_cast<const unsigned char*>(p.q) + (b * p.q_b + head * p.q_h) * (long)sizeof(T);
+    const unsigned char* gb = reinterpret_cast<const unsigned char*>(p.go) + (b * p.go_b + head * p.go_h) * (long)sizeof(T);
+    qc.issue(qb + (long)t * TQ * qst, qst, nchunk, valid, at, wave, lane);
+    gc.issue(gb + (long)t * TQ * gst, gst, nchunk, valid, at + S::TILE, wave, lane);
+    const long row = ((long)b * p.H + head) * p.Nq;
+    if (wave == 0) copy_words(p.lse + row, (long)t * TQ, p.Nq - 1, at + 2 * S::TILE, lane);
+    if (wave == 1) copy_words(p.delta + row, (long)t * TQ, p.Nq - 1, at + 2 * S::TILE + 256, lane);
+    if (rq && wave == 2) copy_words(p.docq + (long)b * p.Nq, (long)t * TQ, p.Nq - 1, at + 2 * S::TILE + 512, lane);
+  };
+
+  f32x16 dk[DP / 32], dv[DP / 32];
+#pragma unroll
+  for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.f;
+
+  int head = head0, t = next(t0), buf = 0;
+  const int tfirst = t;
+  if (t < t1) stage(0, head, t);
+  while (t < t1) {
+    wait_copies();
+    __syncthreads();
+    int tn = next(t + 1), headn = head;
+    if (tn >= t1 && head + 1 < head1) { tn = tfirst; headn = head + 1; }
+    if (tn < t1) stage(buf ^ 1, headn, tn);
+    unsigned char* Q = lds + buf * S::STAGE;
+    unsigned char* GO = Q + S::TILE;
+    const float* lse = reinterpret_cast<const float*>(GO + S::TILE);
+    const float* delta = lse + 64;
+    const int* ids = reinterpret_cast<const int*>(delta + 64);
+    const int i0 = t * TQ;
+    bool docmask = false, skip = p.causal && prefix <= jw && i0 + TQ - 1 + off < jw;
+    if (rq) {
+      const int4 qr = range(t);
+      if (qr.z) { zero_rows<T, DP, TQ>(Q, ids, p.Nq - i0, tid, 256); zero_rows<T, DP, TQ>(GO, ids, p.Nq - i0, tid, 256); __syncthreads(); }
+      docmask = !one_document(qr, krw);
+      skip |= !ranges_meet(qr, krw);
+    }
+    if (!skip) {
+      const float slope2 = BIAS ? p.slopes[head] * 1.44269504088896f : 0.f;
+      const bool masked = docmask || i0 + TQ > p.Nq || (p.causal && i0 + off < jw + 31 && prefix < jw + 32);
+#pragma unroll
+      for (int ib = 0; ib < NB; ++ib) {
+        f32x16 x, y;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = y[r] = 0.f;
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) at_mma(tile_row<T, DP>(Q, 32 * ib + (lane & 31), ks, h), kf[ks], x);
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) at_mma(tile_row<T, DP>(GO, 32 * ib + (lane & 31), ks, h), vf[ks], y);
+        const float away = BIAS ? (float)(key - off - i0 - 32 * ib - 4 * h) : 0.f;
+        const int need = max(first, -0x20000000) - i0 - 32 * ib - 4 * h, room = p.Nq - i0 - 32 * ib - 4 * h;
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+          const f32x4 le = *reinterpret_cast<const f32x4*>(lse + 32 * ib + 8 * g + 4 * h);
+          const f32x4 de = *reinterpret_cast<const f32x4*>(delta + 32 * ib + 8 * g + 4 * h);
+          int4 di = make_int4(mydoc, mydoc, mydoc, mydoc);
+          if (docmask) di = *reinterpret_cast<const int4*>(ids + 32 * ib + 8 * g + 4 * h);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int r = 4 * g + e;
+            float th = 0.f;
+            float z = at_score<T, CAP>(p, x[r], th);
+            if constexpr (BIAS) z -= slope2 * fabsf(away - (float)acc_row(r));
+            float pr = __builtin_amdgcn_exp2f(z - le[e]);
+            float ds = pr * (y[r] - de[e]);
+            if constexpr (CAP) ds *= 1.f - th * th;
+            if (masked) {
+              const int dr = e == 0 ? di.x : e == 1 ? di.y : e == 2 ? di.z : di.w;
+              const bool see = acc_row(r) >= need && acc_row(r) < room && (!docmask || (dr == mydoc && dr >= 0));
+              pr = see ? pr : 0.f;
+              ds = see ? ds : 0.f;
+            }
+            x[r] = pr;
+            y[r] = ds;
+          }
+        }
+#pragma unroll
+        for (int s2 = 0; s2 < 2; ++s2) {
+          const frag_t pf = at_pack<T>(x, s2), sf = at_pack<T>(y, s2);
+#pragma unroll
+          for (int d = 0; d < DP / 32; ++d) {
+            at_mma(tile_col<T, DP>(GO, 32 * ib + 16 * s2, d, lane), pf, dv[d]);
+            at_mma(tile_col<T, DP>(Q, 32 * ib + 16 * s2, d, lane), sf, dk[d]);
+          }
+        }
+      }
+    }
+    t = tn;
+    head = headn;
+    buf ^= 1;
+  }
+  if (jw + (lane & 31) < p.Nk) {
+    typedef T t4 __attribute__((ext_vector_type(4)));
+    const long row = (((long)b * p.Nk + key) * heads + hx) * p.D;
+#pragma unroll
+    for (int d = 0; d < DP / 32; ++d)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        const int c = 32 * d + 8 * g + 4 * h;
+        if (c >= p.D) continue;
+        if (p.part_k) {
+          f32x4 wk, wv;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) { wk[j] = dk[d][4 * g + j] * p.scale; wv[j] = dv[d][4 * g + j]; }
+          *reinterpret_cast<f32x4*>(p.part_k + row + c) = wk;
+          *reinterpret_cast<f32x4*>(p.part_v + row + c) = wv;
+        } else {
+          t4 wk, wv;
+#pragma unroll
+          for (int j = 0; j < 4; ++j) { wk[j] = (T)(dk[d][4 * g + j] * p.scale); wv[j] = (T)dv[d][4 * g + j]; }
+          *reinterpret_cast<t4*>(reinterpret_cast<T*>(p.dk) + row + c) = wk;
+          *reinterpret_cast<t4*>(reinterpret_cast<T*>(p.dv) + row + c) = wv;
+        }
+      }
+  }
+}
+
+// the heads of a group summed in their order: [rows][G][D] fp32 -> [rows][D]
+template <typename T>
+__global__ __launch_bounds__(256) void k_attention_group_sum(const float* pk, const float* pv, T* dk, T* dv, long n4, int G, int d4) {
+  const long e = (long)blockIdx.x * 256 + threadIdx.x;
+  if (e >= n4) return;
+  const long row = e / d4;
+  const int c = (int)(e - row * d4);
+  f32x4 a = {0.f, 0.f, 0.f, 0.f}, w = a;
+  for (int g = 0; g < G; ++g) {
+    const long at = ((row * G + g) * d4 + c) * 4;
+    a += *reinterpret_cast<const f32x4*>(pk + at);
+    w += *reinterpret_cast<const f32x4*>(pv + at);
+  }
+  typedef T t4 __attribute__((ext_vector_type(4)));
+  t4 x, y;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) { x[j] = (T)a[j]; y[j] = (T)w[j]; }
+  *reinterpret_cast<t4*>(dk + e * 4) = x;
+  *reinterpret_cast<t4*>(dv + e * 4) = y;
+}
+
+template <typename T, int DP>
+int attention_bwd_launch(const AttentionParams& p, hipStream_t s) {
+  typedef BwdShape<T, DP> S;
+  const long rows = (long)p.B * p.Nq * p.H;
+  const long bq = (long)p.B * p.H * ((p.Nq + 127) / 128), bk = (long)p.B * (p.part_k ? p.H : p.Hk) * ((p.Nk + 127) / 128);
+  if (bq > 0x7fffffffL || bk > 0x7fffffffL || (rows + 15) / 16 > 0x7fffffffL) return CRAFT_ERR_UNSUPPORTED;
+  hipLaunchKernelGGL(k_attention_delta<T>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, p, const_cast<float*>(p.delta));
+  HIP_CHECK_RET(hipGetLastError());
+  auto go = [&](auto kernel, long blocks) {
+    HIP_CHECK_RET(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS));
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), S::LDS, s, p);
+    return (int)hipGetLastError();
+  };
+  int rc;
+  if (p.cap > 0.f) rc = p.slopes ? go(k_attention_dkv<T, DP, true, true>, bk) : go(k_attention_dkv<T, DP, true, false>, bk);
+  else rc = p.slopes ? go(k_attention_dkv<T, DP, false, true>, bk) : go(k_attention_dkv<T, DP, false, false>, bk);
+  if (rc) return rc;
+  if (p.part_k) {
+    const long n4 = (long)p.B * p.Nk * p.Hk * (p.D / 4);
+    if ((n4 + 255) / 256 > 0x7fffffffL) return CRAFT_ERR_UNSUPPORTED;
+    hipLaunchKernelGGL(k_attention_group_sum<T>, dim3((unsigned)((n4 + 255) / 256)), dim3(256), 0, s, p.part_k, p.part_v, reinterpret_cast<T*>(p.dk),
+                       reinterpret_cast<T*>(p.dv), n4, p.H / p.Hk, p.D / 4);
+    HIP_CHECK_RET(hipGetLastError());
+  }
+  if (p.cap > 0.f) return p.slopes ? go(k_attention_dq<T, DP, true, true>, bq) : go(k_attention_dq<T, DP, true, false>, bq);
+  return p.slopes ? go(k_attention_dq<T, DP, false, true>, bq) : go(k_attention_dq<T, DP, false, false>, bq);
+}
+
+}  // namespace craft

@@ -1,0 +1,261 @@
+// Shared pieces of the masked / capped / biased attention kernels (kernels_attention_*.hip):
+//
+//   z[i][j] = cap(scale * q_i . k_j) - slope_h * |pos_i - j|,   cap(x) = c tanh(x / c) or x,   pos_i = i + Nk - Nq
+//   p = softmax of z over the keys a query sees,   o_i = sum_j p_ij v_j
+//
+// Every kernel computes its scores as 32 x 32 MFMA blocks whose A operand comes out of LDS (rows = the tokens that a block walks over) and whose
+// B operand lies in registers (columns = the 32 tokens that a wave owns: lane & 31).  A lane then holds 16 scores of ONE of its own tokens, in
+// accumulator order -- row 8 (r >> 2) + 4 (lane >> 5) + (r & 3) of the block in register r -- which is, with no exchange between lanes, the B operand
+// of the next product over those rows: the order of a contraction is free as long as both operands use the same one, so the transposing reads of
+// the A operand simply fetch their rows in accumulator order.  Probabilities and score gradients never leave their lane's registers.
+//
+// LDS tiles are [row][DP] in the tensors' own type, 16-byte chunks swizzled within a row (tile_swz) so that both the row reads (ds_read_b128) and
+// the transposing reads (ds_read_b64_tr_b16) of a tile are free of bank conflicts.  They are filled by LDS-DMA: the copy writes LDS linearly, so the
+// swizzle is applied to the global addresses of the lanes.
+#pragma once
+#include <type_traits>
+#include "launch.hpp"
+
+namespace craft {
+
+#define CRAFT_LDS __attribute__((address_space(3)))
+typedef __fp16 at_fp16x4 __attribute__((__vector_size__(4 * sizeof(__fp16))));
+typedef __bf16 at_bf16x4 __attribute__((__vector_size__(4 * sizeof(__bf16))));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
+typedef unsigned u32x4_at __attribute__((ext_vector_type(4)));
+
+struct AttentionParams {
+  const void *q, *k, *v, *o, *go;              // o, go (gradient of o): backward only
+  void *out, *dq, *dk, *dv;
+  long q_b, q_n, q_h, k_b, k_n, k_h, v_b, v_n, v_h, o_b, o_n, o_h, go_b, go_n, go_h;   // strides in elements; the last axis is contiguous
+  int B, Nq, Nk, H, Hk, D;
+  float c2;                                    // scale * log2(e): scores are kept as powers of two
+  float ca, cap2;                              // capped: 2 scale / cap * log2(e) and cap * log2(e)
+  float scale, cap;
+  const float* slopes;                         // [H], natural units
+  const int *prefix, *docq, *dock;             // [B], [B][Nq], [B][Nk]; each may be null
+  const int4 *rq, *rk;                         // per 32 tokens: {least document, greatest document, any negative one, 0}
+  int causal;
+  float* lse;                                  // [B][H][Nq] log2 of the sum of 2^z; +inf for a query that sees nothing (so that 2^(z - lse) = 0)
+  const float* delta;                          // [B][H][Nq] sum_d go * o
+  float *part_o, *part_ml;                     // token kernel: partial results of the splits
+  int splits;
+  float *part_k, *part_v;                      // backward: per query head partial key / value gradients (null: written directly)
+};
+
+template <typename T> struct AtFrag { typedef f32x8 type; };
+template <> struct AtFrag<_Float16> { typedef f16x8 type; };
+template <> struct AtFrag<__bf16> { typedef bf16x8 type; };
+
+// D (16 rows of contraction) += A B.  fp32: eight exact 32x32x2 products; instruction j contracts element j of both lane halves.
+__device__ __forceinline__ void at_mma(const f16x8& a, const f16x8& b, f32x16& c) { c = __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ void at_mma(const bf16x8& a, const bf16x8& b, f32x16& c) { c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ void at_mma(const f32x8& a, const f32x8& b, f32x16& c) {
+#pragma unroll
+  for (int j = 0; j < 8; ++j) c = __builtin_amdgcn_mfma_f32_32x32x2f32(a[j], b[j], c, 0, 0, 0);
+}
+
+// Chunk c (16 bytes) of row r lies at slot c ^ tile_swz(r).  CPR = chunks per row.  16 consecutive rows must reach 16 different slots of the 256-byte
+// bank row (ds_read_b128), and the 64-byte segments that a transposing read takes from 4 consecutive rows must be 4 different quarters of it.
+template <int CPR>
+__device__ __forceinline__ int tile_swz(int r) {
+  if constexpr (CPR >= 16) return ((r & 3) << 2) | ((r >> 2) & 3);
+  else if constexpr (CPR == 8) return (((r >> 1) & 1) << 2) | ((r >> 2) & 3);
+  else return (r >> 2) & 3;
+}
+template <typename T, int DP> constexpr int at_cpr() { return DP * (int)sizeof(T) / 16; }
+
+// row read: 8 consecutive columns 16 ks + 8 h .. of row `row`
+template <typename T, int DP>
+__device__ __forceinline__ typename AtFrag<T>::type tile_row(const unsigned char* t, int row, int ks, int h) {
+  constexpr int CPR = at_cpr<T, DP>();
+  const int f = tile_swz<CPR>(row);
+  const unsigned char* r = t + row * (DP * (int)sizeof(T));
+  if constexpr (sizeof(T) == 2) {
+    return *reinterpret_cast<const typename AtFrag<T>::type*>(r + (((2 * ks + h) ^ f) << 4));
+  } else {
+    const f32x4 a = *reinterpret_cast<const f32x4*>(r + (((4 * ks + 2 * h) ^ f) << 4));
+    const f32x4 b = *reinterpret_cast<const f32x4*>(r + (((4 * ks + 2 * h + 1) ^ f) << 4));
+    f32x8 v;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
+    return v;
+  }
+}
+
+// transposing read: column 32 db + (lane & 31) of rows row0 + 4 h + {0..3} and row0 + 8 + 4 h + {0..3} (accumulator order), row0 a multiple of 16
+template <typename T, int DP>
+__device__ __forceinline__ typename AtFrag<T>::type tile_col(const unsigned char* t, int row0, int db, int lane) {
+  constexpr int CPR = at_cpr<T, DP>();
+  const int h = lane >> 5;
+  typename AtFrag<T>::type v;
+  if constexpr (sizeof(T) == 2) {
+    const int j = lane & 15, mh = (lane >> 4) & 1, c = 4 * db + 2 * mh + ((j & 3) >> 1);
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int row = row0 + 8 * u + 4 * h + (j >> 2);
+      const int off = row * (DP * 2) + ((c ^ tile_swz<CPR>(row)) << 4) + ((j & 1) << 3);
+      if constexpr (std::is_same<T, __bf16>::value) {
+        const at_bf16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((CRAFT_LDS at_bf16x4*)((CRAFT_LDS unsigned char*)t + off));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[4 * u + i] = x[i];
+      } else {
+        const at_fp16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4f16((CRAFT_LDS at_fp16x4*)((CRAFT_LDS unsigned char*)t + off));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) v[4 * u + i] = (_Float16)x[i];
+      }
+    }
+  } else {
+    const int col = 32 * db + (lane & 31);
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int row = row0 + 8 * u + 4 * h + i;
+        v[4 * u + i] = *reinterpret_cast<const float*>(t + row * (DP * 4) + ((((col >> 2) ^ tile_swz<CPR>(row)) << 4) | ((col & 3) << 2)));
+      }
+  }
+  return v;
+}
+
+// 8 accumulator values (registers 8 s .. 8 s + 7) as a B operand.  16-bit types: the probabilities (at most 2^8 before normalisation) and score
+// gradients are rounded to the tensors' type here, once, to nearest; their sums are taken in fp32 before the rounding.
+template <typename T>
+__device__ __forceinline__ typename AtFrag<T>::type at_pack(const f32x16& x, int s) {
+  typename AtFrag<T>::type v;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = (T)x[8 * s + j];
+  return v;
+}
+
+// the row of a 32-row block that register r of a lane holds, less 4 h
+__device__ __forceinline__ constexpr int acc_row(int r) { return 8 * (r >> 2) + (r & 3); }
+
+// a value and its partner's in the other half of the wave
+__device__ __forceinline__ float at_other_half(float x) { return __shfl_xor(x, 32); }
+
+// B operand in registers: row `row` of a [.., D] matrix, columns 16 ks + 8 h .. (zero behind D; D is a multiple of 8)
+template <typename T, int DP>
+__device__ __forceinline__ void load_own(const T* row, int D, int h, typename AtFrag<T>::type (&f)[DP / 16]) {
+#pragma unroll
+  for (int ks = 0; ks < DP / 16; ++ks) {
+    const int c = 16 * ks + 8 * h;
+    typename AtFrag<T>::type v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) v[j] = (T)0.f;
+    if (c < D) v = *reinterpret_cast<const typename AtFrag<T>::type*>(row + c);
+    f[ks] = v;
+  }
+}
+
+// LDS-DMA of ROWS rows (those from `valid` on repeat the last valid one; the chunks behind D repeat the last real one: both are only ever
+// multiplied by zeros or masked) by WAVES waves; this wave's share.  Issues only: wait for vmcnt and pass a barrier before reading.
+template <typename T, int DP, int ROWS, int WAVES>
+struct TileCopy {
+  static constexpr int CPR = at_cpr<T, DP>(), CHUNKS = ROWS * CPR, PER = CHUNKS / 64 / WAVES;
+  static_assert(CHUNKS % (64 * WAVES) == 0, "whole wave instructions");
+  unsigned voff[PER];
+  __device__ __forceinline__ static unsigned offset(int wave, int lane, int i, unsigned stride, int nchunk, int valid) {
+    const int L = (wave * PER + i) * 64 + lane, row = L / CPR, pos = L % CPR;
+    const int c = min(pos ^ tile_swz<CPR>(row), nchunk - 1);
+    return (unsigned)min(row, valid - 1) * stride + ((unsigned)c << 4);
+  }
+  __device__ __forceinline__ void init(int wave, int lane, unsigned stride, int nchunk) {
+#pragma unroll
+    for (int i = 0; i < PER; ++i) voff[i] = offset(wave, lane, i, stride, nchunk, ROWS);
+  }
+  // base: row 0 of the tile (wave-uniform); stride: bytes between rows; lds: byte address of the tile in LDS
+  __device__ __forceinline__ void issue(const unsigned char* base, unsigned stride, int nchunk, int valid, unsigned lds, int wave, int lane) const {
+    const unsigned long a = (unsigned long)base;
+    u32x4_at d;
+    d[0] = __builtin_amdgcn_readfirstlane((unsigned)a);
+    d[1] = __builtin_amdgcn_readfirstlane((unsigned)(a >> 32));
+    d[2] = 0xffffffffu;
+    d[3] = 0x00020000u;
+    if (valid >= ROWS) {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) one(d, voff[i], lds + (unsigned)(wave * PER + i) * 1024u);
+    } else {
+#pragma unroll
+      for (int i = 0; i < PER; ++i) one(d, offset(wave, lane, i, stride, nchunk, valid), lds + (unsigned)(wave * PER + i) * 1024u);
+    }
+  }
+  __device__ __forceinline__ static void one(const u32x4_at& d, unsigned v, unsigned lds) {
+    const unsigned dst = __builtin_amdgcn_readfirstlane(lds);
+    unsigned keep;
+    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+                 : "=&s"(keep) : "v"(v), "s"(dst), "s"(d) : "memory");
+  }
+};
+// 64 words base[min(first + lane, last)] -> LDS, by one wave
+__device__ __forceinline__ void copy_words(const void* base, long first, long last, unsigned lds, int lane) {
+  const unsigned long a = (unsigned long)base + 4ul * (unsigned long)first;
+  u32x4_at d;
+  d[0] = __builtin_amdgcn_readfirstlane((unsigned)a);
+  d[1] = __builtin_amdgcn_readfirstlane((unsigned)(a >> 32));
+  d[2] = 0xffffffffu;
+  d[3] = 0x00020000u;
+  const unsigned v = 4u * (unsigned)min((long)lane, last - first);
+  const unsigned dst = __builtin_amdgcn_readfirstlane(lds);
+  unsigned keep;
+  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dword %1, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
+               : "=&s"(keep) : "v"(v), "s"(dst), "s"(d) : "memory");
+}
+__device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
+
+// zero the rows of a tile whose document is negative: what lies there may be anything, and 0 * inf is not 0.  All threads; barrier behind it.
+template <typename T, int DP, int ROWS>
+__device__ __forceinline__ void zero_rows(unsigned char* t, const int* docs, int valid, int tid, int nthread) {
+  constexpr int CPR = at_cpr<T, DP>();
+  for (int c = tid; c < ROWS * CPR; c += nthread) {
+    const int row = c / CPR;
+    if (docs[min(row, valid - 1)] < 0) *reinterpret_cast<f32x4*>(t + c * 16) = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+}
+
+// a document range over 32-token groups [g0, g1] joined (wave-uniform)
+__device__ __forceinline__ int4 join_ranges(const int4* r, int g0, int g1) {
+  int4 a = r[g0];
+  for (int g = g0 + 1; g <= g1; ++g) {
+    const int4 b = r[g];
+    a.x = min(a.x, b.x); a.y = max(a.y, b.y); a.z |= b.z;
+  }
+  return a;
+}
+__device__ __forceinline__ bool ranges_meet(const int4& a, const int4& b) { return a.x <= b.y && b.x <= a.y; }
+__device__ __forceinline__ bool one_document(const int4& a, const int4& b) { return !a.z && !b.z && a.x == a.y && b.x == b.y && a.x == b.x; }
+
+// the score of a product, as a power of two; th: tanh, for the gradient.  fp32 tensors take the library's tanh (the quick form is off by 1e-7 of the cap).
+template <typename T, bool CAP>
+__device__ __forceinline__ float at_score(const AttentionParams& p, float s, float& th) {
+  if constexpr (!CAP) return s * p.c2;
+  if constexpr (std::is_same<T, float>::value) th = tanhf(s * p.scale / p.cap);
+  else th = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * p.ca) + 1.f);      // (exp2 = inf: 1;  exp2 = 0: -1)
+  return th * p.cap2;
+}
+
+// token range of a walk: the first and the last tile of [t0, t1) whose documents meet `own`, over the whole block
+template <int THREADS>
+__device__ __forceinline__ void tiles_of_documents(const int4* r, int groups, int gpt, const int4& own, int& t0, int& t1, int tid, int* red) {
+  int lo = 0x7fffffff, hi = -1;
+  for (int t = t0 + tid; t < t1; t += THREADS) {
+    const int4 a = join_ranges(r, t * gpt, min(t * gpt + gpt, groups) - 1);
+    if (ranges_meet(a, own)) { lo = min(lo, t); hi = max(hi, t); }
+  }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) { lo = min(lo, __shfl_xor(lo, o)); hi = max(hi, __shfl_xor(hi, o)); }
+  if ((tid & 63) == 0) { red[2 * (tid >> 6)] = lo; red[2 * (tid >> 6) + 1] = hi; }
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < THREADS / 64; ++w) { lo = min(lo, red[2 * w]); hi = max(hi, red[2 * w + 1]); }
+  t0 = __builtin_amdgcn_readfirstlane(lo);
+  t1 = __builtin_amdgcn_readfirstlane(hi) + 1;
+  if (t1 <= 0) t0 = t1 = 0;
+}
+
+// the launchers of each (type, padded width); `what` 0 forward, 1 single tokens, 2 gradient of q, 3 gradients of k and v
+template <typename T, int DP> int attention_fwd_launch(const AttentionParams& p, hipStream_t s);
+template <typename T, int DP> int attention_token_launch(const AttentionParams& p, hipStream_t s);
+template <typename T, int DP> int attention_bwd_launch(const AttentionParams& p, hipStream_t s);
+
+}  // namespace craft

@@ -1,0 +1,9 @@
+// _Float16 attention, head width up to 32 (attention_fwd / _token / _bwd.inc.hpp)
+#include "attention_fwd.inc.hpp"
+#include "attention_token.inc.hpp"
+#include "attention_bwd.inc.hpp"
+namespace craft {
+template int attention_fwd_launch<_Float16, 32>(const AttentionParams&, hipStream_t);
+template int attention_token_launch<_Float16, 32>(const AttentionParams&, hipStream_t);
+template int attention_bwd_launch<_Float16, 32>(const AttentionParams&, hipStream_t);
+}  // namespace craft

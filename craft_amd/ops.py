@@ -6,6 +6,7 @@ is forwarded as ``ld``).  No compute happens in Python.
 """
 from __future__ import annotations
 
+import functools
 import math
 import os
 import threading
@@ -644,3 +645,315 @@ def pack_convf1_mfma(w: torch.Tensor, prec: int) -> torch.Tensor:
     out = torch.empty(planes * round_up(co, 32) * 128, device=w.device, dtype=torch.bfloat16 if prec == hip.PREC_BF16 else torch.float16)
     call("craft_pack_weights", m, co, 128, prec, out)
     return out
+
+
+# ------------------------------------------------------------------------------------------------
+# LayerNorm with weights
+# ------------------------------------------------------------------------------------------------
+DTYPE_CODE = {torch.float32: PREC_F32, torch.bfloat16: hip.PREC_BF16, torch.float16: hip.PREC_F16}
+LAYER_NORM_MAX_WIDTH = 16384
+
+
+def _on_device(*tensors):
+    """The tensors' common device (their own: kernels are enqueued on ITS current stream, whichever device is current)."""
+    dev = tensors[0].device
+    for t in tensors:
+        if t is not None and t.device != dev:
+            raise hip.CraftHipError(f"tensors on different devices: {dev} and {t.device}")
+    if dev.type != "cuda":
+        raise hip.CraftHipError("craft_amd HIP ops need device tensors (no CPU fallback)")
+    return dev
+
+
+def _norm_rows(x: torch.Tensor):
+    """(x as rows of one stride, the stride): x itself where its leading axes are one run of rows, else a copy."""
+    C = x.shape[-1]
+    if x.dim() == 1:
+        return (x, C) if x.stride(0) == 1 or C == 1 else (x.contiguous(), C)
+    if x.stride(-1) == 1 or C == 1:
+        lead = [(n, st) for n, st in zip(x.shape[:-1], x.stride()[:-1]) if n != 1]
+        if not lead:
+            return x, C
+        if all(a[1] == b[0] * b[1] for a, b in zip(lead, lead[1:])):
+            return x, lead[-1][1]
+    return x.contiguous(), C
+
+
+def _check_layer_norm(x, weight, bias, eps):
+    if x.dtype not in DTYPE_CODE:
+        raise hip.CraftHipError(f"layer_norm: fp32, fp16 or bf16 rows, not {x.dtype}")
+    if x.dim() < 1 or not 1 <= x.shape[-1] <= LAYER_NORM_MAX_WIDTH:
+        raise hip.CraftHipError(f"layer_norm: a last axis of 1 .. {LAYER_NORM_MAX_WIDTH}, not {tuple(x.shape)}")
+    if not eps >= 0:
+        raise hip.CraftHipError("layer_norm: eps must not be negative")
+    wt = None
+    for t, name in ((weight, "weight"), (bias, "bias")):
+        if t is None:
+            continue
+        if t.shape != x.shape[-1:] or t.dtype not in (x.dtype, torch.float32):
+            raise hip.CraftHipError(f"layer_norm: {name} must be [{x.shape[-1]}] of {x.dtype} or fp32, not {tuple(t.shape)} of {t.dtype}")
+        if wt is not None and t.dtype != wt:
+            raise hip.CraftHipError("layer_norm: weight and bias must have one type")
+        wt = t.dtype
+    _on_device(x, weight, bias)
+    return wt or x.dtype
+
+
+def _layer_norm(x, weight, bias, eps, out, stats: bool):
+    wt = _check_layer_norm(x, weight, bias, eps)
+    C = x.shape[-1]
+    rows = x.numel() // C
+    if out is None:
+        out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+        raise hip.CraftHipError("layer_norm: out must be of x's shape, type and device")
+    y, ldy = _norm_rows(out)
+    if y.data_ptr() != out.data_ptr() or (rows > 1 and ldy < C):
+        raise hip.CraftHipError("layer_norm: out must be one run of rows with contiguous channels")
+    mean = rstd = None
+    if stats:
+        mean, rstd = torch.empty(2, rows, device=x.device, dtype=torch.float32)
+    if rows:
+        xr, ldx = _norm_rows(x)
+        w, b = (None if t is None else t.contiguous() for t in (weight, bias))
+        with torch.cuda.device(x.device):
+            call("craft_layer_norm_fwd", xr, ldx, w, b, rows, C, float(eps), DTYPE_CODE[x.dtype], DTYPE_CODE[wt], y, ldy if rows > 1 else C, mean, rstd)
+    return out, mean, rstd
+
+
+def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
+               out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """LayerNorm over the last axis (width up to 16384) of fp32 / fp16 / bf16 rows; weight and bias [C] of the rows' type or fp32, each optional.
+    Statistics in fp32, the result rounded once to x's type.  ``tokens_norm`` is the weightless fp32 form of the model's tokens; the differentiable
+    form is ``autograd.layer_norm``."""
+    with torch.no_grad():
+        return _layer_norm(x, weight, bias, eps, out, False)[0]
+
+
+def layer_norm_bwd(x: torch.Tensor, weight: Optional[torch.Tensor], bias_type: Optional[torch.dtype], dy: torch.Tensor, mean: torch.Tensor,
+                   rstd: torch.Tensor, need=(True, True, True)):
+    """(dx, dweight, dbias) of ``layer_norm`` from its saved row statistics; ``need`` leaves gradients out."""
+    C = x.shape[-1]
+    rows = x.numel() // C
+    wt = weight.dtype if weight is not None else bias_type or x.dtype
+    new = lambda want, shape, t: torch.empty(shape, device=x.device, dtype=t) if want else None      # noqa: E731
+    dx, dw, db = new(need[0], x.shape, x.dtype), new(need[1], (C,), wt), new(need[2], (C,), wt)
+    if not rows:
+        return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
+    xr, ldx = _norm_rows(x)
+    g, ldg = _norm_rows(dy.to(x.dtype))
+    # the block's share of the rows: as many blocks as rows (a block takes 1024 / 256 / 16 rows at a time only at small widths), at most 4 for
+    # each compute unit -- more partial sums cost more than they hide
+    blocks = min(rows, 1024)
+    ws = torch.empty(blocks * 2 * C, device=x.device, dtype=torch.float32) if need[1] or need[2] else None
+    with torch.cuda.device(x.device):
+        call("craft_layer_norm_bwd", xr, ldx, g, ldg if rows > 1 else C, None if weight is None else weight.contiguous(), mean, rstd, rows, C,
+             DTYPE_CODE[x.dtype], DTYPE_CODE[wt], dx, C, dw, db, ws, blocks)
+    return dx, dw, db
+
+
+# ------------------------------------------------------------------------------------------------
+# orthogonalisation of updates
+# ------------------------------------------------------------------------------------------------
+NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)        # the quintic that takes (0, 1] near 1 in 5 steps
+ORTHOGONALIZE_MAX_SIDE = 32768                   # the smaller side of a matrix
+_ORTHOGONALIZE_JOBS = 60                         # matrices of one set of launches
+
+
+@functools.lru_cache(maxsize=64)
+def _newton_schulz_scales(coeffs):
+    """Powers of two that bring the operands of the products just below fp16's largest number: a matrix' entries are bounded by its largest singular
+    value, and those follow the polynomial from [0, 1]."""
+    g = [i / 4096 for i in range(4097)]
+    top = [1.0, 1.0, 1e-3]
+    for a, b, c in coeffs:
+        q = [b * x * x + c * x ** 4 for x in g]
+        top = [max(top[0], *map(abs, g)), max(top[1], *(x * x for x in g)), max(top[2], *map(abs, q))]
+        g = [a * x + y * x for x, y in zip(g, q)]
+        if not max(map(abs, g)) <= 100.0:
+            raise hip.CraftHipError(f"orthogonalize: coefficients {coeffs} let singular values grow without bound")
+    return tuple(2.0 ** math.floor(math.log2(48000.0 / t)) for t in top)
+
+
+def _newton_schulz_coeffs(steps, coeffs):
+    flat = all(isinstance(c, (int, float)) for c in coeffs)
+    rows = [tuple(float(x) for x in coeffs)] * steps if flat else [tuple(float(x) for x in c) for c in coeffs]
+    if steps != len(rows) or not 1 <= steps <= 64 or any(len(r) != 3 or not all(math.isfinite(x) for x in r) for r in rows):
+        raise hip.CraftHipError("orthogonalize: coeffs are three finite numbers, or three for each of 1 .. 64 steps")
+    return tuple(rows)
+
+
+def orthogonalize(mats: Sequence[torch.Tensor], steps: int = 5, coeffs=NEWTON_SCHULZ, eps: float = 1e-7, out: Optional[Sequence[torch.Tensor]] = None):
+    """Every matrix of the list with its singular values moved towards 1: X = G / (|G|_F + eps), then ``steps`` times X <- a X + (b A + c A A) X with
+    A = X X^T from the smaller side.  ``coeffs``: (a, b, c), or one triple a step.  fp32 / fp16 / bf16 matrices of any strides, the smaller side up to
+    32768; fp32-class arithmetic whatever the type, one rounding at the end.  The whole list shares its launches.  ``out`` (may be ``mats``): where the
+    results go.  ``train.FlatMuon`` is the optimizer that uses it."""
+    rows = _newton_schulz_coeffs(steps, coeffs)
+    scales = _newton_schulz_scales(rows)
+    if not 0 <= eps < float("inf"):
+        raise hip.CraftHipError("orthogonalize: eps must be finite and not negative")
+    mats = list(mats)
+    for g in mats:
+        if g.dim() != 2 or g.dtype not in DTYPE_CODE:
+            raise hip.CraftHipError(f"orthogonalize: fp32, fp16 or bf16 matrices, not {list(g.shape)} of {g.dtype}")
+        if min(g.shape) > ORTHOGONALIZE_MAX_SIDE or max(g.shape) > 1 << 24:
+            raise hip.CraftHipError(f"orthogonalize: {list(g.shape)}: the smaller side up to {ORTHOGONALIZE_MAX_SIDE}, the larger up to 2^24")
+    if out is None:
+        out = [torch.empty(g.shape, device=g.device, dtype=g.dtype) for g in mats]
+    else:
+        out = list(out)
+        if len(out) != len(mats) or any(o.shape != g.shape or o.dtype != g.dtype or o.device != g.device for o, g in zip(out, mats)):
+            raise hip.CraftHipError("orthogonalize: out must be a list of the matrices' shapes, types and devices")
+        if any(o.numel() and (o.stride(1) != 1 and o.shape[1] > 1 or o.stride(0) < o.shape[1] and o.shape[0] > 1) for o in out):
+            raise hip.CraftHipError("orthogonalize: out needs contiguous columns")
+    if not mats:
+        return out
+    device = _on_device(*mats)
+    import ctypes
+    flat = hip.carray(ctypes.c_float, [x for r in rows for x in r])
+    with torch.no_grad(), torch.cuda.device(device):
+        for code in sorted({DTYPE_CODE[g.dtype] for g in mats}):
+            todo = [(g, o) for g, o in zip(mats, out) if DTYPE_CODE[g.dtype] == code and g.numel()]
+            for i in range(0, len(todo), _ORTHOGONALIZE_JOBS):
+                jobs, keep, nbytes = [], [], 0
+                for g, o in todo[i:i + _ORTHOGONALIZE_JOBS]:
+                    if (g.stride(1) != 1 and g.shape[1] > 1) or g.stride(0) < 0:
+                        g = g.contiguous()
+                        keep.append(g)
+                    m, k = (round_up(x, 64) for x in sorted(g.shape))
+                    nbytes += 256 + 12 * m * k + 8 * m * m
+                    jobs += [g.data_ptr(), g.stride(0), o.data_ptr(), max(o.stride(0), o.shape[1]), *g.shape]
+                ws = torch.empty(nbytes, device=device, dtype=torch.uint8)
+                call("craft_orthogonalize", hip.carray(ctypes.c_long, jobs), len(jobs) // 6, flat, steps, float(eps), *scales, code, ws, nbytes)
+    return out
+
+
+# ------------------------------------------------------------------------------------------------
+# attention with a cap, a distance bias and causal / prefix / document masks
+# ------------------------------------------------------------------------------------------------
+def _strided(t: torch.Tensor) -> torch.Tensor:
+    """t itself where the kernels can read it in place: contiguous head width, 16-byte steps, rows less than 16 MiB apart; else a copy."""
+    step = 16 // t.element_size()
+    ok = (t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or (s >= 0 and s % step == 0) for n, s in zip(t.shape[:3], t.stride()))
+          and (t.shape[1] == 1 or t.stride(1) * t.element_size() < 1 << 24))
+    return t if ok else t.contiguous()
+
+
+def _strides(t: torch.Tensor):
+    return [0 if n == 1 else s for n, s in zip(t.shape[:3], t.stride())]
+
+
+class AttentionPlan:
+    """The checked arguments of one attention call."""
+
+    def __init__(self, q, k, v, scale, cap, slopes, causal, prefix, docs, docs_k):
+        err = hip.CraftHipError
+        if q.dim() != 4 or k.dim() != 4 or v.dim() != 4:
+            raise err("attention: q, k, v are [batch, tokens, heads, width]")
+        if q.dtype not in DTYPE_CODE or k.dtype != q.dtype or v.dtype != q.dtype:
+            raise err(f"attention: q, k, v of one type, fp32, fp16 or bf16, not {q.dtype}, {k.dtype}, {v.dtype}")
+        B, Nq, H, D = q.shape
+        Nk, Hk = k.shape[1:3]
+        if k.shape != (B, Nk, Hk, D) or v.shape != k.shape:
+            raise err(f"attention: shapes {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)} do not fit")
+        if H < 1 or Hk < 1 or H % Hk:
+            raise err(f"attention: {H} query heads are no multiple of {Hk} key heads")
+        if D % 8 or not 8 <= D <= 128:
+            raise err(f"attention: a head width that is a multiple of 8, up to 128, not {D}")
+        if not 0 <= float(cap) <= 1e30:
+            raise err("attention: cap must be positive, or 0 for none")
+        scale = D ** -0.5 if scale is None else float(scale)
+        if not abs(scale) <= 1e30:
+            raise err("attention: scale must be finite")
+        if prefix is not None and not causal:
+            raise err("attention: a prefix opens a causal mask: pass causal=True")
+        if slopes is not None and (slopes.shape != (H,) or slopes.dtype != torch.float32):
+            raise err(f"attention: slopes must be [{H}] of fp32")
+        if slopes is not None and slopes.requires_grad and torch.is_grad_enabled():
+            raise err("attention: slopes have no gradient here")
+        if docs is None and docs_k is not None:
+            raise err("attention: docs_k needs docs")
+        if docs is not None and docs_k is None:
+            if Nq != Nk:
+                raise err("attention: docs alone serves q and k of one length; pass docs_k too")
+            docs_k = docs
+        for t, shape, name in ((prefix, (B,), "prefix"), (docs, (B, Nq), "docs"), (docs_k, (B, Nk), "docs_k")):
+            if t is not None and (t.shape != shape or t.dtype != torch.int32):
+                raise err(f"attention: {name} must be {list(shape)} of int32, not {list(t.shape)} of {t.dtype}")
+        if max(B, Nq, Nk) >= 1 << 29:
+            raise err("attention: sizes below 2^29")
+        self.device = _on_device(q, k, v, slopes, prefix, docs, docs_k)
+        self.dims = (B, Nq, Nk, H, Hk, D)
+        self.q, self.k, self.v = _strided(q), _strided(k), _strided(v)
+        self.scale, self.cap, self.causal = scale, float(cap), int(bool(causal))
+        self.slopes, self.prefix, self.docs, self.docs_k = (None if t is None else t.contiguous() for t in (slopes, prefix, docs, docs_k))
+        self.code = DTYPE_CODE[q.dtype]
+
+    def range_bytes(self) -> int:
+        B, Nq, Nk = self.dims[:3]
+        return 0 if self.docs is None else 16 * B * ((Nq + 31) // 32 + (Nk + 31) // 32)
+
+    def new(self, nbytes: int) -> Optional[torch.Tensor]:
+        return torch.empty(nbytes, device=self.device, dtype=torch.uint8) if nbytes else None
+
+    def shape(self, *more):
+        import ctypes
+        return hip.carray(ctypes.c_long, [*self.dims] + [s for t in (self.q, self.k, self.v, *more) for s in _strides(t)])
+
+    def masks(self):
+        return self.slopes, self.prefix, self.docs, self.docs_k
+
+    def splits(self) -> int:
+        """0: blocks of 128 queries.  A few query rows (the tokens times the query heads of a key head) take the single-token kernel, whose keys are
+        split over so many blocks: two for each compute unit in all, a split at least 256 keys."""
+        B, Nq, Nk, H, Hk, D = self.dims
+        rows = Nq * (H // Hk)
+        if rows > 64:
+            return 0
+        return max(1, min(512 // (B * Hk * ((rows + 31) // 32)), (Nk + 255) // 256))
+
+    def forward(self, out: torch.Tensor, lse: Optional[torch.Tensor]):
+        B, Nq, Nk, H, Hk, D = self.dims
+        splits = 0 if lse is not None else self.splits()
+        nbytes = self.range_bytes() if not splits else 4 * B * Nq * H * splits * (D + 2) if splits > 1 else 0
+        with torch.cuda.device(self.device):
+            call("craft_attention_fwd", self.q, self.k, self.v, self.shape(out), *self.masks(), self.scale, self.cap, self.causal, self.code, splits, out,
+                 lse, self.new(nbytes), nbytes)
+
+    def backward(self, out: torch.Tensor, lse: torch.Tensor, go: torch.Tensor):
+        B, Nq, Nk, H, Hk, D = self.dims
+        go = _strided(go.to(self.q.dtype))
+        dq = torch.empty(B, Nq, H, D, device=self.device, dtype=self.q.dtype)
+        dk, dv = torch.empty(2, B, Nk, Hk, D, device=self.device, dtype=self.q.dtype)
+        # key / value gradients of shared heads: one block walks over the group's heads, unless that leaves compute units without a block
+        split_group = int(H > Hk and B * Hk * ((Nk + 127) // 128) < 512)
+        nbytes = self.range_bytes() + (4 * B * H * Nq + 15) // 16 * 16 + split_group * 8 * B * Nk * H * D
+        with torch.cuda.device(self.device):
+            call("craft_attention_bwd", self.q, self.k, self.v, out, lse, go, self.shape(out, go), *self.masks(), self.scale, self.cap, self.causal, self.code,
+                 split_group, dq, dk, dv, self.new(nbytes), nbytes)
+        return dq, dk, dv
+
+
+def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optional[float] = None, cap: float = 0.0, slopes: Optional[torch.Tensor] = None,
+              causal: bool = False, prefix: Optional[torch.Tensor] = None, docs: Optional[torch.Tensor] = None, docs_k: Optional[torch.Tensor] = None,
+              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """softmax(z) v over the keys each query sees, z = cap tanh(scale q k / cap) - slope_h |pos_i - j|.
+
+    q [B, Nq, H, D]; k, v [B, Nk, Hk, D] of the same type (fp32, fp16, bf16), H a multiple of Hk (query head h reads key head h // (H / Hk)), D a multiple
+    of 8 up to 128; any strides (views the kernels cannot read in place are copied).  Query i stands at position i + Nk - Nq: new tokens at the end of a
+    cache.  scale: 1 / sqrt(D) by default; cap 0: none; slopes [H] fp32.  ``causal``: keys up to the query's position, and with ``prefix`` [B] int32 also
+    the first prefix[b] keys.  ``docs`` [B, Nq] (and ``docs_k`` [B, Nk]) int32: only keys of the query's document; a negative document is padding, which
+    nothing sees and whose rows of q, k, v may hold anything.  A query that sees nothing gives zeros.  Softmax sums and products accumulate in fp32;
+    16-bit types round the probabilities to their own type for the product with v.  ``flash_attention`` and ``attn_probs`` are the model's own forms over
+    an image's tokens; the differentiable form is ``autograd.attention``."""
+    with torch.no_grad():
+        plan = AttentionPlan(q, k, v, scale, cap, slopes, causal, prefix, docs, docs_k)
+        if out is None:
+            out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
+        elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or _strided(out) is not out:
+            raise hip.CraftHipError("attention: out must be of q's shape, type and device, with 16-byte aligned rows")
+        if out.numel() and not k.shape[1]:
+            return out.zero_()
+        if out.numel():
+            plan.forward(out, None)
+        return out

@@ -281,10 +281,7 @@ class FlatAdamW:
         call("craft_sumsq", self.flat_grad, self.numel, self._sumsq)
         call("craft_loss_scale_update", self._sumsq, self._scaler, float(grad_mul), float(max_norm), float(self.betas[0]), float(self.betas[1]),
              float(self.growth), float(self.backoff), int(self.growth_interval))
-        for a, b in self.segments:
-            call("craft_adamw_step_dyn", self.flat[a:b], self.flat_grad[a:b], self.exp_avg[a:b], self.exp_avg_sq[a:b], b - a,
-                 float(self.lr if lr is None else lr), float(self.betas[0]), float(self.betas[1]), float(self.eps),
-                 float(self.weight_decay), self._scaler)
+        self._apply_update(float(self.lr if lr is None else lr))
         if self.flat.is_cuda:              # asynchronous read-back of the record (pinned buffer + event): metrics / logs, never the step
             self._snap.copy_(self._scaler, non_blocking=True)
             self._snap_event = torch.cuda.Event()
@@ -292,6 +289,14 @@ class FlatAdamW:
         # the kernel wrote through raw pointers: p._version / data_ptr() did not move, so tell the packed-weight caches
         from .hip import bump_weights_epoch
         bump_weights_epoch()
+
+    def _apply_update(self, lr: float):
+        self._adamw(self.segments, lr)
+
+    def _adamw(self, segments, lr: float):
+        for a, b in segments:
+            call("craft_adamw_step_dyn", self.flat[a:b], self.flat_grad[a:b], self.exp_avg[a:b], self.exp_avg_sq[a:b], b - a, lr, float(self.betas[0]),
+                 float(self.betas[1]), float(self.eps), float(self.weight_decay), self._scaler)
 
     def _check_views(self):
         """model.zero_grad(set_to_none=True), model.to(...) or p.grad = ... silently detach parameters / gradients from the
@@ -324,11 +329,80 @@ class FlatAdamW:
             n = p.numel()
             st = sd["state"].get(i)
             if st is not None:
+                if "exp_avg" not in st:
+                    raise ValueError(f"FlatAdamW: the state of parameter {i} is another optimizer's ({', '.join(map(str, st))})")
                 self.exp_avg[off:off + n].copy_(st["exp_avg"].reshape(-1))
                 self.exp_avg_sq[off:off + n].copy_(st["exp_avg_sq"].reshape(-1))
                 self.step_count = int(float(st["step"]))
         g = sd["param_groups"][0]
         self.lr, self.betas, self.eps, self.weight_decay = g["lr"], tuple(g["betas"]), g["eps"], g["weight_decay"]
+
+
+class FlatMuon(FlatAdamW):
+    """Momentum whose matrices are orthogonalised before they are applied (ops.orthogonalize), over ``FlatAdamW``'s flat buffers and loss scaling:
+
+        buf = momentum buf + g;   u = g + momentum buf (Nesterov) or buf;   p = (1 - lr wd) p - lr s O(u),   s = match_rms sqrt(max(rows, cols))
+
+    for every parameter that is a matrix of at least ``matrix_min`` rows and columns once its trailing axes are flattened (a convolution's
+    [cout, cin KH KW]); AdamW for the others (biases, norms, position tables, one-channel heads).  An orthogonal matrix of r rows and c columns has entries of
+    rms 1 / sqrt(max(r, c)): s brings them to ``match_rms``, about that of an AdamW update, so that one learning rate serves both.  The momentum of a
+    matrix lives in its range of ``exp_avg``; its range of ``exp_avg_sq`` is not used.  Every data-parallel rank orthogonalises the same summed
+    gradient with the same bits (no atomics)."""
+
+    def __init__(self, params: Iterable[torch.nn.Parameter], lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
+                 unused: Iterable[torch.nn.Parameter] = (), momentum: float = 0.95, nesterov: bool = True, ns_steps: int = 5, matrix_min: int = 16,
+                 match_rms: float = 0.2):
+        super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, unused=unused)
+        if not 0 <= momentum < 1:
+            raise ValueError("FlatMuon: momentum must be in [0, 1)")
+        self.momentum, self.nesterov, self.ns_steps, self.match_rms = momentum, nesterov, ns_steps, match_rms
+        skip = set(self.unused_index)
+        self.matrix_index = [i for i, p in enumerate(self.params)
+                             if i not in skip and p.dim() >= 2 and min(p.shape[0], p.numel() // max(1, p.shape[0])) >= matrix_min]
+        matrices = set(self.matrix_index)
+        self.adam_segments, start = [], 0
+        for i, (p, off) in enumerate(zip(self.params, self.offsets)):      # FlatAdamW.segments without the matrices' ranges
+            if i in skip or i in matrices:
+                if off > start:
+                    self.adam_segments.append((start, off))
+                start = off + p.numel()
+        if self.numel > start:
+            self.adam_segments.append((start, self.numel))
+        self._update = torch.zeros_like(self.flat) if self.matrix_index else None
+        self._segs = [(self.offsets[i], self.params[i].numel()) for i in self.matrix_index]
+        self._mats = [self._update[off:off + n].view(self.params[i].shape[0], -1) for i, (off, n) in zip(self.matrix_index, self._segs)]
+
+    def _apply_update(self, lr: float):
+        import ctypes
+
+        from . import ops
+        from .hip import carray
+        self._adamw(self.adam_segments, lr)
+        if not self.matrix_index:
+            return
+        segs, n = carray(ctypes.c_long, [x for s in self._segs for x in s]), len(self._segs)
+        scales = carray(ctypes.c_float, [self.match_rms * math.sqrt(max(m.shape)) for m in self._mats])
+        call("craft_muon_momentum", self.flat_grad, self.exp_avg, self._update, segs, n, float(self.momentum), int(self.nesterov), self._scaler)
+        ops.orthogonalize(self._mats, steps=self.ns_steps, out=self._mats)
+        call("craft_muon_apply", self.flat, self._update, segs, scales, n, lr, float(self.weight_decay), self._scaler)
+
+    def state_dict(self) -> Dict:
+        sd = super().state_dict()
+        for i in self.matrix_index:
+            st = sd["state"][i]
+            sd["state"][i] = {"step": st["step"], "momentum_buffer": st["exp_avg"]}
+        sd["param_groups"][0].update(momentum=self.momentum, nesterov=self.nesterov, ns_steps=self.ns_steps, match_rms=self.match_rms,
+                                     matrices=list(self.matrix_index))
+        return sd
+
+    def load_state_dict(self, sd: Dict):
+        g = sd["param_groups"][0]
+        if g.get("matrices") != self.matrix_index:
+            raise ValueError("FlatMuon: the state is another optimizer's, or of a model with other matrices")
+        as_adam = {i: {"step": st["step"], "exp_avg": st["momentum_buffer"], "exp_avg_sq": torch.zeros_like(st["momentum_buffer"])}
+                   if "momentum_buffer" in st else st for i, st in sd["state"].items()}
+        super().load_state_dict({"state": as_adam, "param_groups": sd["param_groups"]})
+        self.momentum, self.nesterov, self.ns_steps, self.match_rms = g["momentum"], g["nesterov"], g["ns_steps"], g["match_rms"]
 
 
 def _broadcast(t: torch.Tensor, src: int, group=None):
@@ -366,10 +440,15 @@ def unused_parameters(model: torch.nn.Module) -> List[torch.nn.Parameter]:
     return out
 
 
-def fetch_optimizer(model: torch.nn.Module, lr: float, wdecay: float, epsilon: float, num_steps: int):
+OPTIMIZERS = {"adamw": FlatAdamW, "muon": FlatMuon}
+
+
+def fetch_optimizer(model: torch.nn.Module, lr: float, wdecay: float, epsilon: float, num_steps: int, optimizer: str = "adamw"):
     """train.py:76-85: AdamW(lr, weight_decay, eps) + OneCycleLR(max_lr=lr, total_steps=num_steps+100, pct_start=0.05,
-    linear anneal, no momentum cycling)."""
-    opt = FlatAdamW(model.parameters(), lr=lr, weight_decay=wdecay, eps=epsilon, unused=unused_parameters(model))
+    linear anneal, no momentum cycling).  ``optimizer="muon"``: FlatMuon under the same schedule."""
+    if optimizer not in OPTIMIZERS:
+        raise ValueError(f"optimizer {optimizer!r}: one of {', '.join(OPTIMIZERS)}")
+    opt = OPTIMIZERS[optimizer](model.parameters(), lr=lr, weight_decay=wdecay, eps=epsilon, unused=unused_parameters(model))
     return opt, OneCycleLR(lr, num_steps + 100, pct_start=0.05)
 
 
@@ -405,16 +484,16 @@ class Trainer:
     un-scaled norm).  A non-finite gradient skips the update exactly like GradScaler.step: weights, moments and the optimizer's step
     count stay (the LR schedule advances, as in train.py:236-237), the skip is counted (``metrics['skipped_steps']``) and a dynamic
     scale backs off.  The scale, the counters and the decision live in a device record (FlatAdamW._scaler); the host reads them back
-    asynchronously for the metrics only."""
+    asynchronously for the metrics only.  ``optimizer``: "adamw" (the reference's) or "muon" (FlatMuon)."""
 
     def __init__(self, model: torch.nn.Module, lr: float = 4e-4, wdecay: float = 1e-4, epsilon: float = 1e-8, num_steps: int = 100000,
                  clip: float = 1.0, gamma: float = 0.8, iters: int = 12, add_noise: bool = False, freeze_bn: bool = False, group=None,
-                 reference_loss_scaling: bool = False, loss_scale="auto"):
+                 reference_loss_scaling: bool = False, loss_scale="auto", optimizer: str = "adamw"):
         self.model = model
         self.loss_scale = loss_scale
         if getattr(model, "args", None) is not None:      # fp16 operand roles are legal under the loss scale (train_forward.training_precision)
             model.args.hip_loss_scaled = loss_scale == "auto" or bool(loss_scale and float(loss_scale) > 1.0)
-        self.optimizer, self.scheduler = fetch_optimizer(model, lr, wdecay, epsilon, num_steps)
+        self.optimizer, self.scheduler = fetch_optimizer(model, lr, wdecay, epsilon, num_steps, optimizer)
         self.clip, self.gamma, self.iters, self.add_noise, self.freeze_bn, self.group = clip, gamma, iters, add_noise, freeze_bn, group
         self.reference_loss_scaling = reference_loss_scaling
         self.total_steps = 0

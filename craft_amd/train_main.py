@@ -43,6 +43,8 @@ def parse(argv=None) -> argparse.Namespace:
     ap.add_argument("--hip_precision", default=None)
     ap.add_argument("--wdecay", type=float, default=0.00005)
     ap.add_argument("--epsilon", type=float, default=1e-8)
+    # (not a flag of the reference: "muon" orthogonalises the momentum of every weight matrix, train.FlatMuon)
+    ap.add_argument("--optimizer", default="adamw", choices=["adamw", "muon"])
     ap.add_argument("--clip", type=float, default=1.0)
     ap.add_argument("--gamma", type=float, default=0.8)
     ap.add_argument("--add_noise", action="store_true")
@@ -157,7 +159,7 @@ def main(argv=None) -> Optional[str]:
     model = CRAFT(default_args(**over)).to(dev)
     freeze = ns.freeze_bn and ns.stage != "chairs"                    # train.py:196-197
     tr = Trainer(model, lr=ns.lr, wdecay=ns.wdecay, epsilon=ns.epsilon, num_steps=ns.num_steps, clip=ns.clip, gamma=ns.gamma, iters=ns.iters,
-                 add_noise=ns.add_noise, freeze_bn=freeze)
+                 add_noise=ns.add_noise, freeze_bn=freeze, optimizer=ns.optimizer)
     log = {"total_steps": 0, "val_steps": [], "val_results": {}}
     if ns.restore_ckpt:
         msg, saved = load_checkpoint(ns.restore_ckpt, model, tr.optimizer, tr.scheduler, ns.load_optimizer_state, ns.load_scheduler_state,

@@ -650,6 +650,52 @@ int craft_convex_upsample(const float* mask, const float* flow, int B, int H8, i
 int craft_coords_init(const float* flow_init_nchw, int B, int H8, int W8, float* coords0, float* coords1,
                       float* flow, void* stream);
 
+/* ---- LayerNorm with weights, attention under masks, biases and a cap, orthogonalisation -------------------------------------------
+ * dtype / wdtype: CRAFT_PREC_F32, _BF16 or _F16, the type of the tensors themselves (statistics and sums are fp32). */
+
+/* y = (x - mean) / sqrt(var + eps) * w + b over the last axis, rows of any stride (ldx, ldy in elements, channels contiguous, any alignment),
+ * 1 <= C <= 16384.  w, b: [C] of wdtype (the rows' type or fp32), either may be NULL.  mean, rstd: [rows] for the backward pass, both or neither.
+ * x == y (same stride) is allowed. */
+int craft_layer_norm_fwd(const void* x, long ldx, const void* w, const void* b, long rows, int C, float eps, int dtype, int wdtype, void* y, long ldy,
+                         float* mean, float* rstd, void* stream);
+/* its gradients; dx (rows' type), dw, db (wdtype) may each be NULL.  `blocks` blocks share the rows; ws: blocks * 2 * C floats when dw or db is wanted
+ * (their partial sums, joined in a fixed order).  lddy may be 0 (one gradient row for all). */
+int craft_layer_norm_bwd(const void* x, long ldx, const void* dy, long lddy, const void* w, const float* mean, const float* rstd, long rows, int C,
+                         int dtype, int wdtype, void* dx, long lddx, void* dw, void* db, float* ws, int blocks, void* stream);
+
+/* o_i = sum_j softmax_j(cap tanh(scale q_i . k_j / cap) - slope_h |pos_i - j|) v_j over the keys j that query i sees, pos_i = i + Nk - Nq.
+ *   causal: j <= pos_i, or j < prefix[b] (prefix: [B], NULL: none; needs causal);   doc_q [B][Nq], doc_k [B][Nk] (both or NULL): doc_k[j] == doc_q[i] >= 0.
+ *   A query that sees nothing gives 0.  Rows of q, k, v whose document is negative may hold anything (inf and NaN included); every other value must be finite.
+ *   cap 0: no cap;  slopes: [H] fp32, NULL: no bias.
+ * shape: 18 host longs B, Nq, Nk, H, Hk, D, then the (batch, token, head) strides in elements of q, k, v, out.  H % Hk == 0 (query head h reads key head
+ * h / (H / Hk)), D % 8 == 0, D <= 128, strides multiples of 16 bytes, pointers 16-byte aligned, the last axis contiguous.
+ * splits 0: blocks of 128 queries, whose log2-sums go to lse ([B][H][Nq], NULL: not wanted; +inf where nothing is seen).  splits >= 1: for a few rows
+ * (Nq * H / Hk up to about 64): the keys split over so many blocks; no lse.
+ * ws (16-byte aligned): splits 0 with documents: 16 * B * (ceil(Nq / 32) + ceil(Nk / 32)) bytes;  splits > 1: B * Nq * H * splits * (D + 2) floats. */
+int craft_attention_fwd(const void* q, const void* k, const void* v, const long* shape, const float* slopes, const int* prefix, const int* doc_q,
+                        const int* doc_k, float scale, float cap, int causal, int dtype, int splits, void* out, float* lse, void* ws, long ws_bytes, void* stream);
+/* gradients of q [B][Nq][H][D], k and v [B][Nk][Hk][D], contiguous.  shape: 21 host longs, as above with the strides of grad_out last.
+ * split_group 1: a block per query head for the key / value gradients and a sum over the heads of a group behind it (more blocks, fp32 partial results).
+ * ws (16-byte aligned): the documents' ranges as above, then B * H * Nq floats rounded up to 16 bytes, then with split_group 2 * B * Nk * H * D floats.
+ * The result does not depend on the order in which blocks run. */
+int craft_attention_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse, const void* grad_out, const long* shape,
+                        const float* slopes, const int* prefix, const int* doc_q, const int* doc_k, float scale, float cap, int causal, int dtype,
+                        int split_group, void* dq, void* dk, void* dv, void* ws, long ws_bytes, void* stream);
+
+/* A list of matrices orthogonalised: X = G / (|G|_F + eps), then `steps` times X <- a X + (b A + c A A) X with A = X X^T (from the smaller side).
+ * jobs: n x 6 host longs {src, ld_src, dst, ld_dst, rows, cols} (device pointers; strides in elements, columns contiguous; dst may be src), n <= 60,
+ * min(rows, cols) <= 32768.  coeffs: steps x {a, b, c}.  The products are fp32-class: operands in two fp16 planes of the value times s_x (X), s_a (A),
+ * s_b (b A + c A A), powers of two that keep every entry below 65504.
+ * ws (256-byte aligned): n * 256 bytes, then per matrix with m = min, k = max of (rows, cols), both rounded up to 64: 12 m k + 8 m m bytes. */
+int craft_orthogonalize(const long* jobs, int n, const float* coeffs, int steps, float eps, float s_x, float s_a, float s_b, int dtype, void* ws,
+                        long ws_bytes, void* stream);
+/* The optimizer around it, over n ranges {offset, length} (host longs) of flat fp32 buffers; state: the record of craft_loss_scale_update (a skipped step
+ * writes nothing).  momentum: buf = momentum buf + g, update = nesterov ? g + momentum buf : buf, g = gm grad.
+ * apply: param = (1 - lr weight_decay) param - lr scales[i] update. */
+int craft_muon_momentum(const float* grad, float* buf, float* update, const long* segs, int n, float momentum, int nesterov, const void* state, void* stream);
+int craft_muon_apply(float* param, const float* update, const long* segs, const float* scales, int n, float lr, float weight_decay, const void* state,
+                     void* stream);
+
 #ifdef __cplusplus
 }
 #endif

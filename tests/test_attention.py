@@ -1,0 +1,339 @@
+"""ops.attention / autograd.attention against the formula in 64 bits: types, head layouts, lengths, masks, strides, and what they refuse."""
+import math
+
+import pytest
+import torch
+
+from attention_reference import attention64, check, visible
+
+gpu = pytest.mark.gpu
+TYPES = {"fp16": torch.float16, "bf16": torch.bfloat16, "fp32": torch.float32}
+
+
+def make(t, B, nq, nk, H, Hk, D, seed=0, spread=3.0, device="cuda"):
+    g = torch.Generator().manual_seed(seed)
+    n = lambda *s: torch.randn(*s, generator=g)                            # noqa: E731
+    return [x.to(TYPES[t]).to(device) for x in (spread * n(B, nq, H, D), n(B, nk, Hk, D), n(B, nk, Hk, D), n(B, nq, H, D))]
+
+
+def slopes_of(H, device="cuda"):
+    return torch.tensor([2.0 ** (-8.0 * (h + 1) / H) for h in range(H)], device=device)
+
+
+def doc_ids(B, n, pieces, padding, seed=0, device="cuda"):
+    g = torch.Generator().manual_seed(seed)
+    out = torch.full((B, n), -1, dtype=torch.int32)
+    for b in range(B):
+        m = n - padding
+        cut = sorted({0, m, *torch.randint(0, m + 1, (pieces - 1,), generator=g).tolist()})
+        for d, (a, e) in enumerate(zip(cut, cut[1:])):
+            out[b, a:e] = d
+    return out.to(device)
+
+
+def both(t, B, nq, nk, H, Hk, D, seed=0, spread=3.0, **how):
+    """The differentiable form with its gradients and the inference form, each against 64 bits."""
+    from craft_amd import autograd, ops
+    q, k, v, go = make(t, B, nq, nk, H, Hk, D, seed, spread)
+    res, tol = attention64(q, k, v, go, **how)
+    q, k, v = (x.requires_grad_() for x in (q, k, v))
+    o = autograd.attention(q, k, v, **how)
+    check([o, *torch.autograd.grad(o, (q, k, v), go)], res, tol)
+    check([ops.attention(q, k, v, **how)], res[:1], tol[:1])
+
+
+# ---------------------------------------------------------------------------------------------------------------- CPU: the oracle and the refusals
+def test_reference_gradients_are_autograds():
+    """The formulas the kernels are held to, against torch's own differentiation of the definition."""
+    q, k, v, go = make("fp32", 2, 9, 13, 4, 2, 8, device="cpu")
+    how = dict(cap=4.0, slopes=slopes_of(4, "cpu"), causal=True, prefix=torch.tensor([0, 7], dtype=torch.int32))
+    res, _ = attention64(q, k, v, go, **how)
+    a, b, c = (x.double().requires_grad_() for x in (q, k, v))
+    kk, vv = (x.transpose(1, 2).repeat_interleave(2, 1) for x in (b, c))
+    z = 4.0 * torch.tanh(a.transpose(1, 2) @ kk.mT / math.sqrt(8) / 4.0)
+    z = z - slopes_of(4, "cpu").double()[:, None, None] * ((torch.arange(9)[:, None] + 4) - torch.arange(13)).abs()
+    o = (torch.softmax(z.masked_fill(~visible(9, 13, True, how["prefix"], batch=2)[:, None], -math.inf), -1) @ vv).transpose(1, 2)
+    for r, g in zip(res, (o, *torch.autograd.grad(o, (a, b, c), go.double()))):
+        assert torch.allclose(r, g, rtol=1e-12, atol=1e-12)
+
+
+@pytest.mark.parametrize("change, says", [
+    (dict(q=torch.zeros(1, 4, 3, 16), k=torch.zeros(1, 4, 2, 16), v=torch.zeros(1, 4, 2, 16)), "no multiple"),
+    (dict(q=torch.zeros(1, 4, 2, 12), k=torch.zeros(1, 4, 2, 12), v=torch.zeros(1, 4, 2, 12)), "multiple of 8"),
+    (dict(q=torch.zeros(1, 4, 2, 136), k=torch.zeros(1, 4, 2, 136), v=torch.zeros(1, 4, 2, 136)), "multiple of 8"),
+    (dict(k=torch.zeros(1, 4, 2, 8)), "do not fit"),
+    (dict(v=torch.zeros(1, 5, 2, 16)), "do not fit"),
+    (dict(q=torch.zeros(4, 2, 16)), "are \\[batch"),
+    (dict(k=torch.zeros(1, 4, 2, 16, dtype=torch.float16)), "one type"),
+    (dict(q=torch.zeros(1, 4, 2, 16).double(), k=torch.zeros(1, 4, 2, 16).double(), v=torch.zeros(1, 4, 2, 16).double()), "one type"),
+    (dict(cap=-1.0), "cap"), (dict(cap=float("nan")), "cap"), (dict(cap=float("inf")), "cap"),
+    (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale"),
+    (dict(prefix=torch.zeros(1, dtype=torch.int32)), "causal=True"),
+    (dict(prefix=torch.zeros(2, dtype=torch.int32), causal=True), "prefix must"),
+    (dict(prefix=torch.zeros(1, dtype=torch.int64), causal=True), "prefix must"),
+    (dict(slopes=torch.zeros(3)), "slopes"), (dict(slopes=torch.zeros(2).half()), "slopes"),
+    (dict(slopes=torch.zeros(2, requires_grad=True)), "no gradient"),
+    (dict(docs=torch.zeros(1, 3, dtype=torch.int32)), "docs must"),
+    (dict(docs=torch.zeros(1, 4)), "docs must"),
+    (dict(docs_k=torch.zeros(1, 4, dtype=torch.int32)), "needs docs"),
+    (dict(docs=torch.zeros(1, 4, dtype=torch.int32), docs_k=torch.zeros(1, 3, dtype=torch.int32)), "docs_k must"),
+    (dict(q=torch.zeros(1, 3, 2, 16), docs=torch.zeros(1, 3, dtype=torch.int32)), "docs_k too"),
+    (dict(), "device tensors"),
+])
+def test_refusals(change, says):
+    from craft_amd import autograd, ops
+    from craft_amd.hip import CraftHipError
+    args = dict(q=torch.zeros(1, 4, 2, 16), k=torch.zeros(1, 4, 2, 16), v=torch.zeros(1, 4, 2, 16), **{})
+    args.update(change)
+    q, k, v = args.pop("q"), args.pop("k"), args.pop("v")
+    with torch.enable_grad(), pytest.raises(CraftHipError, match=says):
+        autograd.attention(q, k, v, **args)
+    if says != "no gradient":                                             # (without gradients, slopes that have one are a plain input)
+        with pytest.raises(CraftHipError, match=says):
+            ops.attention(q, k, v, **args)
+
+
+def test_entry_points_check_their_arguments():
+    """The C entry points refuse what their kernels assume, before anything is launched (no GPU needed)."""
+    import ctypes
+
+    from craft_amd import hip
+    lib = hip.load()
+    buf = 4096                                                             # an aligned address that is never read: every call below is refused first
+    good = [1, 4, 4, 2, 2, 16] + [128, 32, 16] * 4
+
+    def fwd(shape=good, q=buf, k=buf, v=buf, out=buf, scale=1.0, cap=0.0, causal=0, dtype=2, splits=0, docs=(None, None), prefix=None, ws=None, ws_bytes=0, lse=None):
+        return lib.craft_attention_fwd(q, k, v, (ctypes.c_long * len(shape))(*shape), None, prefix, docs[0], docs[1], scale, cap, causal, dtype, splits, out, lse,
+                                       ws, ws_bytes, None)
+
+    def with_(i, x):
+        s = list(good)
+        s[i] = x
+        return s
+    ARG, ALIGN, UNSUPPORTED = 10001, 10002, 10003
+    assert fwd(with_(0, 0)) == UNSUPPORTED and fwd(with_(1, -1)) == UNSUPPORTED and fwd(with_(2, 1 << 29)) == UNSUPPORTED
+    assert fwd(with_(3, 3)) == UNSUPPORTED and fwd(with_(5, 136)) == UNSUPPORTED and fwd(with_(5, 20)) == ALIGN
+    assert fwd(with_(7, 36)) == ALIGN and fwd(with_(10, -16)) == ALIGN and fwd(with_(10, 1 << 23)) == UNSUPPORTED
+    assert fwd(q=buf + 8) == ALIGN and fwd(k=None) == ALIGN and fwd(out=buf + 2) == ALIGN
+    assert fwd(dtype=3) == ARG and fwd(cap=-1.0) == ARG and fwd(cap=float("nan")) == ARG and fwd(scale=float("nan")) == ARG
+    assert fwd(docs=(buf, None)) == ARG and fwd(docs=(buf, buf)) == ARG                      # (no workspace for the ranges)
+    assert fwd(prefix=buf) == ARG and fwd(splits=-1) == ARG and fwd(splits=2) == ARG and fwd(splits=1, lse=buf) == ARG
+    shape5 = (ctypes.c_long * 21)(*(good + [128, 32, 16]))
+    bwd = lambda ws, n, lse=buf, dk=buf: lib.craft_attention_bwd(buf, buf, buf, buf, lse, buf, shape5, None, None, None, None, 1.0, 0.0, 0, 2, 1, buf, dk, buf, ws, n, None)  # noqa: E731
+    assert bwd(None, 0) == ARG and bwd(buf, 31) == ARG and bwd(buf, 1 << 20, lse=None) == ARG and bwd(buf, 1 << 20, dk=buf + 4) == ALIGN
+
+
+# ---------------------------------------------------------------------------------------------------------------- GPU
+SHAPES = [  # B, queries, keys, heads, key heads, width
+    (1, 1, 1, 1, 1, 8), (2, 2, 2, 2, 1, 16), (1, 31, 33, 2, 2, 32), (1, 64, 64, 1, 1, 40), (2, 65, 65, 3, 3, 64), (1, 127, 129, 2, 1, 72),
+    (1, 130, 130, 4, 2, 128), (2, 1, 300, 8, 2, 128), (1, 5, 77, 4, 4, 64), (1, 200, 40, 2, 2, 64), (1, 300, 300, 6, 2, 24), (1, 40, 530, 12, 1, 64)]
+
+
+@gpu
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_plain(device, t, shape):
+    both(t, *shape)
+
+
+@gpu
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("shape", SHAPES, ids=lambda s: "x".join(map(str, s)))
+def test_causal_capped_biased(device, t, shape):
+    """All at once; more queries than keys leaves the first rows empty."""
+    both(t, *shape, causal=True, cap=5.0, slopes=slopes_of(shape[3]))
+
+
+@gpu
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("cap, slopes, causal", [(0.0, True, False), (30.0, False, False), (2.0, True, False), (0.0, True, True), (0.0, False, True)])
+def test_one_by_one(device, t, cap, slopes, causal):
+    both(t, 2, 150, 150, 4, 2, 64, cap=cap, slopes=slopes_of(4) if slopes else None, causal=causal)
+
+
+@gpu
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("nq, nk, prefix", [(150, 150, [0, 150]), (70, 200, [1, 131]), (33, 33, [500, 17]), (140, 20, [3, 0]), (1, 90, [90, 4]), (140, 140, [64, 63])])
+def test_prefix(device, t, nq, nk, prefix):
+    both(t, 2, nq, nk, 4, 2, 64, causal=True, prefix=torch.tensor(prefix, dtype=torch.int32, device="cuda"))
+
+
+@gpu
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("n, pieces, padding", [(33, 1, 0), (65, 3, 7), (200, 5, 0), (300, 9, 140), (300, 2, 299), (128, 128, 0), (40, 1, 40)])
+@pytest.mark.parametrize("causal", [False, True])
+def test_documents(device, t, n, pieces, padding, causal):
+    both(t, 2, n, n, 4, 2, 64, causal=causal, docs=doc_ids(2, n, pieces, padding))
+
+
+@gpu
+@pytest.mark.parametrize("t", list(TYPES))
+def test_documents_out_of_order(device, t):
+    """Interleaved documents (no sorted runs), other ids for queries and keys, queries whose document no key has."""
+    g = torch.Generator().manual_seed(5)
+    dq = torch.randint(-1, 6, (2, 90), generator=g, dtype=torch.int32).cuda()
+    dk = torch.randint(-1, 5, (2, 210), generator=g, dtype=torch.int32).cuda()
+    both(t, 2, 90, 210, 4, 2, 64, docs=dq, docs_k=dk)
+    both(t, 2, 90, 210, 4, 2, 64, docs=dq, docs_k=dk, causal=True, prefix=torch.tensor([40, 0], dtype=torch.int32, device="cuda"), cap=3.0)
+    both(t, 2, 3, 210, 4, 2, 64, docs=dq[:, :3].contiguous(), docs_k=dk)
+
+
+@gpu
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("nq", [1, 100])
+def test_padding_may_hold_anything(device, t, nq):
+    """inf and NaN in rows whose document is negative reach nothing, in the results and in the gradients; the padded rows' own are zero."""
+    from craft_amd import autograd, ops
+    q, k, v, go = make(t, 2, nq, 100, 4, 2, 64)
+    dk = doc_ids(2, 100, 3, 30)
+    dq = dk[:, -nq:].contiguous() if nq > 1 else torch.zeros(2, 1, dtype=torch.int32, device="cuda")
+    res, tol = attention64(q, k, v, go, docs=dq, docs_k=dk)
+    bad = torch.tensor([math.nan, math.inf, -math.inf], device="cuda").to(q.dtype)
+    for x, d in ((q, dq), (go, dq), (k, dk), (v, dk)):
+        m = (d < 0)[:, :, None, None].expand(x.shape)
+        x[m] = bad[torch.arange(int(m.sum()), device="cuda") % 3]
+    q, k, v = (x.requires_grad_() for x in (q, k, v))
+    o = autograd.attention(q, k, v, docs=dq, docs_k=dk)
+    grads = torch.autograd.grad(o, (q, k, v), go)
+    check([o, *grads], res, tol)
+    check([ops.attention(q, k, v, docs=dq, docs_k=dk)], res[:1], tol[:1])
+    assert not grads[0][dq < 0].any() and not grads[1][dk < 0].any() and not grads[2][dk < 0].any() and not o[dq < 0].any()
+
+
+@gpu
+@pytest.mark.parametrize("t", list(TYPES))
+def test_large_scores(device, t):
+    """Scores in the hundreds: the running maximum carries the sums; a cap brings them back."""
+    both(t, 1, 140, 140, 2, 2, 64, spread=60.0)
+    both(t, 1, 140, 140, 2, 2, 64, spread=60.0, cap=20.0, causal=True)
+    both(t, 1, 140, 140, 2, 2, 64, scale=-0.3)
+
+
+@gpu
+def test_rising_scores(device):
+    """Every later key tile raises the maximum: the output is rescaled each time."""
+    from craft_amd import ops
+    q = torch.ones(1, 4, 1, 32, device="cuda", dtype=torch.bfloat16)
+    k = (torch.arange(512, device="cuda").float()[None, :, None, None] / 8).expand(1, 512, 1, 32).to(torch.bfloat16)
+    v = torch.randn(1, 512, 1, 32, device="cuda").bfloat16()
+    for n in (4, 100):
+        qq = q[:, :1].expand(1, n, 1, 32).contiguous()
+        res, tol = attention64(qq, k, v, scale=1.0)
+        check([ops.attention(qq, k, v, scale=1.0)], res, tol)
+
+
+@gpu
+def test_views(device):
+    """Slices of one packed projection, a head-major layout, expanded heads, and rows that no 16-byte step fits are read right."""
+    from craft_amd import autograd, ops
+    g = torch.Generator().manual_seed(3)
+    qkv = torch.randn(2, 70, 3, 4, 64, generator=g).half().cuda()
+    q, k, v = qkv.unbind(2)
+    res, tol = attention64(q, k, v, causal=True)
+    check([ops.attention(q, k, v, causal=True)], res, tol)
+    hm = [x.transpose(1, 2).contiguous().transpose(1, 2) for x in (q, k, v)]
+    check([ops.attention(*hm, causal=True)], res, tol)
+    odd = torch.randn(2 * 70 * 4 * 67 + 5, generator=g).half().cuda()
+    odd = [torch.as_strided(odd, (2, 70, 4, 64), (70 * 4 * 67, 4 * 67, 67, 1), i) for i in (1, 3, 5)]
+    res, tol = attention64(*odd)
+    check([ops.attention(*odd)], res, tol)
+    k1, v1 = (x[:, :, :1].expand(2, 70, 4, 64) for x in (k, v))
+    res, tol = attention64(q, k1, v1)
+    check([ops.attention(q, k1, v1)], res, tol)
+    out = torch.zeros(2, 70, 8, 64, device="cuda", dtype=torch.float16)
+    assert ops.attention(q, k1, v1, out=out[:, :, 2:6]).data_ptr() == out[:, :, 2:6].data_ptr()
+    check([out[:, :, 2:6]], res, tol)
+    assert not out[:, :, :2].any() and not out[:, :, 6:].any()
+    # gradients through views, and a gradient that is an expanded scalar
+    leaf = qkv.clone().requires_grad_()
+    autograd.attention(*leaf.unbind(2), causal=True).sum().backward()
+    res, tol = attention64(q, k, v, torch.ones_like(q), causal=True)
+    check([res[0], *leaf.grad.unbind(2)], res, tol)
+
+
+@gpu
+def test_lengths_of_zero(device):
+    from craft_amd import autograd, ops
+    for nq, nk, B in ((0, 5, 1), (5, 0, 1), (5, 5, 0)):
+        q, k, v, go = make("bf16", B, nq, nk, 4, 2, 64)
+        assert ops.attention(q, k, v).shape == q.shape and not ops.attention(q, k, v).any()
+        q, k, v = (x.requires_grad_() for x in (q, k, v))
+        for g, x in zip(torch.autograd.grad(autograd.attention(q, k, v), (q, k, v), go), (q, k, v)):
+            assert g.shape == x.shape and not g.any()
+
+
+@gpu
+def test_long_cache_past_32_bits(device):
+    """Keys and values that lie more than 2^32 bytes behind the first: only the last one scores above the others."""
+    from craft_amd import ops
+    nk, Hk, D = (1 << 20) + 77, 18, 128                                    # 4.8 GB each
+    k = torch.zeros(1, nk, Hk, D, device="cuda", dtype=torch.bfloat16)
+    v = torch.zeros(1, nk, Hk, D, device="cuda", dtype=torch.bfloat16)
+    last = torch.randn(Hk, D, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    k[0, -1], v[0, -1] = 8.0, last
+    q = torch.full((1, 1, Hk, D), 8.0, device="cuda", dtype=torch.bfloat16)
+    o = ops.attention(q, k, v, causal=True)
+    assert torch.equal(o[0, 0], last)                                      # exp(-724) of the rest
+    o = ops.attention(q.expand(1, 130, Hk, D), k, v, causal=True)          # the block kernel: only the last query sees the last key
+    assert torch.equal(o[0, -1], last) and not o[0, :-1].any()
+
+
+@gpu
+def test_gradients_against_differences(device):
+    """The fp32 gradients against central differences of the kernel's own forward pass, along random directions.  An fp32 sum of 2 880 products of
+    unit size is off by at most 1e-4; over a step of 2e-2 that is 1e-2 of a derivative of size 10 to 100, and the cubic term is below it."""
+    from craft_amd import autograd
+    q, k, v, go = make("fp32", 1, 45, 45, 2, 1, 32, spread=1.0)
+    how = dict(cap=3.0, causal=True, slopes=slopes_of(2))
+    q, k, v = (x.requires_grad_() for x in (q, k, v))
+    grads = torch.autograd.grad(autograd.attention(q, k, v, **how), (q, k, v), go)
+    for n, x in enumerate((q, k, v)):
+        d = torch.randn(x.shape, generator=torch.Generator().manual_seed(n)).cuda()
+        f = lambda s: (autograd.attention(*[y.detach() + (s * d if m == n else 0) for m, y in enumerate((q, k, v))], **how).double() * go.double()).sum().item()  # noqa: E731,B023
+        num = (f(1e-2) - f(-1e-2)) / 2e-2
+        assert abs(num - (grads[n].double() * d.double()).sum().item()) < 2e-2 * max(1.0, abs(num))
+
+
+@gpu
+@pytest.mark.parametrize("t", ["bf16", "fp32"])
+def test_same_bits_every_time(device, t):
+    """No result depends on the order of blocks or atomics: shared heads, split keys and all."""
+    from craft_amd import autograd, ops
+    q, k, v, go = make(t, 2, 260, 260, 8, 2, 64)
+    q, k, v = (x.requires_grad_() for x in (q, k, v))
+    runs = []
+    for _ in range(3):
+        o = autograd.attention(q, k, v, causal=True)
+        runs.append([o, *torch.autograd.grad(o, (q, k, v), go), ops.attention(q[:, :1], k, v)])
+    assert all(torch.equal(a, b) for r in runs[1:] for a, b in zip(runs[0], r))
+
+
+@gpu
+def test_other_stream_and_captured(device):
+    """On a side stream, and captured into a graph whose replays follow new inputs (single tokens, whole rows, with documents), each against eager."""
+    from craft_amd import ops
+    q, k, v, _ = make("fp16", 2, 130, 130, 4, 2, 64)
+    docs = doc_ids(2, 130, 4, 10)
+    want = ops.attention(q, k, v, docs=docs)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got = ops.attention(q, k, v, docs=docs)
+    side.synchronize()
+    assert torch.equal(got, want)
+    one = q[:, -1:].contiguous()
+    with torch.cuda.stream(side):                                          # (warm-up outside the capture)
+        ops.attention(q, k, v, docs=docs), ops.attention(one, k, v, causal=True)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        a = ops.attention(q, k, v, docs=docs)
+        b = ops.attention(one, k, v, causal=True)
+    for seed in range(4):
+        for x, y in zip((q, k, v), make("fp16", 2, 130, 130, 4, 2, 64, seed=seed)):
+            x.copy_(y)
+        docs.copy_(doc_ids(2, 130, 4, 10, seed=seed))
+        one.copy_(q[:, -1:])
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(a, ops.attention(q, k, v, docs=docs)) and torch.equal(b, ops.attention(one, k, v, causal=True))
