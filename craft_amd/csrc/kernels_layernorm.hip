@@ -3,10 +3,12 @@
 //   y = xn w + b,  xn = (x - mean) rstd;      dx = rstd (g - mean(g) - xn mean(g xn)) with g = dy w,   dw = sum_rows dy xn,   db = sum_rows dy
 //
 // HBM-bound: x is read once forward (and the row held in registers for its two statistics, mean first, then the squares about it, in fp32), x and dy once
-// backward.  A row belongs to TPR threads (16 of a wave, a wave, 4 waves, 16 waves: the smallest that holds it with at most 4 vectors a thread).
+// backward.  A row belongs to TPR threads (16 of a wave, a wave, up to 16 waves), with one vector
+// each up to 1024 vectors.
 // The weight's and the bias' gradients are summed on the way: a thread owns the same columns of every row it meets, so its sums stay in registers over the
 // block's whole share of the rows; the row groups of a block are joined in LDS, the blocks by k_layer_norm_sum -- each in a fixed order, no atomics.
 // Vectors are 16 bytes at any alignment (unaligned loads and stores are native): an odd width costs its last vector element by element, nothing else.
+#include <type_traits>
 #include "launch.hpp"
 #include "../../include/craft_hip.h"
 
@@ -25,35 +27,39 @@ struct LayerNormParams {
   float eps;
 };
 
-template <typename T> struct LnVec { static constexpr int N = 16 / sizeof(T); typedef T type __attribute__((ext_vector_type(16 / sizeof(T)), aligned(sizeof(T)))); };
+template <typename T> struct LnVec { static constexpr int N = 16 / sizeof(T); };
 
-template <typename T, typename W, int N>
-__device__ __forceinline__ void ln_load(const W* p, int col, int C, float (&f)[N]) {
-  typedef W vec __attribute__((ext_vector_type(N), aligned(sizeof(W))));
-  if (col + N <= C) {
-    const vec v = *reinterpret_cast<const vec*>(p + col);
-#pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = (float)v[i];
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; ++i) f[i] = col + i < C ? (float)p[col + i] : 0.f;
+// A thread's vector j holds columns base .. base + N - 1 of the row, of which those below `lo` belong to its neighbour: the last vector of a row whose
+// width is no multiple of N is moved back to end with the row, so that every load is one whole vector with no branch around it (a branch per vector made
+// the loads of a row wait for one another: 28 us instead of 9 for the gradients of 1441 rows of 1027).  A row narrower than a vector goes element by element.
+template <int N>
+struct LnCols {
+  int base, lo;
+  __device__ __forceinline__ LnCols(int col, int C) {
+    base = col + N <= C ? col : C >= N ? C - N : 0;
+    lo = col;                                          // a vector behind the row owns nothing
   }
-}
+  __device__ __forceinline__ bool mine(int i, int C) const { return base + i >= lo && base + i < C; }
+};
+
+// the neighbour's columns get the values that the neighbour writes
 template <typename T, int N>
-__device__ __forceinline__ void ln_store(T* p, int col, int C, const float (&f)[N]) {
+__device__ __forceinline__ void ln_store(T* p, const LnCols<N>& k, int C, const float (&f)[N]) {
   typedef T vec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
-  if (col + N <= C) {
+  if (k.lo >= C) return;
+  if (C >= N) {
     vec v;
 #pragma unroll
     for (int i = 0; i < N; ++i) v[i] = (T)f[i];
-    *reinterpret_cast<vec*>(p + col) = v;
+    *reinterpret_cast<vec*>(p + k.base) = v;
   } else {
 #pragma unroll
-    for (int i = 0; i < N; ++i) if (col + i < C) p[col + i] = (T)f[i];
+    for (int i = 0; i < N; ++i) if (k.base + i < C) p[k.base + i] = (T)f[i];
   }
 }
 
-// sums over the TPR threads of a row, on all of them.  TPR > 64: `red` [2][waves of the row][2], used alternately, so one barrier a call is enough
+// sums over the TPR threads of a row, on all of them.  TPR > 64: `red` [2][waves of the row][2] of the row's group, used alternately, so one barrier a
+// call is enough (all threads of the block have to come)
 template <int TPR, int NS>
 __device__ __forceinline__ void ln_sum(float (&s)[NS], float* red, int wave_in_row, int phase) {
 #pragma unroll
@@ -77,150 +83,205 @@ __device__ __forceinline__ void ln_sum(float (&s)[NS], float* red, int wave_in_r
   }
 }
 
-template <int TPR> constexpr int ln_threads() { return TPR > 256 ? TPR : 256; }
-
-template <typename T, typename W, int TPR, int NV>
-__global__ __launch_bounds__((ln_threads<TPR>())) void k_layer_norm_fwd(LayerNormParams p) {
-  constexpr int N = LnVec<T>::N, RPB = ln_threads<TPR>() / TPR;
-  __shared__ float red[2 * 2 * 16];
+// TH threads: TH / TPR rows at a time; a block walks over the rows blockIdx.x * RPB + group, + gridDim.x * RPB, ... and has the next row's vectors on
+// their way while this one is worked on.  Two blocks to a compute unit.
+template <typename T, typename W, int TPR, int NV, int TH>
+__global__ __launch_bounds__(TH) void k_layer_norm_fwd(LayerNormParams p) {
+  constexpr int N = LnVec<T>::N, RPB = TH / TPR, NW = TPR > 64 ? TPR / 64 : 1;
+  typedef T tvec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+  __shared__ float red[RPB][2 * NW * 2];
   const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
-  const long row = (long)blockIdx.x * RPB + group;
-  if (TPR <= 64 && row >= p.rows) return;             // (TPR > 64: one row per block, always there)
-  const T* x = reinterpret_cast<const T*>(p.x) + row * p.ldx;
-  float v[NV][N];
-  float s[1] = {0.f};
-#pragma unroll
-  for (int j = 0; j < NV; ++j) ln_load<T>(x, (j * TPR + t) * N, p.C, v[j]);
-#pragma unroll
-  for (int j = 0; j < NV; ++j)
-#pragma unroll
-    for (int i = 0; i < N; ++i) s[0] += v[j][i];
-  ln_sum<TPR, 1>(s, red, t >> 6, 0);
-  const float inv = 1.f / (float)p.C, mean = s[0] * inv;
-  s[0] = 0.f;
-#pragma unroll
-  for (int j = 0; j < NV; ++j)
-#pragma unroll
-    for (int i = 0; i < N; ++i) {
-      const float d = (j * TPR + t) * N + i < p.C ? v[j][i] - mean : 0.f;
-      v[j][i] = d;
-      s[0] += d * d;
-    }
-  ln_sum<TPR, 1>(s, red, t >> 6, 1);
-  const float rstd = 1.f / sqrtf(s[0] * inv + p.eps);
-  T* y = reinterpret_cast<T*>(p.y) + row * p.ldy;
+  const bool whole = p.C >= N;                        // (uniform)
+  auto cols = [&](int j) { return LnCols<N>((j * TPR + t) * N, p.C); };
+  const float inv = 1.f / (float)p.C;
+  // the weights stay in registers, in their own type: loads arrive in order, so one inside the loop would wait for the next row
+  typedef W wvec __attribute__((ext_vector_type(N), aligned(sizeof(W))));
+  wvec w[NV], b[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    const int col = (j * TPR + t) * N;
-    if (col >= p.C) continue;
-    float w[N], b[N];
-    if (p.w) ln_load<T>(reinterpret_cast<const W*>(p.w), col, p.C, w);
-    if (p.b) ln_load<T>(reinterpret_cast<const W*>(p.b), col, p.C, b);
+    const int base = cols(j).base;
 #pragma unroll
-    for (int i = 0; i < N; ++i) {
-      float o = v[j][i] * rstd;
-      if (p.w) o *= w[i];
-      if (p.b) o += b[i];
-      v[j][i] = o;
-    }
-    ln_store<T>(y, col, p.C, v[j]);
+    for (int i = 0; i < N; ++i) { w[j][i] = (W)1.f; b[j][i] = (W)0.f; }
+    auto get = [&](const void* q, wvec& v) {
+      const W* c = reinterpret_cast<const W*>(q);
+      if (whole) v = *reinterpret_cast<const wvec*>(c + base);
+      else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) if (base + i < p.C) v[i] = c[base + i];
+      }
+    };
+    if (p.w) get(p.w, w[j]);
+    if (p.b) get(p.b, b[j]);
   }
-  if (p.mean && t == 0) { p.mean[row] = mean; p.rstd[row] = rstd; }
+  tvec xv[NV];
+  auto fetch = [&](long r) {                           // (a group without a row goes through the last one and keeps nothing of it)
+    const T* q = reinterpret_cast<const T*>(p.x) + (r < p.rows ? r : p.rows - 1) * p.ldx;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const int base = cols(j).base;
+      if (whole) xv[j] = *reinterpret_cast<const tvec*>(q + base);
+      else {
+#pragma unroll
+        for (int i = 0; i < N; ++i) xv[j][i] = base + i < p.C ? q[base + i] : q[0];
+      }
+    }
+  };
+  const long step = (long)gridDim.x * RPB;
+  long row = (long)blockIdx.x * RPB + group;
+  fetch(row);
+  for (long row0 = (long)blockIdx.x * RPB; row0 < p.rows; row0 += step, row += step) {
+    const bool on = row < p.rows;
+    float v[NV][N];
+    float s[1] = {0.f};
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const LnCols<N> k = cols(j);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        v[j][i] = (float)xv[j][i];
+        s[0] += k.mine(i, p.C) ? v[j][i] : 0.f;
+      }
+    }
+    if (row0 + step < p.rows) fetch(row + step);
+    ln_sum<TPR, 1>(s, red[group], t >> 6, 0);
+    const float mean = s[0] * inv;
+    s[0] = 0.f;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+      const LnCols<N> k = cols(j);
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        v[j][i] -= mean;
+        s[0] += k.mine(i, p.C) ? v[j][i] * v[j][i] : 0.f;
+      }
+    }
+    ln_sum<TPR, 1>(s, red[group], t >> 6, 1);
+    const float rstd = 1.f / sqrtf(s[0] * inv + p.eps);
+    if (!on) continue;                                 // (behind the row's barriers)
+    T* y = reinterpret_cast<T*>(p.y) + row * p.ldy;
+#pragma unroll
+    for (int j = 0; j < NV; ++j) {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[j][i] = v[j][i] * rstd * (float)w[j][i] + (float)b[j][i];
+      ln_store<T, N>(y, cols(j), p.C, v[j]);
+    }
+    if (p.mean && t == 0) { p.mean[row] = mean; p.rstd[row] = rstd; }
+  }
 }
 
-// a block walks over the rows row0 + blockIdx.x * RPB, + gridDim.x * RPB, ...
-template <typename T, typename W, int TPR, int NV>
-__global__ __launch_bounds__((ln_threads<TPR>())) void k_layer_norm_bwd(LayerNormParams p) {
-  constexpr int N = LnVec<T>::N, TH = ln_threads<TPR>(), RPB = TH / TPR;
-  extern __shared__ float sums[];                     // [2][C] when the row groups of a block are joined
-  __shared__ float red[2 * 2 * 16];
+// 1024 threads: 1024 / TPR rows at a time; a block walks over the rows blockIdx.x * RPB + group, + gridDim.x * RPB, ...  The next row's vectors are on
+// their way while this one is worked on; vectors stay in their own type until used (twice: once for the sums, once for dx), which leaves the registers to
+// the sums of the weight's gradients.  TAIL: the width is no multiple of the vector (the masks it needs cost registers).
+template <typename T, typename W, int TPR, int NV, bool TAIL>
+__global__ __launch_bounds__(1024) void k_layer_norm_bwd(LayerNormParams p) {
+  constexpr int N = LnVec<T>::N, RPB = 1024 / TPR, NW = TPR > 64 ? TPR / 64 : 1;
+  typedef T tvec __attribute__((ext_vector_type(N), aligned(sizeof(T))));
+  typedef W wvec __attribute__((ext_vector_type(N), aligned(sizeof(W))));
+  extern __shared__ float sums[];                     // [2][C]: the row groups of a block are joined here
+  __shared__ float red[RPB][2 * NW * 2];
   const int t = threadIdx.x % TPR, group = threadIdx.x / TPR;
-  float dw[NV][N], db[NV][N], w[NV][N];
+  const bool whole = !TAIL || p.C >= N;               // (uniform)
+  auto cols = [&](int j) { return LnCols<N>((j * TPR + t) * N, p.C); };
+  auto mine = [&](int j, int i) { return TAIL ? cols(j).mine(i, p.C) : (j * TPR + t) * N < p.C; };
+  auto get = [&](auto* q, int base, auto& v) {
+    if (whole) v = *reinterpret_cast<const typename std::remove_reference<decltype(v)>::type*>(q + base);
+    else {
+#pragma unroll
+      for (int i = 0; i < N; ++i) v[i] = base + i < p.C ? q[base + i] : q[0];
+    }
+  };
+  float dw[NV][N], db[NV][N];
+  wvec w[NV];
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
 #pragma unroll
-    for (int i = 0; i < N; ++i) { dw[j][i] = db[j][i] = 0.f; w[j][i] = 1.f; }
-    if (p.w) ln_load<T>(reinterpret_cast<const W*>(p.w), (j * TPR + t) * N, p.C, w[j]);
+    for (int i = 0; i < N; ++i) { dw[j][i] = db[j][i] = 0.f; w[j][i] = (W)1.f; }
+    if (p.w) get(reinterpret_cast<const W*>(p.w), cols(j).base, w[j]);
   }
   const float inv = 1.f / (float)p.C;
   int phase = 0;
-  for (long row0 = (long)blockIdx.x * RPB; row0 < p.rows; row0 += (long)gridDim.x * RPB) {
-    const long row = row0 + group;
-    if (TPR > 64 || row < p.rows) {                   // (whole groups of at most a wave)
-      const T* x = reinterpret_cast<const T*>(p.x) + row * p.ldx;
-      const T* dy = reinterpret_cast<const T*>(p.dy) + row * p.lddy;
-      float v[NV][N], g[NV][N];
+  const long step = (long)gridDim.x * RPB;
+  tvec xv[NV], gv[NV];
+  float mean, rstd;
+  auto fetch = [&](long r) {                           // (a group without a row goes through the last one and keeps nothing of it)
+    const long row = r < p.rows ? r : p.rows - 1;
 #pragma unroll
-      for (int j = 0; j < NV; ++j) { ln_load<T>(x, (j * TPR + t) * N, p.C, v[j]); ln_load<T>(dy, (j * TPR + t) * N, p.C, g[j]); }
-      const float mean = p.mean[row], rstd = p.rstd[row];
-      float s[2] = {0.f, 0.f};
+    for (int j = 0; j < NV; ++j) {
+      get(reinterpret_cast<const T*>(p.x) + row * p.ldx, cols(j).base, xv[j]);
+      get(reinterpret_cast<const T*>(p.dy) + row * p.lddy, cols(j).base, gv[j]);
+    }
+    mean = p.mean[row];
+    rstd = p.rstd[row];
+  };
+  long row = (long)blockIdx.x * RPB + group;
+  fetch(row);
+  for (long row0 = (long)blockIdx.x * RPB; row0 < p.rows; row0 += step, row += step) {
+    const bool on = row < p.rows;
+    tvec x[NV], g[NV];
 #pragma unroll
-      for (int j = 0; j < NV; ++j)
+    for (int j = 0; j < NV; ++j) { x[j] = xv[j]; g[j] = gv[j]; }
+    const float mu = mean, rs = rstd;
+    if (row0 + step < p.rows) fetch(row + step);
+    float s[2] = {0.f, 0.f};
 #pragma unroll
-        for (int i = 0; i < N; ++i) {
-          const float xn = (v[j][i] - mean) * rstd, d = g[j][i];          // (behind the width d = 0: nothing is added)
-          dw[j][i] += d * xn;
-          db[j][i] += d;
-          const float gw = d * w[j][i];
-          s[0] += gw;
-          s[1] += gw * xn;
-          v[j][i] = xn;
-          g[j][i] = gw;
-        }
-      if (p.dx) {
-        ln_sum<TPR, 2>(s, red, t >> 6, phase);
-        phase ^= 1;
+    for (int j = 0; j < NV; ++j)
+#pragma unroll
+      for (int i = 0; i < N; ++i) {
+        const float d = on && mine(j, i) ? (float)g[j][i] : 0.f, xn = ((float)x[j][i] - mu) * rs, gw = d * (float)w[j][i];
+        dw[j][i] += d * xn;
+        db[j][i] += d;
+        s[0] += gw;
+        s[1] += gw * xn;
+      }
+    if (p.dx) {
+      ln_sum<TPR, 2>(s, red[group], t >> 6, phase);
+      phase ^= 1;
+      if (on) {
         const float m0 = s[0] * inv, m1 = s[1] * inv;
         T* dx = reinterpret_cast<T*>(p.dx) + row * p.lddx;
 #pragma unroll
         for (int j = 0; j < NV; ++j) {
-          const int col = (j * TPR + t) * N;
-          if (col >= p.C) continue;
+          float o[N];
 #pragma unroll
-          for (int i = 0; i < N; ++i) g[j][i] = (g[j][i] - m0 - v[j][i] * m1) * rstd;
-          ln_store<T>(dx, col, p.C, g[j]);
+          for (int i = 0; i < N; ++i) o[i] = ((float)g[j][i] * (float)w[j][i] - m0 - ((float)x[j][i] - mu) * rs * m1) * rs;
+          ln_store<T, N>(dx, cols(j), p.C, o);
         }
       }
     }
   }
   if (!p.part) return;
   float* out = p.part + (long)blockIdx.x * 2 * p.C;
-  if constexpr (RPB == 1) {
+  for (int q = 0; q < RPB; ++q) {                     // the groups one behind the other
+    if (group == q) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j) { ln_store<float>(out, (j * TPR + t) * N, p.C, dw[j]); ln_store<float>(out + p.C, (j * TPR + t) * N, p.C, db[j]); }
-  } else {
-    for (int q = 0; q < RPB; ++q) {                   // the groups one behind the other
-      if (group == q) {
+      for (int j = 0; j < NV; ++j)
 #pragma unroll
-        for (int j = 0; j < NV; ++j)
-#pragma unroll
-          for (int i = 0; i < N; ++i) {
-            const int col = (j * TPR + t) * N + i;
-            if (col < p.C) {
-              sums[col] = (q ? sums[col] : 0.f) + dw[j][i];
-              sums[p.C + col] = (q ? sums[p.C + col] : 0.f) + db[j][i];
-            }
+        for (int i = 0; i < N; ++i)
+          if (mine(j, i)) {
+            float* c = (RPB > 1 ? sums : out) + cols(j).base + i;
+            c[0] = (q ? c[0] : 0.f) + dw[j][i];
+            c[p.C] = (q ? c[p.C] : 0.f) + db[j][i];
           }
-      }
-      __syncthreads();
     }
-    for (int c = threadIdx.x; c < 2 * p.C; c += TH) out[c] = sums[c];
+    if (RPB > 1) __syncthreads();
   }
+  if constexpr (RPB > 1)
+    for (int c = threadIdx.x; c < 2 * p.C; c += 1024) out[c] = sums[c];
 }
 
-// [blocks][2][C] -> dw, db; a block of 256: 32 columns x 8 shares of the blocks
+// [blocks][2][C] -> dw, db; a block of 512: 32 columns x 16 shares of the blocks
 template <typename W>
-__global__ __launch_bounds__(256) void k_layer_norm_sum(const float* part, int blocks, int C, W* dw, W* db) {
-  __shared__ float red[8][33];
-  const int c = threadIdx.x & 31, q = threadIdx.x >> 5, col = blockIdx.x * 32 + c;
+__global__ __launch_bounds__(512) void k_layer_norm_sum(const float* part, int blocks, int C, W* dw, W* db) {
+  __shared__ float red[16][33];
+  const int c = threadIdx.x & 31, q = threadIdx.x >> 5, col = min((int)blockIdx.x * 32 + c, 2 * C - 1);
   float s = 0.f;
-  if (col < 2 * C)
-    for (int b = q; b < blocks; b += 8) s += part[(long)b * 2 * C + col];
+#pragma unroll 8
+  for (int b = q; b < blocks; b += 16) s += part[(long)b * 2 * C + col];
   red[q][c] = s;
   __syncthreads();
-  if (q == 0 && col < 2 * C) {
+  if (q == 0 && (int)blockIdx.x * 32 + c < 2 * C) {
 #pragma unroll
-    for (int k = 1; k < 8; ++k) s += red[k][c];
+    for (int k = 1; k < 16; ++k) s += red[k][c];
     if (col < C) { if (dw) dw[col] = (W)s; }
     else if (db) db[col - C] = (W)s;
   }
@@ -229,28 +290,32 @@ __global__ __launch_bounds__(256) void k_layer_norm_sum(const float* part, int b
 template <typename T, typename W>
 static int layer_norm_run(const LayerNormParams& p, int blocks, void* dw, void* db, hipStream_t s) {
   constexpr int N = LnVec<T>::N;
-  auto go = [&](auto fwd, auto bwd, int tpr, int th) {
-    const int rpb = th / tpr;
+  auto go = [&](auto fwd, auto bwd, int tpr) {
     if (!p.dy) {
-      const long grid = (p.rows + rpb - 1) / rpb;
-      if (grid > 0x7fffffffL) return CRAFT_ERR_UNSUPPORTED;
-      hipLaunchKernelGGL(fwd, dim3((unsigned)grid), dim3(th), 0, s, p);
+      const int th = tpr > 512 ? tpr : 512, rpb = th / tpr;
+      const long most = (p.rows + rpb - 1) / rpb, full = th == 512 ? 768 : 256;      // what the card holds at once (72 registers)
+      hipLaunchKernelGGL(fwd, dim3((unsigned)(most < full ? most : full)), dim3(th), 0, s, p);
       return (int)hipGetLastError();
     }
+    const int rpb = 1024 / tpr;
+    const long most = (p.rows + rpb - 1) / rpb;
+    const int grid = most < blocks ? (int)most : blocks;
     const size_t lds = p.part && rpb > 1 ? (size_t)2 * p.C * 4 : 0;
-    hipLaunchKernelGGL(bwd, dim3((unsigned)blocks), dim3(th), lds, s, p);
+    if (lds > 48 * 1024) HIP_CHECK_RET(hipFuncSetAttribute(reinterpret_cast<const void*>(bwd), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    hipLaunchKernelGGL(bwd, dim3((unsigned)grid), dim3(1024), lds, s, p);
     HIP_CHECK_RET(hipGetLastError());
-    if (p.part) hipLaunchKernelGGL(k_layer_norm_sum<W>, dim3((unsigned)((2 * p.C + 31) / 32)), dim3(256), 0, s, p.part, blocks, p.C, (W*)dw, (W*)db);
+    if (p.part) hipLaunchKernelGGL(k_layer_norm_sum<W>, dim3((unsigned)((2 * p.C + 31) / 32)), dim3(512), 0, s, p.part, grid, p.C, (W*)dw, (W*)db);
     return (int)hipGetLastError();
   };
-#define LN_GO(TPR, NV) go(k_layer_norm_fwd<T, W, TPR, NV>, k_layer_norm_bwd<T, W, TPR, NV>, TPR, ln_threads<TPR>())
   const int nv = (p.C + N - 1) / N;                    // vectors of a row
+  const bool tail = p.C % N != 0;
+#define LN_GO(TPR, NV) go(k_layer_norm_fwd<T, W, TPR, NV, (TPR > 512 ? TPR : 512)>, tail ? k_layer_norm_bwd<T, W, TPR, NV, true> : k_layer_norm_bwd<T, W, TPR, NV, false>, TPR)
   if (nv <= 16) return LN_GO(16, 1);
   if (nv <= 64) return LN_GO(64, 1);
-  if (nv <= 128) return LN_GO(64, 2);
-  if (nv <= 256) return LN_GO(64, 4);
-  if (nv <= 512) return LN_GO(256, 2);
-  if (nv <= 1024) return LN_GO(256, 4);
+  if (nv <= 128) return LN_GO(128, 1);
+  if (nv <= 256) return LN_GO(256, 1);
+  if (nv <= 512) return LN_GO(512, 1);
+  if (nv <= 1024) return LN_GO(1024, 1);
   if constexpr (sizeof(T) == 4) if (nv > 2048) return LN_GO(1024, 4);
   return LN_GO(1024, 2);
 #undef LN_GO

@@ -296,7 +296,8 @@ def _ptr(t):
 
 
 def _stream():
-    return torch.cuda.current_stream().cuda_stream
+    """The current stream of the current device as a hipStream_t (the raw getter: torch.cuda.current_stream() builds a Stream object, 3 us a call)."""
+    return torch._C._cuda_getCurrentRawStream(torch._C._cuda_getDevice())
 
 
 # Developer switch (tools/guard_run.py): CRAFT_HIP_DEBUG=<file> writes every entry point's name and arguments to <file> (rewound each call,
@@ -323,14 +324,12 @@ def _debug_note(name, args, conv):
     _debug_file.flush()
 
 
+_PLAIN = frozenset((int, float, type(None), bool))
+
+
 def call(name: str, *args):
     lib = load()
-    conv = []
-    for a in args:
-        if isinstance(a, torch.Tensor) or a is None:
-            conv.append(_ptr(a))
-        else:
-            conv.append(a)
+    conv = [a if type(a) in _PLAIN else _ptr(a) if isinstance(a, torch.Tensor) else a for a in args]      # (isinstance of Tensor is slow on numbers)
     if _DEBUG_PATH:
         _debug_note(name, args, conv)
     rc = getattr(lib, name)(*conv, _stream())

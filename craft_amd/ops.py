@@ -6,6 +6,7 @@ is forwarded as ``ld``).  No compute happens in Python.
 """
 from __future__ import annotations
 
+import contextlib
 import functools
 import math
 import os
@@ -665,6 +666,14 @@ def _on_device(*tensors):
     return dev
 
 
+def _on(dev):
+    """A context in which ``dev`` is the current device."""
+    return _NOTHING if dev.index == torch._C._cuda_getDevice() else torch.cuda.device(dev)
+
+
+_NOTHING = contextlib.nullcontext()
+
+
 def _norm_rows(x: torch.Tensor):
     """(x as rows of one stride, the stride): x itself where its leading axes are one run of rows, else a copy."""
     C = x.shape[-1]
@@ -716,7 +725,7 @@ def _layer_norm(x, weight, bias, eps, out, stats: bool):
     if rows:
         xr, ldx = _norm_rows(x)
         w, b = (None if t is None else t.contiguous() for t in (weight, bias))
-        with torch.cuda.device(x.device):
+        with _on(x.device):
             call("craft_layer_norm_fwd", xr, ldx, w, b, rows, C, float(eps), DTYPE_CODE[x.dtype], DTYPE_CODE[wt], y, ldy if rows > 1 else C, mean, rstd)
     return out, mean, rstd
 
@@ -742,11 +751,10 @@ def layer_norm_bwd(x: torch.Tensor, weight: Optional[torch.Tensor], bias_type: O
         return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
     xr, ldx = _norm_rows(x)
     g, ldg = _norm_rows(dy.to(x.dtype))
-    # the block's share of the rows: as many blocks as rows (a block takes 1024 / 256 / 16 rows at a time only at small widths), at most 4 for
-    # each compute unit -- more partial sums cost more than they hide
-    blocks = min(rows, 1024)
+    # one block of 1024 threads for each compute unit (or fewer, where there are few rows): each leaves one partial sum of the weight's gradients
+    blocks = min(rows, 256)
     ws = torch.empty(blocks * 2 * C, device=x.device, dtype=torch.float32) if need[1] or need[2] else None
-    with torch.cuda.device(x.device):
+    with _on(x.device):
         call("craft_layer_norm_bwd", xr, ldx, g, ldg if rows > 1 else C, None if weight is None else weight.contiguous(), mean, rstd, rows, C,
              DTYPE_CODE[x.dtype], DTYPE_CODE[wt], dx, C, dw, db, ws, blocks)
     return dx, dw, db
@@ -811,7 +819,7 @@ def orthogonalize(mats: Sequence[torch.Tensor], steps: int = 5, coeffs=NEWTON_SC
     device = _on_device(*mats)
     import ctypes
     flat = hip.carray(ctypes.c_float, [x for r in rows for x in r])
-    with torch.no_grad(), torch.cuda.device(device):
+    with torch.no_grad(), _on(device):
         for code in sorted({DTYPE_CODE[g.dtype] for g in mats}):
             todo = [(g, o) for g, o in zip(mats, out) if DTYPE_CODE[g.dtype] == code and g.numel()]
             for i in range(0, len(todo), _ORTHOGONALIZE_JOBS):
@@ -916,7 +924,7 @@ class AttentionPlan:
         B, Nq, Nk, H, Hk, D = self.dims
         splits = 0 if lse is not None else self.splits()
         nbytes = self.range_bytes() if not splits else 4 * B * Nq * H * splits * (D + 2) if splits > 1 else 0
-        with torch.cuda.device(self.device):
+        with _on(self.device):
             call("craft_attention_fwd", self.q, self.k, self.v, self.shape(out), *self.masks(), self.scale, self.cap, self.causal, self.code, splits, out,
                  lse, self.new(nbytes), nbytes)
 
@@ -928,7 +936,7 @@ class AttentionPlan:
         # key / value gradients of shared heads: one block walks over the group's heads, unless that leaves compute units without a block
         split_group = int(H > Hk and B * Hk * ((Nk + 127) // 128) < 512)
         nbytes = self.range_bytes() + (4 * B * H * Nq + 15) // 16 * 16 + split_group * 8 * B * Nk * H * D
-        with torch.cuda.device(self.device):
+        with _on(self.device):
             call("craft_attention_bwd", self.q, self.k, self.v, out, lse, go, self.shape(out, go), *self.masks(), self.scale, self.cap, self.causal, self.code,
                  split_group, dq, dk, dv, self.new(nbytes), nbytes)
         return dq, dk, dv
