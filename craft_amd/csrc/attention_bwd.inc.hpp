@@ -376,14 +376,15 @@ int attention_bwd_launch(const AttentionParams& p, hipStream_t s) {
   if (bq > 0x7fffffffL || bk > 0x7fffffffL || (rows + 15) / 16 > 0x7fffffffL) return CRAFT_ERR_UNSUPPORTED;
   hipLaunchKernelGGL(k_attention_delta<T>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, p, const_cast<float*>(p.delta));
   HIP_CHECK_RET(hipGetLastError());
-  auto go = [&](auto kernel, long blocks) {
-    HIP_CHECK_RET(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS));
+  auto go = [&](auto tag, long blocks) {
+    constexpr auto kernel = decltype(tag)::value;
+    if (const int rc = allow_lds<kernel>(S::LDS)) return rc;
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), S::LDS, s, p);
     return (int)hipGetLastError();
   };
   int rc;
-  if (p.cap > 0.f) rc = p.slopes ? go(k_attention_dkv<T, DP, true, true>, bk) : go(k_attention_dkv<T, DP, true, false>, bk);
-  else rc = p.slopes ? go(k_attention_dkv<T, DP, false, true>, bk) : go(k_attention_dkv<T, DP, false, false>, bk);
+  if (p.cap > 0.f) rc = p.slopes ? go(KernelTag<k_attention_dkv<T, DP, true, true>>(), bk) : go(KernelTag<k_attention_dkv<T, DP, true, false>>(), bk);
+  else rc = p.slopes ? go(KernelTag<k_attention_dkv<T, DP, false, true>>(), bk) : go(KernelTag<k_attention_dkv<T, DP, false, false>>(), bk);
   if (rc) return rc;
   if (p.part_k) {
     const long n4 = (long)p.B * p.Nk * p.Hk * (p.D / 4);
@@ -392,8 +393,8 @@ int attention_bwd_launch(const AttentionParams& p, hipStream_t s) {
                        reinterpret_cast<T*>(p.dv), n4, p.H / p.Hk, p.D / 4);
     HIP_CHECK_RET(hipGetLastError());
   }
-  if (p.cap > 0.f) return p.slopes ? go(k_attention_dq<T, DP, true, true>, bq) : go(k_attention_dq<T, DP, true, false>, bq);
-  return p.slopes ? go(k_attention_dq<T, DP, false, true>, bq) : go(k_attention_dq<T, DP, false, false>, bq);
+  if (p.cap > 0.f) return p.slopes ? go(KernelTag<k_attention_dq<T, DP, true, true>>(), bq) : go(KernelTag<k_attention_dq<T, DP, true, false>>(), bq);
+  return p.slopes ? go(KernelTag<k_attention_dq<T, DP, false, true>>(), bq) : go(KernelTag<k_attention_dq<T, DP, false, false>>(), bq);
 }
 
 }  // namespace craft

@@ -191,13 +191,14 @@ int attention_fwd_launch(const AttentionParams& p, hipStream_t s) {
   typedef FwdShape<T, DP> S;
   const long blocks = (long)p.B * p.H * ((p.Nq + 127) / 128);
   if (blocks > 0x7fffffffL) return CRAFT_ERR_UNSUPPORTED;
-  auto go = [&](auto kernel) {
-    HIP_CHECK_RET(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS));
+  auto go = [&](auto tag) {
+    constexpr auto kernel = decltype(tag)::value;
+    if (const int rc = allow_lds<kernel>(S::LDS)) return rc;
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), S::LDS, s, p);
     return (int)hipGetLastError();
   };
-  if (p.cap > 0.f) return p.slopes ? go(k_attention_fwd<T, DP, true, true>) : go(k_attention_fwd<T, DP, true, false>);
-  return p.slopes ? go(k_attention_fwd<T, DP, false, true>) : go(k_attention_fwd<T, DP, false, false>);
+  if (p.cap > 0.f) return p.slopes ? go(KernelTag<k_attention_fwd<T, DP, true, true>>()) : go(KernelTag<k_attention_fwd<T, DP, true, false>>());
+  return p.slopes ? go(KernelTag<k_attention_fwd<T, DP, false, true>>()) : go(KernelTag<k_attention_fwd<T, DP, false, false>>());
 }
 
 }  // namespace craft

@@ -225,14 +225,15 @@ int attention_token_launch(const AttentionParams& p, hipStream_t s) {
   const int R = p.Nq * (p.H / p.Hk), nrt = (R + 31) / 32;
   const long blocks = (long)p.B * p.Hk * nrt * p.splits, rows = (long)p.B * p.Hk * R;
   if (blocks > 0x7fffffffL || rows > 0x7fffffffL) return CRAFT_ERR_UNSUPPORTED;
-  auto go = [&](auto kernel) {
-    HIP_CHECK_RET(hipFuncSetAttribute(reinterpret_cast<const void*>(kernel), hipFuncAttributeMaxDynamicSharedMemorySize, S::LDS));
+  auto go = [&](auto tag) {
+    constexpr auto kernel = decltype(tag)::value;
+    if (const int rc = allow_lds<kernel>(S::LDS)) return rc;
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(S::WAVES * 64), S::LDS, s, p);
     return (int)hipGetLastError();
   };
   int rc;
-  if (p.cap > 0.f) rc = p.slopes ? go(k_attention_token<T, DP, true, true>) : go(k_attention_token<T, DP, true, false>);
-  else rc = p.slopes ? go(k_attention_token<T, DP, false, true>) : go(k_attention_token<T, DP, false, false>);
+  if (p.cap > 0.f) rc = p.slopes ? go(KernelTag<k_attention_token<T, DP, true, true>>()) : go(KernelTag<k_attention_token<T, DP, true, false>>());
+  else rc = p.slopes ? go(KernelTag<k_attention_token<T, DP, false, true>>()) : go(KernelTag<k_attention_token<T, DP, false, false>>());
   if (rc || p.splits == 1) return rc;
   hipLaunchKernelGGL(k_attention_join<T>, dim3((unsigned)rows), dim3(64), 0, s, p);
   return (int)hipGetLastError();

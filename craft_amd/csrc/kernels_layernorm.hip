@@ -290,7 +290,7 @@ __global__ __launch_bounds__(512) void k_layer_norm_sum(const float* part, int b
 template <typename T, typename W>
 static int layer_norm_run(const LayerNormParams& p, int blocks, void* dw, void* db, hipStream_t s) {
   constexpr int N = LnVec<T>::N;
-  auto go = [&](auto fwd, auto bwd, int tpr) {
+  auto go = [&](auto fwd, auto bwd, int tpr, int (*allow)(int)) {
     if (!p.dy) {
       const int th = tpr > 512 ? tpr : 512, rpb = th / tpr;
       const long most = (p.rows + rpb - 1) / rpb, full = th == 512 ? 768 : 256;      // what the card holds at once (72 registers)
@@ -301,7 +301,7 @@ static int layer_norm_run(const LayerNormParams& p, int blocks, void* dw, void* 
     const long most = (p.rows + rpb - 1) / rpb;
     const int grid = most < blocks ? (int)most : blocks;
     const size_t lds = p.part && rpb > 1 ? (size_t)2 * p.C * 4 : 0;
-    if (lds > 48 * 1024) HIP_CHECK_RET(hipFuncSetAttribute(reinterpret_cast<const void*>(bwd), hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds));
+    if (lds > 48 * 1024) if (const int rc = allow(2 * 8192 * 4)) return rc;      // (rows of up to 8192 share a block)
     hipLaunchKernelGGL(bwd, dim3((unsigned)grid), dim3(1024), lds, s, p);
     HIP_CHECK_RET(hipGetLastError());
     if (p.part) hipLaunchKernelGGL(k_layer_norm_sum<W>, dim3((unsigned)((2 * p.C + 31) / 32)), dim3(512), 0, s, p.part, grid, p.C, (W*)dw, (W*)db);
@@ -309,7 +309,8 @@ static int layer_norm_run(const LayerNormParams& p, int blocks, void* dw, void* 
   };
   const int nv = (p.C + N - 1) / N;                    // vectors of a row
   const bool tail = p.C % N != 0;
-#define LN_GO(TPR, NV) go(k_layer_norm_fwd<T, W, TPR, NV, (TPR > 512 ? TPR : 512)>, tail ? k_layer_norm_bwd<T, W, TPR, NV, true> : k_layer_norm_bwd<T, W, TPR, NV, false>, TPR)
+#define LN_GO(TPR, NV) go(k_layer_norm_fwd<T, W, TPR, NV, (TPR > 512 ? TPR : 512)>, tail ? k_layer_norm_bwd<T, W, TPR, NV, true> : k_layer_norm_bwd<T, W, TPR, NV, false>, TPR, \
+                          tail ? allow_lds<k_layer_norm_bwd<T, W, TPR, NV, true>> : allow_lds<k_layer_norm_bwd<T, W, TPR, NV, false>>)
   if (nv <= 16) return LN_GO(16, 1);
   if (nv <= 64) return LN_GO(64, 1);
   if (nv <= 128) return LN_GO(128, 1);

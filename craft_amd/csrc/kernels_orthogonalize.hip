@@ -3,23 +3,26 @@
 //   X <- G / (|G|_F + eps)   (G transposed where it has more rows than columns: m <= n)
 //   steps times:  A = X X^T,   B = b A + c A^2,   X <- a X + B X
 //
-// Each step is three products whose sizes differ from matrix to matrix, and each needs the one before it: three launches a step for the WHOLE list, a
-// block per output tile of any matrix (a table of the matrices travels in the kernel's arguments).  A and A^2 are symmetric: only their lower tiles are
-// computed and written twice.
+// Each step is three products whose sizes differ from matrix to matrix, and each needs the one before it: two or three launches a step for the WHOLE
+// list, a block per output tile of any matrix.  A and A^2 are symmetric: only their lower
+// tiles are computed, and written twice.
 //
 // Arithmetic: fp32-class.  Every operand is two fp16 planes hi + lo of its value times a power of two (22 bits and more: the scales bring the largest
 // possible entry, which the spectrum bounds, just below fp16's largest number, so that lo keeps its bits), every product three MFMAs with fp32 sums.  The
 // planes take the four bytes of an fp32 value.  The norm is summed in fp64: its error would scale the whole result.
 //
 // All operands are read along their rows: X (rows of n) for X X^T, A for A^2, and B with X^T (rows of m) for B X; the last product's epilogue writes both X
-// and X^T.  X^T is kept twice (blocks of one strip read it whole while others write).  Rows and columns are padded to 64 with zeros, which the products keep.
+// and X^T.  X^T is kept twice (blocks of one strip read it whole while others write).  Rows and columns are padded to 64 (128) with zeros, which the products keep.
 #include "attention_tile.hpp"
 #include "../../include/craft_hip.h"
 
 namespace craft {
 
-constexpr int NS_MAX_JOBS = 60;                      // (the table fits a kernel's 4 KB of arguments)
-constexpr int NS_NORM_BLOCKS = 32;                   // partial norms of a matrix, at most
+constexpr int NS_MAX_JOBS = 60;                      // (the table fits the 4 KB of k_ns_table's arguments)
+constexpr int NS_NORM_BLOCKS = 256;                  // partial norms of a matrix, at most
+constexpr int NS_MAX_BIG = 16;                       // larger ones in one set of launches
+constexpr long NS_PART_BYTES = 512l * 65536;         // partial tiles of the larger ones
+constexpr int NS_SMALL = 256;                        // smaller sides up to here: k_ns_gram / k_ns_update
 
 struct NsJob {
   const void* src; void* dst;
@@ -27,20 +30,33 @@ struct NsJob {
   long ws;                                           // byte offset of the matrix' operands in the workspace
   int rows, cols;                                    // of src and dst
   int mp, np;                                        // of X, padded
-  int first;                                         // its first block in this launch
-  int nb;                                            // blocks of its norm
+  short nb;                                          // blocks of its norm
+  short share[3];                                    // k_ns_big: shares of K in each of the three products
 };
+// The kinds of launches: a matrix' first block in each.
+enum { NS_NORM, NS_INIT, NS_LOWER, NS_ALL, NS_STRIPS, NS_SHARED, NS_KINDS = NS_SHARED + 3 };
+// The matrices' table, in the workspace: kernel arguments lie in host memory, and a search through them costs a kernel ten microseconds.  Which matrix a
+// block belongs to: every lane holds one first block, a ballot finds the last that is not behind.
+struct NsTable {
+  NsJob job[64];
+  int first[NS_KINDS][64];                           // (INT_MAX behind the last)
+  int part[3][64];                                   // k_ns_big: a matrix' first partial tile
+};
+struct NsLoad { NsJob job[NS_MAX_JOBS]; int n, span, side, big; NsTable* table; };
 struct NsParams {
-  NsJob job[NS_MAX_JOBS];
-  int n, dtype;
+  const NsTable* table;
+  int dtype, span;                                   // span: column tiles of a block of k_ns_update
   unsigned char* ws;
   double* norm;                                      // [jobs][NS_NORM_BLOCKS]
   float eps, c0, c1;                                 // epilogue: c0 * (old value) + c1 * (product), scales folded in
+  float b0, b1;                                      // k_ns_update: the same for B
   float s_x;                                         // scale of X
+  float* part;                                       // k_ns_big: partial tiles
   int last, flip;                                    // last step; which of the two X^T is read
 };
+constexpr long NS_TABLE_BYTES = 8192;
+static_assert(sizeof(NsLoad) <= 4096 && sizeof(NsTable) <= NS_TABLE_BYTES, "kernel arguments and the table in the workspace");
 
-static_assert(sizeof(NsParams) <= 4096, "kernel arguments");
 // a matrix' operands: X, X^T, X^T again, A, B; each [2][rows][cols] fp16
 __host__ __device__ __forceinline__ long ns_x_bytes(int mp, int np) { return 4l * mp * np; }
 __host__ __device__ __forceinline__ long ns_bytes(int mp, int np) { return 3 * ns_x_bytes(mp, np) + 2 * 4l * mp * mp; }
@@ -48,10 +64,38 @@ __device__ __forceinline__ _Float16* ns_x(const NsParams& p, const NsJob& j) { r
 __device__ __forceinline__ _Float16* ns_xt(const NsParams& p, const NsJob& j, int which) { return reinterpret_cast<_Float16*>(p.ws + j.ws + (1 + which) * ns_x_bytes(j.mp, j.np)); }
 __device__ __forceinline__ _Float16* ns_a(const NsParams& p, const NsJob& j, int which) { return reinterpret_cast<_Float16*>(p.ws + j.ws + 3 * ns_x_bytes(j.mp, j.np) + which * 4l * j.mp * j.mp); }
 
-__device__ __forceinline__ int ns_job(const NsParams& p, int block) {
-  int lo = 0, hi = p.n;
-  while (hi - lo > 1) { const int m = (lo + hi) >> 1; if (p.job[m].first <= block) lo = m; else hi = m; }
-  return lo;
+// blocks of a matrix in a launch of each kind
+__host__ __device__ __forceinline__ long ns_blocks(const NsJob& j, int kind, int side, int span) {
+  const long tm = j.mp / side, tn = j.np / side, lower = tm * (tm + 1) / 2, all = tm * tn;
+  switch (kind) {
+    case NS_NORM: return j.nb;
+    case NS_INIT: return (long)(j.mp / 64) * (j.np / 64);
+    case NS_LOWER: return lower;
+    case NS_ALL: return all;
+    case NS_STRIPS: return tm * ((tn + span - 1) / span);
+    default: return (kind < NS_SHARED + 2 ? lower : all) * j.share[kind - NS_SHARED];
+  }
+}
+__global__ __launch_bounds__(64) void k_ns_table(NsLoad l) {
+  const int i = threadIdx.x;
+  NsTable* t = l.table;
+  if (i < l.n) t->job[i] = l.job[i];
+  for (int kind = 0; kind < NS_KINDS; ++kind) {
+    long at = i < l.n ? ns_blocks(l.job[i], kind, l.side, l.span) : 0;
+    const long mine = at;
+    for (int o = 1; o < 64; o <<= 1) {                                   // sum over the lanes in front
+      const long v = __shfl_up(at, o);
+      if (i >= o) at += v;
+    }
+    t->first[kind][i] = i < l.n ? (int)(at - mine) : 0x7fffffff;
+    if (kind >= NS_SHARED) t->part[kind - NS_SHARED][i] = (int)(at - mine);
+  }
+}
+__device__ __forceinline__ int ns_job(const NsTable* t, int kind, int block, int& local) {
+  const int f = t->first[kind][threadIdx.x & 63];
+  const int id = 63 - __builtin_clzll(__ballot(f <= block));
+  local = block - __builtin_amdgcn_readlane(f, id);
+  return id;
 }
 __device__ __forceinline__ float ns_get(const void* p, long i, int dtype) {
   return dtype == CRAFT_PREC_F32 ? reinterpret_cast<const float*>(p)[i] : dtype == CRAFT_PREC_F16 ? (float)reinterpret_cast<const _Float16*>(p)[i] : (float)reinterpret_cast<const __bf16*>(p)[i];
@@ -70,34 +114,55 @@ __device__ __forceinline__ void ns_split(const float (&v)[8], _Float16* hi, _Flo
   *reinterpret_cast<f16x8*>(lo) = l;
 }
 
-// partial sums of squares: job.nb blocks share a matrix' rows
-__global__ __launch_bounds__(256) void k_ns_norm(NsParams p) {
-  __shared__ double red[4];
-  const int id = ns_job(p, blockIdx.x);
-  const NsJob& j = p.job[id];
-  const int q = blockIdx.x - j.first;
+// partial sums of squares: job.nb blocks share a matrix' pieces of 8192 columns of a row (of the whole matrix, where its rows are contiguous)
+__global__ __launch_bounds__(1024) void k_ns_norm(NsParams p) {
+  __shared__ double red[16];
+  int q;
+  const int id = ns_job(p.table, NS_NORM, blockIdx.x, q);
+  const NsJob j = p.table->job[id];
+  const bool flat = j.ld_src == j.cols;
+  const long rows = flat ? 1 : j.rows, cols = flat ? (long)j.rows * j.cols : j.cols, segs = (cols + 8191) >> 13, items = rows * segs;
   double s = 0.0;
-  const long total = (long)j.rows * j.cols;
-  for (long e = (long)q * 256 + threadIdx.x; e < total; e += (long)j.nb * 256) {
-    const long r = e / j.cols;
-    const double v = ns_get(j.src, r * j.ld_src + (e - r * j.cols), p.dtype);
-    s += v * v;
+  for (long e = q; e < items; e += j.nb) {
+    const long r = e / segs, c0 = (e - r * segs) * 8192 + threadIdx.x;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = c0 + 1024 * i < cols ? ns_get(j.src, r * j.ld_src + c0 + 1024 * i, p.dtype) : 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) s += (double)v[i] * (double)v[i];
   }
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o);
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) p.norm[id * NS_NORM_BLOCKS + q] = (red[0] + red[1]) + (red[2] + red[3]);
+  if (threadIdx.x == 0) {
+#pragma unroll
+    for (int w = 1; w < 16; ++w) s += red[w];
+    p.norm[id * NS_NORM_BLOCKS + q] = s;
+  }
+}
+
+// Operands lie in the order in which a wave reads them: 32 rows x 16 columns of one plane are 1 KiB, 16 bytes for each lane -- row lane & 31, columns
+// 8 (lane >> 5) .. + 7 -- so that a load of an MFMA operand is one contiguous KiB.  (Rows behind one another, a load touched 32 lines and used a quarter
+// of each, and 8 waves' lines overran the L1: X X^T of 128 x 2560 took 57 us.)  Element offset of the 8 columns at k (a multiple of 8) of a row:
+__device__ __forceinline__ long ns_at(int row, int k, int K) {
+  return (((long)(row >> 5) * (K >> 4) + (k >> 4)) * 64 + ((k >> 3) & 1) * 32 + (row & 31)) * 8;
 }
 
 // G -> X and X^T, a block per 64 x 64 tile of X
 __global__ __launch_bounds__(256) void k_ns_init(NsParams p) {
   __shared__ float t[64][65];
-  const int id = ns_job(p, blockIdx.x);
-  const NsJob& j = p.job[id];
-  const int q = blockIdx.x - j.first, tn = j.np >> 6, ti = (q / tn) * 64, tj = (q % tn) * 64;
-  double sum = 0.0;
-  for (int b = 0; b < j.nb; ++b) sum += p.norm[id * NS_NORM_BLOCKS + b];
+  __shared__ double red[4];
+  int q;
+  const int id = ns_job(p.table, NS_INIT, blockIdx.x, q);
+  const NsJob j = p.table->job[id];
+  const int tn = j.np >> 6, ti = (q / tn) * 64, tj = (q % tn) * 64;
+  double sum = (int)threadIdx.x < j.nb ? p.norm[id * NS_NORM_BLOCKS + threadIdx.x] : 0.0;
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) sum += __shfl_xor(sum, o);
+  if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
+  __syncthreads();
+  sum = (red[0] + red[1]) + (red[2] + red[3]);
   const float f = (float)((double)p.s_x / (sqrt(sum) + (double)p.eps));
   const bool flip = j.rows > j.cols;
   const int r0 = flip ? tj : ti, c0 = flip ? ti : tj;                    // the tile of G
@@ -111,43 +176,76 @@ __global__ __launch_bounds__(256) void k_ns_init(NsParams p) {
   _Float16* xt = ns_xt(p, j, 0);
   const long plane = (long)j.mp * j.np;
   for (int e = threadIdx.x; e < 512; e += 256) {
-    const int r = e >> 3, c = (e & 7) * 8;
+    const int r = e & 63, c = (e >> 6) * 8;
     float v[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = t[r][c + i];
-    _Float16* o = x + (long)(ti + r) * j.np + tj + c;
+    _Float16* o = x + ns_at(ti + r, tj + c, j.np);
     ns_split(v, o, o + plane);
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] = t[c + i][r];
-    o = xt + (long)(tj + r) * j.mp + ti + c;
+    o = xt + ns_at(tj + r, ti + c, j.mp);
     ns_split(v, o, o + plane);
   }
 }
 
-// One 64 x 64 tile of P Q^T, both read along their rows of K straight into MFMA operands (no operand is used twice within a wave, so LDS would not save
-// a load): the 8 waves of a block share K, their partial tiles are summed in LDS in the order of the waves.
-//   PHASE 0: A = X X^T;  1: B = b A + c A A^T;  2: X = a X + B (X^T)^T
-template <int PHASE>
-__global__ __launch_bounds__(512) void k_ns_product(NsParams p) {
-  extern __shared__ __align__(16) float part[];                          // [8][64][64]
-  const int id = ns_job(p, blockIdx.x);
-  const NsJob& j = p.job[id];
-  const int q = blockIdx.x - j.first, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
-  int ti, tj;
-  if constexpr (PHASE < 2) {                                             // lower tiles, row by row
-    ti = (int)((sqrtf(8.f * (float)q + 1.f) - 1.f) * 0.5f);
-    while ((ti + 1) * (ti + 2) / 2 <= q) ++ti;
-    while (ti * (ti + 1) / 2 > q) --ti;
-    tj = q - ti * (ti + 1) / 2;
-  } else {
-    const int tm = j.mp >> 6;
-    tj = q / tm;
-    ti = q - tj * tm;
+__device__ __forceinline__ void ns_lower(int q, int& ti, int& tj) {      // tile q of the lower triangle, row by row
+  ti = (int)((sqrtf(8.f * (float)q + 1.f) - 1.f) * 0.5f);
+  while ((ti + 1) * (ti + 2) / 2 <= q) ++ti;
+  while (ti * (ti + 1) / 2 > q) --ti;
+  tj = q - ti * (ti + 1) / 2;
+}
+// acc += one 16-step of a 32 x 32 product of two-plane operands (lo lo is below the sums' own rounding)
+__device__ __forceinline__ void ns_mma(const f16x8& ph, const f16x8& pl, const f16x8& qh, const f16x8& ql, f32x16& acc) {
+  at_mma(pl, qh, acc);
+  at_mma(ph, ql, acc);
+  at_mma(ph, qh, acc);
+}
+__device__ __forceinline__ f16x8 ns_ld(const _Float16* q) { return *reinterpret_cast<const f16x8*>(q); }
+
+// What leaves a finished tile t ([N][N + 1] in LDS): the last step's result to dst ...
+template <int N>
+__device__ __forceinline__ void ns_result(const NsParams& p, const NsJob& j, const float* t, int ti, int tj, int tid, int threads) {
+  const bool flip = j.rows > j.cols;
+  const int r0 = (flip ? tj : ti) * N, c0 = (flip ? ti : tj) * N;
+  for (int e = tid; e < N * N; e += threads) {
+    const int r = e / N, c = e % N;
+    if (r0 + r < j.rows && c0 + c < j.cols) ns_put(j.dst, (long)(r0 + r) * j.ld_dst + c0 + c, p.dtype, flip ? t[c * (N + 1) + r] : t[r * (N + 1) + c]);
   }
-  const int K = PHASE == 0 ? j.np : j.mp;
-  const _Float16* P = PHASE == 0 ? ns_x(p, j) : ns_a(p, j, PHASE - 1);
-  const _Float16* Q = PHASE == 2 ? ns_xt(p, j, p.flip) : P;
-  const long pp = PHASE == 0 ? (long)j.mp * j.np : (long)j.mp * j.mp, qp = PHASE == 1 ? pp : (long)j.mp * j.np;
+}
+// ... or the tile as planes at (ti, tj) of `out` (rows of K) and its transpose at (tj, ti) of `outt` (rows of Kt)
+template <int N>
+__device__ __forceinline__ void ns_planes(const float* t, _Float16* out, int K, long plane, _Float16* outt, int Kt, int ti, int tj, int tid, int threads) {
+#pragma unroll 1
+  for (int e = tid; e < N * N / 8; e += threads) {
+    const int row = e % N, c = (e / N) * 8;
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = t[row * (N + 1) + c + i];
+    _Float16* o = out + ns_at(ti * N + row, tj * N + c, K);
+    ns_split(v, o, o + plane);
+    if (outt) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) v[i] = t[(c + i) * (N + 1) + row];
+      o = outt + ns_at(tj * N + row, ti * N + c, Kt);
+      ns_split(v, o, o + plane);
+    }
+  }
+}
+
+// ---- matrices whose smaller side is at most 256: two launches a step, bound by the launches' and loads' latency
+// A = X X^T, a block per 64 x 64 tile: the 8 waves share K and read both operands straight into MFMA operands (a wave would use none twice, so LDS would
+// not save a load); their partial tiles are summed in LDS in the order of the waves.
+__global__ __launch_bounds__(512) void k_ns_gram(NsParams p) {
+  extern __shared__ __align__(16) float part[];                          // [8][64][64]
+  int q;
+  const NsJob j = p.table->job[ns_job(p.table, NS_LOWER, blockIdx.x, q)];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
+  int ti, tj;
+  ns_lower(q, ti, tj);
+  const int K = j.np;
+  const _Float16* X = ns_x(p, j);
+  const long plane = (long)j.mp * j.np;
   const int nk = K >> 4, k0 = nk * wave / 8, k1 = nk * (wave + 1) / 8;
   f32x16 acc[2][2];
 #pragma unroll
@@ -156,26 +254,33 @@ __global__ __launch_bounds__(512) void k_ns_product(NsParams p) {
     for (int b = 0; b < 2; ++b)
 #pragma unroll
       for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.f;
-  const _Float16* pr = P + (long)(ti * 64 + (lane & 31)) * K + 8 * h;
-  const _Float16* qr = Q + (long)(tj * 64 + (lane & 31)) * K + 8 * h;
-#pragma unroll 2
-  for (int k = k0; k < k1; ++k) {
-    f16x8 ph[2], pl[2], qh[2], ql[2];
-#pragma unroll
-    for (int a = 0; a < 2; ++a) {
-      ph[a] = *reinterpret_cast<const f16x8*>(pr + (long)a * 32 * K + 16 * k);
-      pl[a] = *reinterpret_cast<const f16x8*>(pr + (long)a * 32 * K + 16 * k + pp);
-      qh[a] = *reinterpret_cast<const f16x8*>(qr + (long)a * 32 * K + 16 * k);
-      ql[a] = *reinterpret_cast<const f16x8*>(qr + (long)a * 32 * K + 16 * k + qp);
-    }
+  // a diagonal tile has one operand
+  const bool diag = ti == tj;
+  const _Float16* pr = X + ns_at(ti * 64, 0, K) + lane * 8;
+  const _Float16* qr = X + ns_at(tj * 64, 0, K) + lane * 8;
+  const long half = (long)(K >> 4) * 512;                                // 32 rows on
+  f16x8 f[2][2][2], g[2][2][2];                                          // [P, Q][32 rows][plane]; the next step's on their way
+  auto fetch = [&](int k) {
 #pragma unroll
     for (int a = 0; a < 2; ++a)
 #pragma unroll
-      for (int b = 0; b < 2; ++b) {
-        at_mma(pl[a], qh[b], acc[a][b]);
-        at_mma(ph[a], ql[b], acc[a][b]);
-        at_mma(ph[a], qh[b], acc[a][b]);
+      for (int e = 0; e < 2; ++e) {
+        g[0][a][e] = ns_ld(pr + a * half + (long)k * 512 + e * plane);
+        if (!diag) g[1][a][e] = ns_ld(qr + a * half + (long)k * 512 + e * plane);
       }
+  };
+  if (k0 < k1) fetch(k0);
+#pragma unroll 1
+  for (int k = k0; k < k1; ++k) {
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) { f[0][a][e] = g[0][a][e]; f[1][a][e] = diag ? g[0][a][e] : g[1][a][e]; }
+    if (k + 1 < k1) fetch(k + 1);
+#pragma unroll
+    for (int a = 0; a < 2; ++a)
+#pragma unroll
+      for (int b = 0; b < 2; ++b) ns_mma(f[0][a][0], f[0][a][1], f[1][b][0], f[1][b][1], acc[a][b]);
   }
   float* mine = part + wave * 4096;
 #pragma unroll
@@ -185,7 +290,6 @@ __global__ __launch_bounds__(512) void k_ns_product(NsParams p) {
 #pragma unroll
       for (int r = 0; r < 16; ++r) mine[(32 * a + acc_row(r) + 4 * h) * 64 + 32 * b + (lane & 31)] = acc[a][b][r];
   __syncthreads();
-  // thread: row tid / 8, 8 columns
   const int row = tid >> 3, c = (tid & 7) * 8;
   float v[8];
 #pragma unroll
@@ -194,53 +298,259 @@ __global__ __launch_bounds__(512) void k_ns_product(NsParams p) {
   for (int w = 0; w < 8; ++w)
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] += part[w * 4096 + row * 64 + c + i];
-  const int gi = ti * 64 + row, gj = tj * 64 + c;
-  if constexpr (PHASE == 0) {
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] *= p.c1;
-  } else if constexpr (PHASE == 1) {
-    const f16x8 oh = *reinterpret_cast<const f16x8*>(P + (long)gi * K + gj), ol = *reinterpret_cast<const f16x8*>(P + (long)gi * K + gj + pp);
-#pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = p.c0 * ((float)oh[i] + (float)ol[i]) + p.c1 * v[i];
-  } else {
-    // the old X: every thread reads its column group of X^T's rows
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const _Float16* o = Q + (long)(gj + i) * K + gi;
-      v[i] = p.c0 * ((float)o[0] + (float)o[qp]) + p.c1 * v[i];
-    }
-  }
   __syncthreads();                                                       // (all partial tiles are read: the first becomes the finished tile)
 #pragma unroll
-  for (int i = 0; i < 8; ++i) part[row * 65 + c + i] = v[i];
+  for (int i = 0; i < 8; ++i) part[row * 65 + c + i] = v[i] * p.c1;
   __syncthreads();
-  if (PHASE == 2 && p.last) {
-    const bool flip = j.rows > j.cols;
-    const int r0 = flip ? tj * 64 : ti * 64, c0 = flip ? ti * 64 : tj * 64;
-    for (int e = tid; e < 4096; e += 512) {
-      const int r = e >> 6, cc = e & 63;
-      if (r0 + r < j.rows && c0 + cc < j.cols) ns_put(j.dst, (long)(r0 + r) * j.ld_dst + c0 + cc, p.dtype, flip ? part[cc * 65 + r] : part[r * 65 + cc]);
-    }
-    return;
+  _Float16* A = ns_a(p, j, 0);
+  ns_planes<64>(part, A, j.mp, (long)j.mp * j.mp, ti == tj ? nullptr : A, j.mp, ti, tj, tid, 512);
+}
+
+// X <- a X + (b A + c A A) X, a block per 64 rows and p.span tiles of 64 columns of X: it first makes its 64 rows of B = b A + c A A in LDS (the product
+// A A again in every block of the same rows: m is small, and a launch of its own would cost more), then multiplies them with X^T's rows.  What it reads
+// was written by other dies a launch ago, so a load takes microseconds: all that the first part needs is asked for at once, its 64 rows of A by LDS-DMA,
+// each wave's own 32 rows into registers.
+constexpr int NS_UPD_B = 2 * 64 * 256 * 2, NS_UPD_LDS = 2 * NS_UPD_B;
+__global__ __launch_bounds__(512) void k_ns_update(NsParams p) {
+  extern __shared__ __align__(16) unsigned char lds[];
+  unsigned char* bt = lds + NS_UPD_B;                                    // B's 64 rows; in front of them A's, later the tile of X
+  float* part = reinterpret_cast<float*>(lds);                           // [2][64][65]
+  const unsigned lds0 = (unsigned)(size_t)(CRAFT_LDS unsigned char*)lds;
+  int q;
+  const NsJob j = p.table->job[ns_job(p.table, NS_STRIPS, blockIdx.x, q)];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l31 = lane & 31;
+  const int tm = j.mp >> 6, ti = q % tm, tj0 = (q / tm) * p.span, tj1 = min(tj0 + p.span, j.np >> 6);
+  const int K = j.mp, nk = K >> 4;
+  const _Float16* A = ns_a(p, j, 0);
+  const _Float16* XT = ns_xt(p, j, p.flip);
+  const long pa = (long)K * K, px = (long)K * j.np;
+  // 32-row blocks 2 ti and 2 ti + 1 of A, as they lie: [plane][32 rows][16 columns] x 1 KiB
+  const int pl = nk * 2048;                                              // bytes of a plane of 64 rows
+  for (int i = wave; i < 4 * nk; i += 8) {
+    const int e = i / (2 * nk), r = i - e * 2 * nk;
+    const unsigned long base = (unsigned long)(A + ns_at(64 * ti, 0, K) + e * pa + (long)r * 512);
+    u32x4_at d;
+    d[0] = __builtin_amdgcn_readfirstlane((unsigned)base);
+    d[1] = __builtin_amdgcn_readfirstlane((unsigned)(base >> 32));
+    d[2] = 0xffffffffu;
+    d[3] = 0x00020000u;
+    TileCopy<_Float16, 32, 128, 4>::one(d, (unsigned)lane * 16u, lds0 + (unsigned)(i * 1024));
   }
-  float u[8];                                                            // the tile's transpose: row `row`, 8 columns
+  const int sa = wave & 1, sb = (wave >> 1) & 1, half = wave >> 2, nh = nk >> 1, kh0 = half * nh;
+  f16x8 xh[8], xl[8];
+  auto fetch = [&](int tj) {
+    const _Float16* xr = XT + ns_at(64 * tj + 32 * sb, 0, K) + (long)kh0 * 512 + lane * 8;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) u[i] = part[(c + i) * 65 + row];
-  if constexpr (PHASE < 2) {
-    _Float16* out = ns_a(p, j, PHASE);
-    const long plane = (long)j.mp * j.mp;
-    _Float16* o = out + (long)gi * j.mp + gj;
-    ns_split(v, o, o + plane);
-    if (ti != tj) {
-      o = out + (long)(tj * 64 + row) * j.mp + ti * 64 + c;
-      ns_split(u, o, o + plane);
+    for (int k = 0; k < 8; ++k)
+      if (k < nh) { xh[k] = ns_ld(xr + k * 512); xl[k] = ns_ld(xr + k * 512 + px); }
+  };
+  fetch(tj0);
+  const bool makes = 32 * wave < K;
+  const _Float16* cr = A + ns_at(32 * wave, 0, K) + lane * 8;
+  f16x8 ch[4], cl[4];
+  auto columns = [&](int k) {
+#pragma unroll
+    for (int u = 0; u < 4; ++u) { ch[u] = ns_ld(cr + (long)(k + u) * 512); cl[u] = ns_ld(cr + (long)(k + u) * 512 + pa); }
+  };
+  if (makes) columns(0);
+  wait_copies();
+  __syncthreads();
+  // ---- wave w: columns 32 w .. of the 64 rows of B, as the transposed product (B is symmetric): lane = row, registers = columns
+  if (makes) {
+    f32x16 acc[2];
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[b][r] = 0.f;
+#pragma unroll 1
+    for (int k = 0; k < nk; k += 4) {                                    // (nk is a multiple of 4)
+      f16x8 dh[4], dl[4];
+#pragma unroll
+      for (int u = 0; u < 4; ++u) { dh[u] = ch[u]; dl[u] = cl[u]; }
+      if (k + 4 < nk) columns(k + 4);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int b = 0; b < 2; ++b) {
+          const unsigned char* ir = lds + (b * nk + k + u) * 1024 + lane * 16;
+          ns_mma(dh[u], dl[u], *reinterpret_cast<const f16x8*>(ir), *reinterpret_cast<const f16x8*>(ir + pl), acc[b]);
+        }
     }
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        // columns 32 wave + 8 g + 4 h .. of row l31 of block b
+        const int at = (b * nk + 2 * wave + (g >> 1)) * 1024 + (g & 1) * 512 + l31 * 16 + 8 * h;
+        const f16x4 oh = *reinterpret_cast<const f16x4*>(lds + at), ol = *reinterpret_cast<const f16x4*>(lds + at + pl);
+        f16x4 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const float v = p.b0 * ((float)oh[e] + (float)ol[e]) + p.b1 * acc[b][4 * g + e];
+          hi[e] = (_Float16)v;
+          lo[e] = (_Float16)(v - (float)hi[e]);
+        }
+        *reinterpret_cast<f16x4*>(bt + at) = hi;
+        *reinterpret_cast<f16x4*>(bt + at + pl) = lo;
+      }
+  }
+  __syncthreads();
+  // ---- the products: wave = (32 x 32 part of the tile, half of K); the next tile's rows of X^T are asked for behind this one's products
+  const unsigned char* bl = bt + (sa * nk + kh0) * 1024 + lane * 16;
+#pragma unroll 1
+  for (int tj = tj0; tj < tj1; ++tj) {
+    f32x16 acc;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+      if (k < nh) ns_mma(*reinterpret_cast<const f16x8*>(bl + k * 1024), *reinterpret_cast<const f16x8*>(bl + k * 1024 + pl), xh[k], xl[k], acc);
+    if (tj + 1 < tj1) fetch(tj + 1);
+    if (tj > tj0) __syncthreads();                                        // (the last tile has left `part`)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) part[half * 64 * 65 + (32 * sa + acc_row(r) + 4 * h) * 65 + 32 * sb + l31] = acc[r];
+    __syncthreads();
+    const int row = tid & 63, c = (tid >> 6) * 8;
+    const _Float16* old = ns_x(p, j) + ns_at(64 * ti + row, 64 * tj + c, j.np);       // (only this block touches its tile of X)
+    const f16x8 oh = ns_ld(old), ol = ns_ld(old + px);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      float* t = part + row * 65 + c + i;
+      t[0] = p.c0 * ((float)oh[i] + (float)ol[i]) + p.c1 * (t[0] + t[64 * 65]);
+    }
+    __syncthreads();
+    if (p.last) ns_result<64>(p, j, part, ti, tj, tid, 512);
+    else ns_planes<64>(part, ns_x(p, j), j.np, px, ns_xt(p, j, p.flip ^ 1), j.mp, ti, tj, tid, 512);
+  }
+}
+
+// ---- larger matrices: three launches a step, bound by the matrix units.  128 x 128 tiles, 4 waves of 64 x 64 each (12 MFMAs for 8 operand reads),
+// 32 columns of K at a time by LDS-DMA into two stages, two blocks to a compute unit.
+//   PHASE 0: A = X X^T;  1: B = b A + c A A;  2: X <- a X + B X.   MODE 0: whole tiles;  1: job.share[PHASE] shares of K, each leaving an fp32 tile;  2: their sum
+constexpr int NS_BIG_TILE = 128 * 64, NS_BIG_STAGE = 4 * NS_BIG_TILE, NS_BIG_LDS = 128 * 129 * 4 > 2 * NS_BIG_STAGE ? 128 * 129 * 4 : 2 * NS_BIG_STAGE;
+template <int PHASE, int MODE>
+__global__ __launch_bounds__(256, 2) void k_ns_big(NsParams p) {
+  extern __shared__ __align__(16) unsigned char lds[];
+  const unsigned lds0 = (unsigned)(size_t)(CRAFT_LDS unsigned char*)lds;
+  const int block = MODE == 2 ? blockIdx.x : xcd_chunk(blockIdx.x, gridDim.x);
+  int q, split = 0;
+  const int id = ns_job(p.table, MODE == 1 ? NS_SHARED + PHASE : PHASE < 2 ? NS_LOWER : NS_ALL, block, q);
+  const NsJob j = p.table->job[id];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l31 = lane & 31;
+  const int splits = MODE == 0 ? 1 : j.share[PHASE];
+  if (MODE == 1) { split = q % splits; q /= splits; }
+  int ti, tj;
+  if constexpr (PHASE < 2) ns_lower(q, ti, tj);
+  else { const int tm = j.mp >> 7; tj = q / tm; ti = q - tj * tm; }
+  const int K = PHASE == 0 ? j.np : j.mp;
+  const _Float16* P = PHASE == 0 ? ns_x(p, j) : ns_a(p, j, PHASE - 1);
+  const _Float16* Q = PHASE == 2 ? ns_xt(p, j, p.flip) : P;
+  const long pp = PHASE == 0 ? (long)j.mp * j.np : (long)j.mp * j.mp, qp = PHASE == 1 ? pp : (long)j.mp * j.np;
+  const int wa = wave >> 1, wb = wave & 1;
+  f32x16 acc[2][2];
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) acc[a][b][r] = 0.f;
+  // a partial tile: [wave][a][b][r / 4][lane][4]
+  float* part = p.part + ((long)p.table->part[PHASE][id] + (long)q * splits) * 16384 + wave * 4096 + lane * 4;
+  if constexpr (MODE < 2) {
+    // a stage: [P hi, P lo, Q hi, Q lo][32-row block][16 columns] x 1 KiB; wave w copies the blocks w
+    const _Float16* src[4] = {P + ns_at(ti * 128, 0, K), P + pp + ns_at(ti * 128, 0, K), Q + ns_at(tj * 128, 0, K), Q + qp + ns_at(tj * 128, 0, K)};
+    const int nk = K >> 5, k0 = nk * split / splits, k1 = nk * (split + 1) / splits;
+    const unsigned voff = (unsigned)wave * (unsigned)(K >> 4) * 1024u + (unsigned)lane * 16u;
+    auto stage = [&](int buf, int k) {
+#pragma unroll
+      for (int s = 0; s < 4; ++s) {
+        const unsigned long base = (unsigned long)(src[s] + (long)k * 1024);
+        u32x4_at d;
+        d[0] = __builtin_amdgcn_readfirstlane((unsigned)base);
+        d[1] = __builtin_amdgcn_readfirstlane((unsigned)(base >> 32));
+        d[2] = 0xffffffffu;
+        d[3] = 0x00020000u;
+#pragma unroll
+        for (int u = 0; u < 2; ++u)
+          TileCopy<_Float16, 32, 128, 4>::one(d, voff + u * 1024u, lds0 + (unsigned)(buf * NS_BIG_STAGE + s * NS_BIG_TILE + wave * 2048 + u * 1024));
+      }
+    };
+    if (k0 < k1) stage(0, k0);
+    for (int k = k0; k < k1; ++k) {
+      const int buf = (k - k0) & 1;
+      wait_copies();
+      __syncthreads();
+      if (k + 1 < k1) stage(buf ^ 1, k + 1);
+      const unsigned char* t = lds + buf * NS_BIG_STAGE + lane * 16;
+#pragma unroll
+      for (int ks = 0; ks < 2; ++ks) {
+        f16x8 ph[2], pl[2], qh[2], ql[2];
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+          const unsigned char* r = t + ((2 * wa + a) * 2 + ks) * 1024;
+          const unsigned char* c = t + ((2 * wb + a) * 2 + ks) * 1024;
+          ph[a] = *reinterpret_cast<const f16x8*>(r);
+          pl[a] = *reinterpret_cast<const f16x8*>(r + NS_BIG_TILE);
+          qh[a] = *reinterpret_cast<const f16x8*>(c + 2 * NS_BIG_TILE);
+          ql[a] = *reinterpret_cast<const f16x8*>(c + 3 * NS_BIG_TILE);
+        }
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int b = 0; b < 2; ++b) ns_mma(ph[a], pl[a], qh[b], ql[b], acc[a][b]);
+      }
+    }
+    if constexpr (MODE == 1) {
+      part += (long)split * 16384;
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<f32x4*>(part + ((a * 2 + b) * 4 + g) * 256) = f32x4{acc[a][b][4 * g], acc[a][b][4 * g + 1], acc[a][b][4 * g + 2], acc[a][b][4 * g + 3]};
+      return;
+    }
+    __syncthreads();
   } else {
-    const long plane = (long)j.mp * j.np;
-    _Float16* o = ns_x(p, j) + (long)gi * j.np + gj;
-    ns_split(v, o, o + plane);
-    o = ns_xt(p, j, p.flip ^ 1) + (long)(tj * 64 + row) * j.mp + ti * 64 + c;
-    ns_split(u, o, o + plane);
+    for (int s = 0; s < splits; ++s)                                     // in their order
+#pragma unroll
+      for (int a = 0; a < 2; ++a)
+#pragma unroll
+        for (int b = 0; b < 2; ++b)
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            const f32x4 v = *reinterpret_cast<const f32x4*>(part + (long)s * 16384 + ((a * 2 + b) * 4 + g) * 256);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[a][b][4 * g + e] += v[e];
+          }
+  }
+  float* t = reinterpret_cast<float*>(lds);
+#pragma unroll
+  for (int a = 0; a < 2; ++a)
+#pragma unroll
+    for (int b = 0; b < 2; ++b)
+#pragma unroll
+      for (int r = 0; r < 16; ++r) t[(64 * wa + 32 * a + acc_row(r) + 4 * h) * 129 + 64 * wb + 32 * b + l31] = acc[a][b][r] * p.c1;
+  __syncthreads();
+  if constexpr (PHASE > 0) {                                             // the old value: A's tile, or X's (only this block touches it)
+    const _Float16* O = PHASE == 1 ? P : ns_x(p, j);
+    const int ld = PHASE == 1 ? K : j.np;
+    const long plane = PHASE == 1 ? pp : qp;
+    for (int e = tid; e < 2048; e += 256) {
+      const int row = e & 127, c = (e >> 7) * 8;
+      const _Float16* o = O + ns_at(ti * 128 + row, tj * 128 + c, ld);
+      const f16x8 oh = ns_ld(o), ol = ns_ld(o + plane);
+#pragma unroll
+      for (int i = 0; i < 8; ++i) t[row * 129 + c + i] += p.c0 * ((float)oh[i] + (float)ol[i]);
+    }
+    __syncthreads();
+  }
+  if (PHASE == 2 && p.last) ns_result<128>(p, j, t, ti, tj, tid, 256);
+  else if constexpr (PHASE == 2) ns_planes<128>(t, ns_x(p, j), j.np, qp, ns_xt(p, j, p.flip ^ 1), j.mp, ti, tj, tid, 256);
+  else {
+    _Float16* out = ns_a(p, j, PHASE);
+    ns_planes<128>(t, out, j.mp, (long)j.mp * j.mp, ti == tj ? nullptr : out, j.mp, ti, tj, tid, 256);
   }
 }
 
@@ -301,72 +611,107 @@ static int muon_launch(MuonParams& p, const long* segs, const float* scales, int
 
 using namespace craft;
 
-extern "C" int craft_orthogonalize(const long* jobs, int n, const float* coeffs, int steps, float eps, float s_x, float s_a, float s_b, int dtype, void* ws,
-                                   long ws_bytes, void* stream) {
-  if (!jobs || !coeffs || n <= 0 || n > NS_MAX_JOBS || steps < 1 || steps > 64 || dtype < 0 || dtype > 2) return CRAFT_ERR_ARG;
-  if (!(eps >= 0.f) || !(s_x > 0.f) || !(s_a > 0.f) || !(s_b > 0.f) || (reinterpret_cast<uintptr_t>(ws) & 255) || !ws) return CRAFT_ERR_ARG;
-  NsParams p = {};
-  p.n = n; p.dtype = dtype; p.eps = eps; p.s_x = s_x;
-  p.norm = reinterpret_cast<double*>(ws);
-  long at = (long)n * NS_NORM_BLOCKS * 8;
-  p.ws = reinterpret_cast<unsigned char*>(ws);
-  long lower = 0, tiles = 0, norms = 0;
-  for (int i = 0; i < n; ++i) {
-    const long* d = jobs + 6 * i;                                        // src, ld_src, dst, ld_dst, rows, cols
-    NsJob& j = p.job[i];
-    if (!d[0] || !d[2] || d[4] <= 0 || d[5] <= 0 || d[1] < 0 || d[3] < d[5]) return CRAFT_ERR_ARG;
-    if (d[4] > 65536 || d[5] > 1l << 24 || (d[5] > 65536 && d[4] > 65536)) return CRAFT_ERR_UNSUPPORTED;
-    j.src = reinterpret_cast<const void*>(d[0]); j.ld_src = d[1]; j.dst = reinterpret_cast<void*>(d[2]); j.ld_dst = d[3];
-    j.rows = (int)d[4]; j.cols = (int)d[5];
-    const int m = j.rows < j.cols ? j.rows : j.cols, nn = j.rows < j.cols ? j.cols : j.rows;
-    if (m > 32768) return CRAFT_ERR_UNSUPPORTED;
-    j.mp = (m + 63) / 64 * 64; j.np = (nn + 63) / 64 * 64;
-    j.ws = at;
-    at += ns_bytes(j.mp, j.np);
-    const long el = (long)j.rows * j.cols;
-    j.nb = (int)(el / 8192 < 1 ? 1 : el / 8192 > NS_NORM_BLOCKS ? NS_NORM_BLOCKS : el / 8192);
-    norms += j.nb;
-    lower += (long)(j.mp / 64) * (j.mp / 64 + 1) / 2;
-    tiles += (long)(j.mp / 64) * (j.np / 64);
-  }
-  if (at > ws_bytes) return CRAFT_ERR_ARG;
-  if (lower > 0x7fffffffL || tiles > 0x7fffffffL) return CRAFT_ERR_UNSUPPORTED;
-  const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  auto number = [&](int what) {                                          // first blocks: 0 norms, 1 lower tiles, 2 all tiles
-    int first = 0;
-    for (int i = 0; i < n; ++i) {
-      NsJob& j = p.job[i];
-      const int tm = j.mp / 64, tn = j.np / 64;
-      j.first = first;
-      first += what == 0 ? j.nb : what == 1 ? tm * (tm + 1) / 2 : tm * tn;
-    }
+namespace craft {
+// one set of launches: matrices that are all small or all large
+static int ns_run(NsLoad& l, NsParams& p, const float* coeffs, int steps, float s_a, float s_b, hipStream_t s) {
+  auto count = [&](int kind) {
+    long c = 0;
+    for (int i = 0; i < l.n; ++i) c += ns_blocks(l.job[i], kind, l.side, l.span);
+    return c;
   };
-  constexpr int LDS = 8 * 4096 * 4;
-  const void* kernels[3] = {reinterpret_cast<const void*>(k_ns_product<0>), reinterpret_cast<const void*>(k_ns_product<1>), reinterpret_cast<const void*>(k_ns_product<2>)};
-  for (const void* k : kernels) HIP_CHECK_RET(hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, LDS));
-  number(0);
-  hipLaunchKernelGGL(k_ns_norm, dim3((unsigned)norms), dim3(256), 0, s, p);
+  if (l.big) {
+    // shares of K for tiles too few to fill the card: as many blocks as it holds at once (two to a compute unit), at least 256 columns of K each
+    const long tiles[3] = {count(NS_LOWER), count(NS_LOWER), count(NS_ALL)};
+    for (int i = 0; i < l.n; ++i)
+      for (int ph = 0; ph < 3; ++ph) {
+        const long most = (ph == 0 ? l.job[i].np : l.job[i].mp) / 256, want = 512 / tiles[ph];
+        const long v = want < most ? want : most;
+        l.job[i].share[ph] = (short)(v < 1 ? 1 : v);
+      }
+  } else {
+    // a block's column tiles: one while the card holds a block for each, then as many as keep about two blocks to a compute unit
+    const long v = (count(NS_ALL) + 511) / 512;
+    l.span = p.span = (int)(v < 1 ? 1 : v > 16 ? 16 : v);
+  }
+  for (int kind = 0; kind < NS_KINDS; ++kind)
+    if (count(kind) > 0x7ffffffeL) return CRAFT_ERR_UNSUPPORTED;
+  auto go = [&](auto tag, int kind, int threads, int lds) {
+    constexpr auto kernel = decltype(tag)::value;
+    if (lds > 0) if (const int rc = allow_lds<kernel>(lds)) return rc;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)count(kind)), dim3(threads), lds, s, p);
+    return (int)hipGetLastError();
+  };
+#define NS_TRY(x) do { const int rc_ = (x); if (rc_) return rc_; } while (0)
+  hipLaunchKernelGGL(k_ns_table, dim3(1), dim3(64), 0, s, l);
   HIP_CHECK_RET(hipGetLastError());
-  number(2);
-  hipLaunchKernelGGL(k_ns_init, dim3((unsigned)tiles), dim3(256), 0, s, p);
-  HIP_CHECK_RET(hipGetLastError());
+  NS_TRY(go(KernelTag<k_ns_norm>(), NS_NORM, 1024, 0));
+  NS_TRY(go(KernelTag<k_ns_init>(), NS_INIT, 256, 0));
+  // a product of the larger ones: whole tiles, or shares of K and their sum
+  auto product = [&](auto whole, auto shared, auto sum, int ph) {
+    const int kind = ph < 2 ? NS_LOWER : NS_ALL;
+    if (count(NS_SHARED + ph) == count(kind)) return go(whole, kind, 256, NS_BIG_LDS);
+    const int rc = go(shared, NS_SHARED + ph, 256, NS_BIG_LDS);
+    return rc ? rc : go(sum, kind, 256, NS_BIG_LDS);
+  };
   for (int t = 0; t < steps; ++t) {
     const float a = coeffs[3 * t], b = coeffs[3 * t + 1], c = coeffs[3 * t + 2];
     p.flip = t & 1;
     p.last = t == steps - 1;
-    number(1);
-    p.c0 = 0.f; p.c1 = s_a / (s_x * s_x);
-    hipLaunchKernelGGL(k_ns_product<0>, dim3((unsigned)lower), dim3(512), LDS, s, p);
-    HIP_CHECK_RET(hipGetLastError());
-    p.c0 = b * s_b / s_a; p.c1 = c * s_b / (s_a * s_a);
-    hipLaunchKernelGGL(k_ns_product<1>, dim3((unsigned)lower), dim3(512), LDS, s, p);
-    HIP_CHECK_RET(hipGetLastError());
-    number(2);
-    p.c0 = p.last ? a / s_x : a; p.c1 = (p.last ? 1.f / s_x : 1.f) / s_b;   // B X carries s_b s_x; the last one leaves without a scale
-    hipLaunchKernelGGL(k_ns_product<2>, dim3((unsigned)tiles), dim3(512), LDS, s, p);
-    HIP_CHECK_RET(hipGetLastError());
+    const float gram = s_a / (p.s_x * p.s_x), b0 = b * s_b / s_a, b1 = c * s_b / (s_a * s_a);
+    const float x0 = p.last ? a / p.s_x : a, x1 = (p.last ? 1.f / p.s_x : 1.f) / s_b;      // B X carries s_b s_x; the last one leaves without a scale
+    if (!l.big) {
+      p.c1 = gram;
+      NS_TRY(go(KernelTag<k_ns_gram>(), NS_LOWER, 512, 8 * 4096 * 4));
+      p.c0 = x0; p.c1 = x1; p.b0 = b0; p.b1 = b1;
+      NS_TRY(go(KernelTag<k_ns_update>(), NS_STRIPS, 512, NS_UPD_LDS));
+      continue;
+    }
+    p.c0 = 0.f; p.c1 = gram;
+    NS_TRY(product(KernelTag<k_ns_big<0, 0>>(), KernelTag<k_ns_big<0, 1>>(), KernelTag<k_ns_big<0, 2>>(), 0));
+    p.c0 = b0; p.c1 = b1;
+    NS_TRY(product(KernelTag<k_ns_big<1, 0>>(), KernelTag<k_ns_big<1, 1>>(), KernelTag<k_ns_big<1, 2>>(), 1));
+    p.c0 = x0; p.c1 = x1;
+    NS_TRY(product(KernelTag<k_ns_big<2, 0>>(), KernelTag<k_ns_big<2, 1>>(), KernelTag<k_ns_big<2, 2>>(), 2));
   }
+#undef NS_TRY
   return 0;
+}
+}  // namespace craft
+
+extern "C" int craft_orthogonalize(const long* jobs, int n, const float* coeffs, int steps, float eps, float s_x, float s_a, float s_b, int dtype, void* ws,
+                                   long ws_bytes, void* stream) {
+  if (!jobs || !coeffs || n <= 0 || steps < 1 || steps > 64 || dtype < 0 || dtype > 2) return CRAFT_ERR_ARG;
+  if (!(eps >= 0.f) || !(s_x > 0.f) || !(s_a > 0.f) || !(s_b > 0.f) || (reinterpret_cast<uintptr_t>(ws) & 255) || !ws) return CRAFT_ERR_ARG;
+  const bool big = (jobs[4] < jobs[5] ? jobs[4] : jobs[5]) > NS_SMALL;
+  if (n > (big ? NS_MAX_BIG : NS_MAX_JOBS)) return CRAFT_ERR_ARG;
+  NsLoad l = {};
+  NsParams p = {};
+  l.n = n; l.big = big; l.side = big ? 128 : 64; l.span = 1;
+  l.table = reinterpret_cast<NsTable*>(ws);
+  p.table = l.table; p.dtype = dtype; p.eps = eps; p.s_x = s_x; p.span = 1;
+  p.ws = reinterpret_cast<unsigned char*>(ws);
+  p.norm = reinterpret_cast<double*>(p.ws + NS_TABLE_BYTES);
+  long at = NS_TABLE_BYTES + (long)n * NS_NORM_BLOCKS * 8;
+  const int pad = l.side;
+  for (int i = 0; i < n; ++i) {
+    const long* d = jobs + 6 * i;                                        // src, ld_src, dst, ld_dst, rows, cols
+    NsJob& j = l.job[i];
+    if (!d[0] || !d[2] || d[4] <= 0 || d[5] <= 0 || d[1] < 0 || d[3] < d[5]) return CRAFT_ERR_ARG;
+    const long m = d[4] < d[5] ? d[4] : d[5], nn = d[4] < d[5] ? d[5] : d[4];
+    if (m > 32768 || nn > 1l << 22) return CRAFT_ERR_UNSUPPORTED;
+    if ((m > NS_SMALL) != big) return CRAFT_ERR_ARG;
+    j.src = reinterpret_cast<const void*>(d[0]); j.ld_src = d[1]; j.dst = reinterpret_cast<void*>(d[2]); j.ld_dst = d[3];
+    j.rows = (int)d[4]; j.cols = (int)d[5];
+    j.mp = (int)((m + pad - 1) / pad * pad); j.np = (int)((nn + pad - 1) / pad * pad);
+    j.ws = at;
+    at += ns_bytes(j.mp, j.np);
+    const long el = m * nn;
+    j.nb = (short)(el / 8192 < 1 ? 1 : el / 8192 > NS_NORM_BLOCKS ? NS_NORM_BLOCKS : el / 8192);
+    j.share[0] = j.share[1] = j.share[2] = 1;
+  }
+  if (at + (big ? NS_PART_BYTES : 0) > ws_bytes) return CRAFT_ERR_ARG;
+  p.part = reinterpret_cast<float*>(p.ws + at);
+  return ns_run(l, p, coeffs, steps, s_a, s_b, reinterpret_cast<hipStream_t>(stream));
 }
 
 extern "C" int craft_muon_momentum(const float* grad, float* buf, float* update, const long* segs, int n, float momentum, int nesterov, const void* state,

@@ -765,7 +765,7 @@ def layer_norm_bwd(x: torch.Tensor, weight: Optional[torch.Tensor], bias_type: O
 # ------------------------------------------------------------------------------------------------
 NEWTON_SCHULZ = (3.4445, -4.7750, 2.0315)        # the quintic that takes (0, 1] near 1 in 5 steps
 ORTHOGONALIZE_MAX_SIDE = 32768                   # the smaller side of a matrix
-_ORTHOGONALIZE_JOBS = 60                         # matrices of one set of launches
+_ORTHOGONALIZE_SMALL = 256                       # smaller sides up to here take the kernels that live on latency: 60 matrices to a set of launches, else 16
 
 
 @functools.lru_cache(maxsize=64)
@@ -804,8 +804,8 @@ def orthogonalize(mats: Sequence[torch.Tensor], steps: int = 5, coeffs=NEWTON_SC
     for g in mats:
         if g.dim() != 2 or g.dtype not in DTYPE_CODE:
             raise hip.CraftHipError(f"orthogonalize: fp32, fp16 or bf16 matrices, not {list(g.shape)} of {g.dtype}")
-        if min(g.shape) > ORTHOGONALIZE_MAX_SIDE or max(g.shape) > 1 << 24:
-            raise hip.CraftHipError(f"orthogonalize: {list(g.shape)}: the smaller side up to {ORTHOGONALIZE_MAX_SIDE}, the larger up to 2^24")
+        if min(g.shape) > ORTHOGONALIZE_MAX_SIDE or max(g.shape) > 1 << 22:
+            raise hip.CraftHipError(f"orthogonalize: {list(g.shape)}: the smaller side up to {ORTHOGONALIZE_MAX_SIDE}, the larger up to 2^22")
     if out is None:
         out = [torch.empty(g.shape, device=g.device, dtype=g.dtype) for g in mats]
     else:
@@ -820,16 +820,20 @@ def orthogonalize(mats: Sequence[torch.Tensor], steps: int = 5, coeffs=NEWTON_SC
     import ctypes
     flat = hip.carray(ctypes.c_float, [x for r in rows for x in r])
     with torch.no_grad(), _on(device):
-        for code in sorted({DTYPE_CODE[g.dtype] for g in mats}):
-            todo = [(g, o) for g, o in zip(mats, out) if DTYPE_CODE[g.dtype] == code and g.numel()]
-            for i in range(0, len(todo), _ORTHOGONALIZE_JOBS):
-                jobs, keep, nbytes = [], [], 0
-                for g, o in todo[i:i + _ORTHOGONALIZE_JOBS]:
+        groups = {}
+        for g, o in zip(mats, out):
+            if g.numel():
+                groups.setdefault((DTYPE_CODE[g.dtype], min(g.shape) > _ORTHOGONALIZE_SMALL), []).append((g, o))
+        for (code, large), todo in groups.items():
+            most, pad = (16, 128) if large else (60, 64)
+            for i in range(0, len(todo), most):
+                jobs, keep, nbytes = [], [], 8192 + ((32 << 20) if large else 0)
+                for g, o in todo[i:i + most]:
                     if (g.stride(1) != 1 and g.shape[1] > 1) or g.stride(0) < 0:
                         g = g.contiguous()
                         keep.append(g)
-                    m, k = (round_up(x, 64) for x in sorted(g.shape))
-                    nbytes += 256 + 12 * m * k + 8 * m * m
+                    m, k = (round_up(x, pad) for x in sorted(g.shape))
+                    nbytes += 2048 + 12 * m * k + 8 * m * m
                     jobs += [g.data_ptr(), g.stride(0), o.data_ptr(), max(o.stride(0), o.shape[1]), *g.shape]
                 ws = torch.empty(nbytes, device=device, dtype=torch.uint8)
                 call("craft_orthogonalize", hip.carray(ctypes.c_long, jobs), len(jobs) // 6, flat, steps, float(eps), *scales, code, ws, nbytes)

@@ -683,10 +683,11 @@ int craft_attention_bwd(const void* q, const void* k, const void* v, const void*
                         int split_group, void* dq, void* dk, void* dv, void* ws, long ws_bytes, void* stream);
 
 /* A list of matrices orthogonalised: X = G / (|G|_F + eps), then `steps` times X <- a X + (b A + c A A) X with A = X X^T (from the smaller side).
- * jobs: n x 6 host longs {src, ld_src, dst, ld_dst, rows, cols} (device pointers; strides in elements, columns contiguous; dst may be src), n <= 60,
- * min(rows, cols) <= 32768.  coeffs: steps x {a, b, c}.  The products are fp32-class: operands in two fp16 planes of the value times s_x (X), s_a (A),
+ * jobs: n x 6 host longs {src, ld_src, dst, ld_dst, rows, cols} (device pointers; strides in elements, columns contiguous; dst may be src); the
+ * smaller sides of a list are either all at most 256 (n <= 60) or all larger (n <= 16, at most 32768); the larger sides at most 2^22.  coeffs: steps x {a, b, c}.  The products are fp32-class: operands in two fp16 planes of the value times s_x (X), s_a (A),
  * s_b (b A + c A A), powers of two that keep every entry below 65504.
- * ws (256-byte aligned): n * 256 bytes, then per matrix with m = min, k = max of (rows, cols), both rounded up to 64: 12 m k + 8 m m bytes. */
+ * ws (256-byte aligned): 8192 + n * 2048 bytes, then per matrix with m = min, k = max of (rows, cols), both rounded up to 64 (larger: 128): 12 m k + 8 m m
+ * bytes, then for the larger ones 32 MiB. */
 int craft_orthogonalize(const long* jobs, int n, const float* coeffs, int steps, float eps, float s_x, float s_a, float s_b, int dtype, void* ws,
                         long ws_bytes, void* stream);
 /* The optimizer around it, over n ranges {offset, length} (host longs) of flat fp32 buffers; state: the record of craft_loss_scale_update (a skipped step

@@ -85,7 +85,7 @@ def test_entry_points_check_their_arguments():
     def run(job=(buf, 8, buf, 8, 8, 8), n=1, coeffs=co, steps=1, eps=1e-7, s=(1.0, 1.0, 1.0), dt=0, ws=buf, nbytes=1 << 20):
         return lib.craft_orthogonalize((ctypes.c_long * 6)(*job), n, coeffs, steps, eps, *s, dt, ws, nbytes, None)
     assert run(n=0) == ARG and run(n=61) == ARG and run(steps=0) == ARG and run(coeffs=None) == ARG and run(eps=-1.0) == ARG and run(dt=3) == ARG
-    assert run(s=(0.0, 1.0, 1.0)) == ARG and run(ws=None) == ARG and run(ws=buf + 16) == ARG and run(nbytes=256 + 20 * 4096 - 1) == ARG
+    assert run(s=(0.0, 1.0, 1.0)) == ARG and run(ws=None) == ARG and run(ws=buf + 16) == ARG and run(nbytes=8192 + 2048 + 20 * 4096 - 1) == ARG
     assert run((0, 8, buf, 8, 8, 8)) == ARG and run((buf, 8, buf, 7, 8, 8)) == ARG and run((buf, 8, buf, 8, 0, 8)) == ARG
     assert run((buf, 40000, buf, 40000, 40000, 40000)) == UNSUPPORTED
     seg = (ctypes.c_long * 2)(0, 8)
@@ -108,9 +108,11 @@ def test_against_64_bits(device, t, shapes):
 @gpu
 def test_large(device):
     from craft_amd import ops
-    for shape in ((700, 2300), (1024, 1024), (1100, 640)):
+    for shape in ((700, 2300), (1024, 1024), (1100, 640), (257, 257), (300, 5000), (256, 9000)):
         mats = grads([shape])
         check(ops.orthogonalize(mats), mats)
+    mats = grads([(300, 700), (64, 64), (1000, 520), (100, 3000), (400, 400)])
+    check(ops.orthogonalize(mats), mats)
 
 
 @gpu
