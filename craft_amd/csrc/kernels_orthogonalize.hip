@@ -3,8 +3,8 @@
 //   X <- G / (|G|_F + eps)   (G transposed where it has more rows than columns: m <= n)
 //   steps times:  A = X X^T,   B = b A + c A^2,   X <- a X + B X
 //
-// Each step is three products whose sizes differ from matrix to matrix, and each needs the one before it: two or three launches a step for the WHOLE
-// list, a block per output tile of any matrix.  A and A^2 are symmetric: only their lower
+// Each step is three products whose sizes differ from matrix to matrix, and each needs the one before it: three launches a step for the WHOLE list, a
+// block per output tile of any matrix.  A and A^2 are symmetric: only their lower
 // tiles are computed, and written twice.
 //
 // Arithmetic: fp32-class.  Every operand is two fp16 planes hi + lo of its value times a power of two (22 bits and more: the scales bring the largest
@@ -34,7 +34,7 @@ struct NsJob {
   short share[3];                                    // k_ns_big: shares of K in each of the three products
 };
 // The kinds of launches: a matrix' first block in each.
-enum { NS_NORM, NS_INIT, NS_LOWER, NS_ALL, NS_STRIPS, NS_SHARED, NS_KINDS = NS_SHARED + 3 };
+enum { NS_NORM, NS_INIT, NS_LOWER, NS_ALL, NS_SHARED, NS_KINDS = NS_SHARED + 3 };
 // The matrices' table, in the workspace: kernel arguments lie in host memory, and a search through them costs a kernel ten microseconds.  Which matrix a
 // block belongs to: every lane holds one first block, a ballot finds the last that is not behind.
 struct NsTable {
@@ -42,14 +42,13 @@ struct NsTable {
   int first[NS_KINDS][64];                           // (INT_MAX behind the last)
   int part[3][64];                                   // k_ns_big: a matrix' first partial tile
 };
-struct NsLoad { NsJob job[NS_MAX_JOBS]; int n, span, side, big; NsTable* table; };
+struct NsLoad { NsJob job[NS_MAX_JOBS]; int n, side, big; NsTable* table; };
 struct NsParams {
   const NsTable* table;
-  int dtype, span;                                   // span: column tiles of a block of k_ns_update
+  int dtype;
   unsigned char* ws;
   double* norm;                                      // [jobs][NS_NORM_BLOCKS]
   float eps, c0, c1;                                 // epilogue: c0 * (old value) + c1 * (product), scales folded in
-  float b0, b1;                                      // k_ns_update: the same for B
   float s_x;                                         // scale of X
   float* part;                                       // k_ns_big: partial tiles
   int last, flip;                                    // last step; which of the two X^T is read
@@ -65,14 +64,13 @@ __device__ __forceinline__ _Float16* ns_xt(const NsParams& p, const NsJob& j, in
 __device__ __forceinline__ _Float16* ns_a(const NsParams& p, const NsJob& j, int which) { return reinterpret_cast<_Float16*>(p.ws + j.ws + 3 * ns_x_bytes(j.mp, j.np) + which * 4l * j.mp * j.mp); }
 
 // blocks of a matrix in a launch of each kind
-__host__ __device__ __forceinline__ long ns_blocks(const NsJob& j, int kind, int side, int span) {
+__host__ __device__ __forceinline__ long ns_blocks(const NsJob& j, int kind, int side) {
   const long tm = j.mp / side, tn = j.np / side, lower = tm * (tm + 1) / 2, all = tm * tn;
   switch (kind) {
     case NS_NORM: return j.nb;
     case NS_INIT: return (long)(j.mp / 64) * (j.np / 64);
     case NS_LOWER: return lower;
     case NS_ALL: return all;
-    case NS_STRIPS: return tm * ((tn + span - 1) / span);
     default: return (kind < NS_SHARED + 2 ? lower : all) * j.share[kind - NS_SHARED];
   }
 }
@@ -81,7 +79,7 @@ __global__ __launch_bounds__(64) void k_ns_table(NsLoad l) {
   NsTable* t = l.table;
   if (i < l.n) t->job[i] = l.job[i];
   for (int kind = 0; kind < NS_KINDS; ++kind) {
-    long at = i < l.n ? ns_blocks(l.job[i], kind, l.side, l.span) : 0;
+    long at = i < l.n ? ns_blocks(l.job[i], kind, l.side) : 0;
     const long mine = at;
     for (int o = 1; o < 64; o <<= 1) {                                   // sum over the lanes in front
       const long v = __shfl_up(at, o);
@@ -233,9 +231,10 @@ __device__ __forceinline__ void ns_planes(const float* t, _Float16* out, int K, 
   }
 }
 
-// ---- matrices whose smaller side is at most 256: two launches a step, bound by the launches' and loads' latency
-// A = X X^T, a block per 64 x 64 tile: the 8 waves share K and read both operands straight into MFMA operands (a wave would use none twice, so LDS would
+// ---- matrices whose smaller side is at most 256: bound by the launches' and loads' latency
+// PHASE 0: A = X X^T, 1: B = b A + c A A, a block per 64 x 64 tile: the 8 waves share K and read both operands straight into MFMA operands (a wave would use none twice, so LDS would
 // not save a load); their partial tiles are summed in LDS in the order of the waves.
+template <int PHASE>
 __global__ __launch_bounds__(512) void k_ns_gram(NsParams p) {
   extern __shared__ __align__(16) float part[];                          // [8][64][64]
   int q;
@@ -243,9 +242,9 @@ __global__ __launch_bounds__(512) void k_ns_gram(NsParams p) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5;
   int ti, tj;
   ns_lower(q, ti, tj);
-  const int K = j.np;
-  const _Float16* X = ns_x(p, j);
-  const long plane = (long)j.mp * j.np;
+  const int K = PHASE == 0 ? j.np : j.mp;
+  const _Float16* X = PHASE == 0 ? ns_x(p, j) : ns_a(p, j, 0);
+  const long plane = (long)j.mp * K;
   const int nk = K >> 4, k0 = nk * wave / 8, k1 = nk * (wave + 1) / 8;
   f32x16 acc[2][2];
 #pragma unroll
@@ -298,130 +297,71 @@ __global__ __launch_bounds__(512) void k_ns_gram(NsParams p) {
   for (int w = 0; w < 8; ++w)
 #pragma unroll
     for (int i = 0; i < 8; ++i) v[i] += part[w * 4096 + row * 64 + c + i];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) v[i] *= p.c1;
+  if constexpr (PHASE == 1) {
+    const _Float16* old = X + ns_at(64 * ti + row, 64 * tj + c, K);
+    const f16x8 oh = ns_ld(old), ol = ns_ld(old + plane);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] += p.c0 * ((float)oh[i] + (float)ol[i]);
+  }
   __syncthreads();                                                       // (all partial tiles are read: the first becomes the finished tile)
 #pragma unroll
-  for (int i = 0; i < 8; ++i) part[row * 65 + c + i] = v[i] * p.c1;
+  for (int i = 0; i < 8; ++i) part[row * 65 + c + i] = v[i];
   __syncthreads();
-  _Float16* A = ns_a(p, j, 0);
+  _Float16* A = ns_a(p, j, PHASE);
   ns_planes<64>(part, A, j.mp, (long)j.mp * j.mp, ti == tj ? nullptr : A, j.mp, ti, tj, tid, 512);
 }
 
-// X <- a X + (b A + c A A) X, a block per 64 rows and p.span tiles of 64 columns of X: it first makes its 64 rows of B = b A + c A A in LDS (the product
-// A A again in every block of the same rows: m is small, and a launch of its own would cost more), then multiplies them with X^T's rows.  What it reads
-// was written by other dies a launch ago, so a load takes microseconds: all that the first part needs is asked for at once, its 64 rows of A by LDS-DMA,
-// each wave's own 32 rows into registers.
-constexpr int NS_UPD_B = 2 * 64 * 256 * 2, NS_UPD_LDS = 2 * NS_UPD_B;
-__global__ __launch_bounds__(512) void k_ns_update(NsParams p) {
-  extern __shared__ __align__(16) unsigned char lds[];
-  unsigned char* bt = lds + NS_UPD_B;                                    // B's 64 rows; in front of them A's, later the tile of X
-  float* part = reinterpret_cast<float*>(lds);                           // [2][64][65]
-  const unsigned lds0 = (unsigned)(size_t)(CRAFT_LDS unsigned char*)lds;
+// X <- a X + B X, a block per 64 x 64 tile: 4 waves of 32 x 32, operands from memory straight into registers, the next step's on their way.  Small blocks:
+// four and more to a compute unit hide one another's latency.  (With B made again in every block, instead of in a launch of its own, the
+// model's step took 40 us here instead of 7 + 28.)
+__global__ __launch_bounds__(256) void k_ns_update(NsParams p) {
+  __shared__ float part[64 * 65];
   int q;
-  const NsJob j = p.table->job[ns_job(p.table, NS_STRIPS, blockIdx.x, q)];
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5, l31 = lane & 31;
-  const int tm = j.mp >> 6, ti = q % tm, tj0 = (q / tm) * p.span, tj1 = min(tj0 + p.span, j.np >> 6);
-  const int K = j.mp, nk = K >> 4;
-  const _Float16* A = ns_a(p, j, 0);
-  const _Float16* XT = ns_xt(p, j, p.flip);
-  const long pa = (long)K * K, px = (long)K * j.np;
-  // 32-row blocks 2 ti and 2 ti + 1 of A, as they lie: [plane][32 rows][16 columns] x 1 KiB
-  const int pl = nk * 2048;                                              // bytes of a plane of 64 rows
-  for (int i = wave; i < 4 * nk; i += 8) {
-    const int e = i / (2 * nk), r = i - e * 2 * nk;
-    const unsigned long base = (unsigned long)(A + ns_at(64 * ti, 0, K) + e * pa + (long)r * 512);
-    u32x4_at d;
-    d[0] = __builtin_amdgcn_readfirstlane((unsigned)base);
-    d[1] = __builtin_amdgcn_readfirstlane((unsigned)(base >> 32));
-    d[2] = 0xffffffffu;
-    d[3] = 0x00020000u;
-    TileCopy<_Float16, 32, 128, 4>::one(d, (unsigned)lane * 16u, lds0 + (unsigned)(i * 1024));
-  }
-  const int sa = wave & 1, sb = (wave >> 1) & 1, half = wave >> 2, nh = nk >> 1, kh0 = half * nh;
-  f16x8 xh[8], xl[8];
-  auto fetch = [&](int tj) {
-    const _Float16* xr = XT + ns_at(64 * tj + 32 * sb, 0, K) + (long)kh0 * 512 + lane * 8;
+  const NsJob j = p.table->job[ns_job(p.table, NS_ALL, blockIdx.x, q)];
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, h = lane >> 5, l31 = lane & 31, sa = wave & 1, sb = wave >> 1;
+  const int tm = j.mp >> 6, tj = q / tm, ti = q - tj * tm, K = j.mp, nk = K >> 4;
+  const long pb = (long)K * K, px = (long)K * j.np;
+  const _Float16* br = ns_a(p, j, 1) + ns_at(64 * ti + 32 * sa, 0, K) + lane * 8;
+  const _Float16* xr = ns_xt(p, j, p.flip) + ns_at(64 * tj + 32 * sb, 0, K) + lane * 8;
+  f32x16 acc;
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k < nh) { xh[k] = ns_ld(xr + k * 512); xl[k] = ns_ld(xr + k * 512 + px); }
-  };
-  fetch(tj0);
-  const bool makes = 32 * wave < K;
-  const _Float16* cr = A + ns_at(32 * wave, 0, K) + lane * 8;
-  f16x8 ch[4], cl[4];
-  auto columns = [&](int k) {
+  for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+  f16x8 f[2][4];                                                         // [step][B hi, B lo, X^T hi, X^T lo]
+  auto fetch = [&](int k) {
 #pragma unroll
-    for (int u = 0; u < 4; ++u) { ch[u] = ns_ld(cr + (long)(k + u) * 512); cl[u] = ns_ld(cr + (long)(k + u) * 512 + pa); }
-  };
-  if (makes) columns(0);
-  wait_copies();
-  __syncthreads();
-  // ---- wave w: columns 32 w .. of the 64 rows of B, as the transposed product (B is symmetric): lane = row, registers = columns
-  if (makes) {
-    f32x16 acc[2];
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) acc[b][r] = 0.f;
-#pragma unroll 1
-    for (int k = 0; k < nk; k += 4) {                                    // (nk is a multiple of 4)
-      f16x8 dh[4], dl[4];
-#pragma unroll
-      for (int u = 0; u < 4; ++u) { dh[u] = ch[u]; dl[u] = cl[u]; }
-      if (k + 4 < nk) columns(k + 4);
-#pragma unroll
-      for (int u = 0; u < 4; ++u)
-#pragma unroll
-        for (int b = 0; b < 2; ++b) {
-          const unsigned char* ir = lds + (b * nk + k + u) * 1024 + lane * 16;
-          ns_mma(dh[u], dl[u], *reinterpret_cast<const f16x8*>(ir), *reinterpret_cast<const f16x8*>(ir + pl), acc[b]);
-        }
+    for (int u = 0; u < 2; ++u) {
+      const long at = (long)(k + u) * 512;
+      f[u][0] = ns_ld(br + at); f[u][1] = ns_ld(br + at + pb); f[u][2] = ns_ld(xr + at); f[u][3] = ns_ld(xr + at + px);
     }
-#pragma unroll
-    for (int b = 0; b < 2; ++b)
-#pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        // columns 32 wave + 8 g + 4 h .. of row l31 of block b
-        const int at = (b * nk + 2 * wave + (g >> 1)) * 1024 + (g & 1) * 512 + l31 * 16 + 8 * h;
-        const f16x4 oh = *reinterpret_cast<const f16x4*>(lds + at), ol = *reinterpret_cast<const f16x4*>(lds + at + pl);
-        f16x4 hi, lo;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float v = p.b0 * ((float)oh[e] + (float)ol[e]) + p.b1 * acc[b][4 * g + e];
-          hi[e] = (_Float16)v;
-          lo[e] = (_Float16)(v - (float)hi[e]);
-        }
-        *reinterpret_cast<f16x4*>(bt + at) = hi;
-        *reinterpret_cast<f16x4*>(bt + at + pl) = lo;
-      }
-  }
-  __syncthreads();
-  // ---- the products: wave = (32 x 32 part of the tile, half of K); the next tile's rows of X^T are asked for behind this one's products
-  const unsigned char* bl = bt + (sa * nk + kh0) * 1024 + lane * 16;
+  };
+  fetch(0);
 #pragma unroll 1
-  for (int tj = tj0; tj < tj1; ++tj) {
-    f32x16 acc;
+  for (int k = 0; k < nk; k += 2) {                                      // (nk is a multiple of 4)
+    f16x8 g[2][4];
 #pragma unroll
-    for (int r = 0; r < 16; ++r) acc[r] = 0.f;
+    for (int u = 0; u < 2; ++u)
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
-      if (k < nh) ns_mma(*reinterpret_cast<const f16x8*>(bl + k * 1024), *reinterpret_cast<const f16x8*>(bl + k * 1024 + pl), xh[k], xl[k], acc);
-    if (tj + 1 < tj1) fetch(tj + 1);
-    if (tj > tj0) __syncthreads();                                        // (the last tile has left `part`)
+      for (int e = 0; e < 4; ++e) g[u][e] = f[u][e];
+    if (k + 2 < nk) fetch(k + 2);
 #pragma unroll
-    for (int r = 0; r < 16; ++r) part[half * 64 * 65 + (32 * sa + acc_row(r) + 4 * h) * 65 + 32 * sb + l31] = acc[r];
-    __syncthreads();
-    const int row = tid & 63, c = (tid >> 6) * 8;
+    for (int u = 0; u < 2; ++u) ns_mma(g[u][0], g[u][1], g[u][2], g[u][3], acc);
+  }
+#pragma unroll
+  for (int r = 0; r < 16; ++r) part[(32 * sa + acc_row(r) + 4 * h) * 65 + 32 * sb + l31] = acc[r] * p.c1;
+  __syncthreads();
+#pragma unroll
+  for (int e = tid; e < 512; e += 256) {
+    const int row = e & 63, c = (e >> 6) * 8;
     const _Float16* old = ns_x(p, j) + ns_at(64 * ti + row, 64 * tj + c, j.np);       // (only this block touches its tile of X)
     const f16x8 oh = ns_ld(old), ol = ns_ld(old + px);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      float* t = part + row * 65 + c + i;
-      t[0] = p.c0 * ((float)oh[i] + (float)ol[i]) + p.c1 * (t[0] + t[64 * 65]);
-    }
-    __syncthreads();
-    if (p.last) ns_result<64>(p, j, part, ti, tj, tid, 512);
-    else ns_planes<64>(part, ns_x(p, j), j.np, px, ns_xt(p, j, p.flip ^ 1), j.mp, ti, tj, tid, 512);
+    for (int i = 0; i < 8; ++i) part[row * 65 + c + i] += p.c0 * ((float)oh[i] + (float)ol[i]);
   }
+  __syncthreads();
+  if (p.last) ns_result<64>(p, j, part, ti, tj, tid, 256);
+  else ns_planes<64>(part, ns_x(p, j), j.np, px, ns_xt(p, j, p.flip ^ 1), j.mp, ti, tj, tid, 256);
 }
 
 // ---- larger matrices: three launches a step, bound by the matrix units.  128 x 128 tiles, 4 waves of 64 x 64 each (12 MFMAs for 8 operand reads),
@@ -616,7 +556,7 @@ namespace craft {
 static int ns_run(NsLoad& l, NsParams& p, const float* coeffs, int steps, float s_a, float s_b, hipStream_t s) {
   auto count = [&](int kind) {
     long c = 0;
-    for (int i = 0; i < l.n; ++i) c += ns_blocks(l.job[i], kind, l.side, l.span);
+    for (int i = 0; i < l.n; ++i) c += ns_blocks(l.job[i], kind, l.side);
     return c;
   };
   if (l.big) {
@@ -628,10 +568,6 @@ static int ns_run(NsLoad& l, NsParams& p, const float* coeffs, int steps, float 
         const long v = want < most ? want : most;
         l.job[i].share[ph] = (short)(v < 1 ? 1 : v);
       }
-  } else {
-    // a block's column tiles: one while the card holds a block for each, then as many as keep about two blocks to a compute unit
-    const long v = (count(NS_ALL) + 511) / 512;
-    l.span = p.span = (int)(v < 1 ? 1 : v > 16 ? 16 : v);
   }
   for (int kind = 0; kind < NS_KINDS; ++kind)
     if (count(kind) > 0x7ffffffeL) return CRAFT_ERR_UNSUPPORTED;
@@ -661,9 +597,11 @@ static int ns_run(NsLoad& l, NsParams& p, const float* coeffs, int steps, float 
     const float x0 = p.last ? a / p.s_x : a, x1 = (p.last ? 1.f / p.s_x : 1.f) / s_b;      // B X carries s_b s_x; the last one leaves without a scale
     if (!l.big) {
       p.c1 = gram;
-      NS_TRY(go(KernelTag<k_ns_gram>(), NS_LOWER, 512, 8 * 4096 * 4));
-      p.c0 = x0; p.c1 = x1; p.b0 = b0; p.b1 = b1;
-      NS_TRY(go(KernelTag<k_ns_update>(), NS_STRIPS, 512, NS_UPD_LDS));
+      NS_TRY(go(KernelTag<k_ns_gram<0>>(), NS_LOWER, 512, 8 * 4096 * 4));
+      p.c0 = b0; p.c1 = b1;
+      NS_TRY(go(KernelTag<k_ns_gram<1>>(), NS_LOWER, 512, 8 * 4096 * 4));
+      p.c0 = x0; p.c1 = x1;
+      NS_TRY(go(KernelTag<k_ns_update>(), NS_ALL, 256, 0));
       continue;
     }
     p.c0 = 0.f; p.c1 = gram;
@@ -686,9 +624,9 @@ extern "C" int craft_orthogonalize(const long* jobs, int n, const float* coeffs,
   if (n > (big ? NS_MAX_BIG : NS_MAX_JOBS)) return CRAFT_ERR_ARG;
   NsLoad l = {};
   NsParams p = {};
-  l.n = n; l.big = big; l.side = big ? 128 : 64; l.span = 1;
+  l.n = n; l.big = big; l.side = big ? 128 : 64;
   l.table = reinterpret_cast<NsTable*>(ws);
-  p.table = l.table; p.dtype = dtype; p.eps = eps; p.s_x = s_x; p.span = 1;
+  p.table = l.table; p.dtype = dtype; p.eps = eps; p.s_x = s_x;
   p.ws = reinterpret_cast<unsigned char*>(ws);
   p.norm = reinterpret_cast<double*>(p.ws + NS_TABLE_BYTES);
   long at = NS_TABLE_BYTES + (long)n * NS_NORM_BLOCKS * 8;

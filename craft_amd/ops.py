@@ -801,43 +801,58 @@ def orthogonalize(mats: Sequence[torch.Tensor], steps: int = 5, coeffs=NEWTON_SC
     if not 0 <= eps < float("inf"):
         raise hip.CraftHipError("orthogonalize: eps must be finite and not negative")
     mats = list(mats)
-    for g in mats:
-        if g.dim() != 2 or g.dtype not in DTYPE_CODE:
-            raise hip.CraftHipError(f"orthogonalize: fp32, fp16 or bf16 matrices, not {list(g.shape)} of {g.dtype}")
-        if min(g.shape) > ORTHOGONALIZE_MAX_SIDE or max(g.shape) > 1 << 22:
-            raise hip.CraftHipError(f"orthogonalize: {list(g.shape)}: the smaller side up to {ORTHOGONALIZE_MAX_SIDE}, the larger up to 2^22")
-    if out is None:
-        out = [torch.empty(g.shape, device=g.device, dtype=g.dtype) for g in mats]
-    else:
+    if out is not None:
         out = list(out)
-        if len(out) != len(mats) or any(o.shape != g.shape or o.dtype != g.dtype or o.device != g.device for o, g in zip(out, mats)):
+        if len(out) != len(mats):
             raise hip.CraftHipError("orthogonalize: out must be a list of the matrices' shapes, types and devices")
-        if any(o.numel() and (o.stride(1) != 1 and o.shape[1] > 1 or o.stride(0) < o.shape[1] and o.shape[0] > 1) for o in out):
-            raise hip.CraftHipError("orthogonalize: out needs contiguous columns")
-    if not mats:
-        return out
-    device = _on_device(*mats)
+    res, groups, device = [], {}, None
+    for i, g in enumerate(mats):                      # (a list of a model's matrices: a microsecond here is fifty)
+        shape, code = g.shape, DTYPE_CODE.get(g.dtype)
+        if len(shape) != 2 or code is None:
+            raise hip.CraftHipError(f"orthogonalize: fp32, fp16 or bf16 matrices, not {list(shape)} of {g.dtype}")
+        r, c = shape
+        small, large = (r, c) if r < c else (c, r)
+        if small > ORTHOGONALIZE_MAX_SIDE or large > 1 << 22:
+            raise hip.CraftHipError(f"orthogonalize: {list(shape)}: the smaller side up to {ORTHOGONALIZE_MAX_SIDE}, the larger up to 2^22")
+        if out is None:
+            o, ldo = None, c
+        else:
+            o = out[i]
+            if o.shape != shape or o.dtype != g.dtype or o.device != g.device:
+                raise hip.CraftHipError("orthogonalize: out must be a list of the matrices' shapes, types and devices")
+            ldo, so = o.stride()
+            if so != 1 and c > 1 or ldo < c and r > 1:
+                raise hip.CraftHipError("orthogonalize: out needs contiguous columns")
+            ldo = max(ldo, c)
+        if device is None:
+            device = _on_device(g)
+        elif g.device != device:
+            _on_device(mats[0], g)
+        if o is None:
+            o = torch.empty(shape, device=device, dtype=g.dtype)
+        res.append(o)
+        if small:
+            groups.setdefault((code, small > _ORTHOGONALIZE_SMALL), []).append((g, o, r, c, small, large, ldo))
     import ctypes
-    flat = hip.carray(ctypes.c_float, [x for r in rows for x in r])
-    with torch.no_grad(), _on(device):
-        groups = {}
-        for g, o in zip(mats, out):
-            if g.numel():
-                groups.setdefault((DTYPE_CODE[g.dtype], min(g.shape) > _ORTHOGONALIZE_SMALL), []).append((g, o))
-        for (code, large), todo in groups.items():
-            most, pad = (16, 128) if large else (60, 64)
-            for i in range(0, len(todo), most):
-                jobs, keep, nbytes = [], [], 8192 + ((32 << 20) if large else 0)
-                for g, o in todo[i:i + most]:
-                    if (g.stride(1) != 1 and g.shape[1] > 1) or g.stride(0) < 0:
-                        g = g.contiguous()
-                        keep.append(g)
-                    m, k = (round_up(x, pad) for x in sorted(g.shape))
-                    nbytes += 2048 + 12 * m * k + 8 * m * m
-                    jobs += [g.data_ptr(), g.stride(0), o.data_ptr(), max(o.stride(0), o.shape[1]), *g.shape]
-                ws = torch.empty(nbytes, device=device, dtype=torch.uint8)
-                call("craft_orthogonalize", hip.carray(ctypes.c_long, jobs), len(jobs) // 6, flat, steps, float(eps), *scales, code, ws, nbytes)
-    return out
+    if groups:
+        flat = hip.carray(ctypes.c_float, [x for row in rows for x in row])
+        with torch.no_grad(), _on(device):
+            for (code, large), todo in groups.items():
+                most, pad = (16, 128) if large else (60, 64)
+                for i in range(0, len(todo), most):
+                    jobs, keep, nbytes = [], [], 8192 + ((32 << 20) if large else 0)
+                    for g, o, r, c, m, k, ldo in todo[i:i + most]:
+                        ld, sc = g.stride()
+                        if (sc != 1 and c > 1) or ld < 0:
+                            g = g.contiguous()
+                            ld = c
+                            keep.append(g)
+                        m, k = (m + pad - 1) // pad * pad, (k + pad - 1) // pad * pad
+                        nbytes += 2048 + 12 * m * k + 8 * m * m
+                        jobs += (g.data_ptr(), ld, o.data_ptr(), ldo, r, c)
+                    ws = torch.empty(nbytes, device=device, dtype=torch.uint8)
+                    call("craft_orthogonalize", hip.carray(ctypes.c_long, jobs), len(jobs) // 6, flat, steps, float(eps), *scales, code, ws, nbytes)
+    return res
 
 
 # ------------------------------------------------------------------------------------------------
