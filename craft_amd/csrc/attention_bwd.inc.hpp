@@ -61,7 +61,11 @@ __global__ __launch_bounds__(256) void k_attention_dq(AttentionParams p) {
   frag_t qf[DP / 16], gf[DP / 16];
   load_own<T, DP>(reinterpret_cast<const T*>(p.q) + b * p.q_b + (long)i * p.q_n + head * p.q_h, p.D, h, qf);
   load_own<T, DP>(reinterpret_cast<const T*>(p.go) + b * p.go_b + (long)i * p.go_n + head * p.go_h, p.D, h, gf);
-  const float lse = p.lse[(long)bh * p.Nq + i], delta = p.delta[(long)bh * p.Nq + i];
+  float row[2] = {p.lse[(long)bh * p.Nq + i], p.delta[(long)bh * p.Nq + i]};
+  arrived(qf);
+  arrived(gf);
+  arrived(row);
+  const float lse = row[0], delta = row[1];
 
   int t0 = 0, t1 = p.causal ? (max(min(max(i_last + off + 1, prefix), p.Nk), 0) + TK - 1) / TK : (p.Nk + TK - 1) / TK;
   int4 qr = make_int4(0, 0, 0, 0), qrw = qr;
@@ -82,8 +86,14 @@ __global__ __launch_bounds__(256) void k_attention_dq(AttentionParams p) {
   vc.init(wave, lane, vst, nchunk);
   const unsigned char* kb = reinterpret_cast<const unsigned char*>(p.k) + (b * p.k_b + kvh * p.k_h) * (long)sizeof(T);
   const unsigned char* vb = reinterpret_cast<const unsigned char*>(p.v) + (b * p.v_b + kvh * p.v_h) * (long)sizeof(T);
-  auto range = [&](int t) { return join_ranges(rk, t * NB, min(t * NB + NB, kgroups) - 1); };
-  auto next = [&](int t) { if (rk) while (t < t1 && !ranges_meet(range(t), qr)) ++t; return t; };
+  auto next = [&](int t, int4& r) {
+    if (rk)
+      for (; t < t1; ++t) {
+        r = uniform_range(join_ranges(rk, t * NB, min(t * NB + NB, kgroups) - 1));
+        if (ranges_meet(r, qr)) break;
+      }
+    return t;
+  };
   auto stage = [&](int buf, int t) {
     const int valid = p.Nk - t * TK;
     const unsigned at = lds0 + (unsigned)buf * S::STAGE;
@@ -99,12 +109,13 @@ __global__ __launch_bounds__(256) void k_attention_dq(AttentionParams p) {
     for (int r = 0; r < 16; ++r) dq[d][r] = 0.f;
   const float slope2 = BIAS ? p.slopes[head] * 1.44269504088896f : 0.f;
 
-  int t = next(t0), buf = 0;
+  int4 kr = make_int4(0, 0, 0, 0), krn = kr;
+  int t = next(t0, kr), buf = 0;
   if (t < t1) stage(0, t);
   while (t < t1) {
     wait_copies();
     __syncthreads();
-    const int tn = next(t + 1);
+    const int tn = next(t + 1, krn);
     if (tn < t1) stage(buf ^ 1, tn);
     unsigned char* K = lds + buf * S::STAGE;
     unsigned char* V = K + S::TILE;
@@ -112,7 +123,6 @@ __global__ __launch_bounds__(256) void k_attention_dq(AttentionParams p) {
     const int k0 = t * TK;
     bool docmask = false, skip = k0 >= lim_hi;
     if (rk) {
-      const int4 kr = range(t);
       if (kr.z) { zero_rows<T, DP, TK>(K, ids, p.Nk - k0, tid, 256); __syncthreads(); }
       docmask = !one_document(kr, qrw);
       skip |= !ranges_meet(kr, qrw);
@@ -162,6 +172,7 @@ __global__ __launch_bounds__(256) void k_attention_dq(AttentionParams p) {
       }
     }
     t = tn;
+    kr = krn;
     buf ^= 1;
   }
   if (i0 + wave * 32 + (lane & 31) < p.Nq) {
@@ -206,6 +217,8 @@ __global__ __launch_bounds__(256) void k_attention_dkv(AttentionParams p) {
   frag_t kf[DP / 16], vf[DP / 16];
   load_own<T, DP>(reinterpret_cast<const T*>(p.k) + b * p.k_b + (long)key * p.k_n + kvh * p.k_h, p.D, h, kf);
   load_own<T, DP>(reinterpret_cast<const T*>(p.v) + b * p.v_b + (long)key * p.v_n + kvh * p.v_h, p.D, h, vf);
+  arrived(kf);
+  arrived(vf);
 
   int t0 = !p.causal || prefix > j0 ? 0 : min(max(j0 - off, 0), p.Nq) / TQ, t1 = (p.Nq + TQ - 1) / TQ;
   int4 kr = make_int4(0, 0, 0, 0), krw = kr;
@@ -224,8 +237,14 @@ __global__ __launch_bounds__(256) void k_attention_dkv(AttentionParams p) {
   TileCopy<T, DP, TQ, 4> qc, gc;
   qc.init(wave, lane, qst, nchunk);
   gc.init(wave, lane, gst, nchunk);
-  auto range = [&](int t) { return join_ranges(rq, t * NB, min(t * NB + NB, qgroups) - 1); };
-  auto next = [&](int t) { if (rq) while (t < t1 && !ranges_meet(range(t), kr)) ++t; return t; };
+  auto next = [&](int t, int4& r) {
+    if (rq)
+      for (; t < t1; ++t) {
+        r = uniform_range(join_ranges(rq, t * NB, min(t * NB + NB, qgroups) - 1));
+        if (ranges_meet(r, kr)) break;
+      }
+    return t;
+  };
   auto stage = [&](int buf, int head, int t) {
     const int valid = p.Nq - t * TQ;
     const unsigned at = lds0 + (unsigned)buf * S::STAGE;
@@ -245,14 +264,16 @@ __global__ __launch_bounds__(256) void k_attention_dkv(AttentionParams p) {
 #pragma unroll
     for (int r = 0; r < 16; ++r) dk[d][r] = dv[d][r] = 0.f;
 
-  int head = head0, t = next(t0), buf = 0;
+  int4 qr = make_int4(0, 0, 0, 0), qrn = qr;
+  int head = head0, t = next(t0, qr), buf = 0;
   const int tfirst = t;
+  const int4 qrfirst = qr;
   if (t < t1) stage(0, head, t);
   while (t < t1) {
     wait_copies();
     __syncthreads();
-    int tn = next(t + 1), headn = head;
-    if (tn >= t1 && head + 1 < head1) { tn = tfirst; headn = head + 1; }
+    int tn = next(t + 1, qrn), headn = head;
+    if (tn >= t1 && head + 1 < head1) { tn = tfirst; qrn = qrfirst; headn = head + 1; }
     if (tn < t1) stage(buf ^ 1, headn, tn);
     unsigned char* Q = lds + buf * S::STAGE;
     unsigned char* GO = Q + S::TILE;
@@ -262,7 +283,6 @@ __global__ __launch_bounds__(256) void k_attention_dkv(AttentionParams p) {
     const int i0 = t * TQ;
     bool docmask = false, skip = p.causal && prefix <= jw && i0 + TQ - 1 + off < jw;
     if (rq) {
-      const int4 qr = range(t);
       if (qr.z) { zero_rows<T, DP, TQ>(Q, ids, p.Nq - i0, tid, 256); zero_rows<T, DP, TQ>(GO, ids, p.Nq - i0, tid, 256); __syncthreads(); }
       docmask = !one_document(qr, krw);
       skip |= !ranges_meet(qr, krw);
@@ -318,6 +338,7 @@ __global__ __launch_bounds__(256) void k_attention_dkv(AttentionParams p) {
       }
     }
     t = tn;
+    qr = qrn;
     head = headn;
     buf ^= 1;
   }

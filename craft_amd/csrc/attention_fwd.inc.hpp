@@ -37,6 +37,13 @@ __global__ __launch_bounds__(256, 2) void k_attention_fwd(AttentionParams p) {
 
   frag_t qf[DP / 16];
   load_own<T, DP>(reinterpret_cast<const T*>(p.q) + b * p.q_b + (long)i * p.q_n + head * p.q_h, p.D, h, qf);
+  constexpr bool RAW = !CAP && !BIAS;           // scores stay products: the maximum is taken of them, the scale goes into the exponential's one fma
+  const float c2 = RAW ? fmaxf(fabsf(p.c2), 1e-30f) : 1.f;
+  if (RAW && p.c2 < 0.f) {
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks) qf[ks] = -qf[ks];
+  }
+  arrived(qf);
 
   int t0 = 0, t1 = p.causal ? (max(min(max(i_last + off + 1, prefix), p.Nk), 0) + TK - 1) / TK : (p.Nk + TK - 1) / TK;
   int4 qr = make_int4(0, 0, 0, 0), qrw = qr;
@@ -57,8 +64,15 @@ __global__ __launch_bounds__(256, 2) void k_attention_fwd(AttentionParams p) {
   vc.init(wave, lane, vst, nchunk);
   const unsigned char* kb = reinterpret_cast<const unsigned char*>(p.k) + (b * p.k_b + kvh * p.k_h) * (long)sizeof(T);
   const unsigned char* vb = reinterpret_cast<const unsigned char*>(p.v) + (b * p.v_b + kvh * p.v_h) * (long)sizeof(T);
-  auto range = [&](int t) { return join_ranges(rk, t * NB, min(t * NB + NB, kgroups) - 1); };
-  auto next = [&](int t) { if (rk) while (t < t1 && !ranges_meet(range(t), qr)) ++t; return t; };
+  // the next tile from t on that has one of the block's documents, and its range
+  auto next = [&](int t, int4& kr) {
+    if (rk)
+      for (; t < t1; ++t) {
+        kr = uniform_range(join_ranges(rk, t * NB, min(t * NB + NB, kgroups) - 1));
+        if (ranges_meet(kr, qr)) break;
+      }
+    return t;
+  };
   auto stage = [&](int buf, int t) {
     const int valid = p.Nk - t * TK;
     const unsigned at = lds0 + (unsigned)buf * S::STAGE;
@@ -75,12 +89,14 @@ __global__ __launch_bounds__(256, 2) void k_attention_fwd(AttentionParams p) {
   float m = -INFINITY, l = 0.f;                 // the running maximum (kept up to 2^8 below the true one) and this lane's share of the sum
   const float slope2 = BIAS ? p.slopes[head] * 1.44269504088896f : 0.f;
 
-  int t = next(t0), buf = 0;
+  const float thr = RAW ? 8.f / c2 : 8.f;
+  int4 kr = make_int4(0, 0, 0, 0), krn = kr;
+  int t = next(t0, kr), buf = 0;
   if (t < t1) stage(0, t);
   while (t < t1) {
     wait_copies();
     __syncthreads();                            // the tile is whole; everybody has left the other buffer
-    const int tn = next(t + 1);
+    const int tn = next(t + 1, krn);
     if (tn < t1) stage(buf ^ 1, tn);
     unsigned char* K = lds + buf * S::STAGE;
     unsigned char* V = K + S::TILE;
@@ -88,7 +104,6 @@ __global__ __launch_bounds__(256, 2) void k_attention_fwd(AttentionParams p) {
     const int k0 = t * TK;
     bool docmask = false, skip = k0 >= lim_hi;
     if (rk) {
-      const int4 kr = range(t);
       if (kr.z) { zero_rows<T, DP, TK>(V, ids, p.Nk - k0, tid, 256); __syncthreads(); }
       docmask = !one_document(kr, qrw);
       skip |= !ranges_meet(kr, qrw);
@@ -102,16 +117,18 @@ __global__ __launch_bounds__(256, 2) void k_attention_fwd(AttentionParams p) {
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks) at_mma(tile_row<T, DP>(K, 32 * kbk + (lane & 31), ks, h), qf[ks], x[kbk]);
       }
-      const float away = BIAS ? (float)(pos - k0 - 4 * h) : 0.f;
+      if constexpr (!RAW) {
+        const float away = BIAS ? (float)(pos - k0 - 4 * h) : 0.f;
 #pragma unroll
-      for (int kbk = 0; kbk < NB; ++kbk)
+        for (int kbk = 0; kbk < NB; ++kbk)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          float th;
-          float z = at_score<T, CAP>(p, x[kbk][r], th);
-          if constexpr (BIAS) z -= slope2 * fabsf(away - (float)(32 * kbk + acc_row(r)));
-          x[kbk][r] = z;
-        }
+          for (int r = 0; r < 16; ++r) {
+            float th;
+            float z = at_score<T, CAP>(p, x[kbk][r], th);
+            if constexpr (BIAS) z -= slope2 * fabsf(away - (float)(32 * kbk + acc_row(r)));
+            x[kbk][r] = z;
+          }
+      }
       if (k0 + TK > lim_lo) {
         const int room = lim - k0 - 4 * h;
 #pragma unroll
@@ -138,8 +155,8 @@ __global__ __launch_bounds__(256, 2) void k_attention_fwd(AttentionParams p) {
         for (int r = 0; r < 16; ++r) mt = fmaxf(mt, x[kbk][r]);
       mt = fmaxf(mt, at_other_half(mt));
       // the output is rescaled only when some query's maximum has grown by more than 2^8: until then its probabilities are merely larger than one
-      if (__ballot(mt > m + 8.f)) {
-        const float mn = fmaxf(m, mt), alpha = m == mn ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+      if (__ballot(mt > m + thr)) {
+        const float mn = fmaxf(m, mt), alpha = m == mn ? 1.f : __builtin_amdgcn_exp2f((m - mn) * c2);
         m = mn;
         l *= alpha;
 #pragma unroll
@@ -147,11 +164,11 @@ __global__ __launch_bounds__(256, 2) void k_attention_fwd(AttentionParams p) {
 #pragma unroll
           for (int r = 0; r < 16; ++r) o[d][r] *= alpha;
       }
-      const float ref = m == -INFINITY ? 0.f : m;
+      const float ref = m == -INFINITY ? 0.f : m * c2;
 #pragma unroll
       for (int kbk = 0; kbk < NB; ++kbk)
 #pragma unroll
-        for (int r = 0; r < 16; ++r) { x[kbk][r] = __builtin_amdgcn_exp2f(x[kbk][r] - ref); l += x[kbk][r]; }
+        for (int r = 0; r < 16; ++r) { x[kbk][r] = __builtin_amdgcn_exp2f(RAW ? fmaf(x[kbk][r], c2, -ref) : x[kbk][r] - ref); l += x[kbk][r]; }
 #pragma unroll
       for (int kbk = 0; kbk < NB; ++kbk)
 #pragma unroll
@@ -162,6 +179,7 @@ __global__ __launch_bounds__(256, 2) void k_attention_fwd(AttentionParams p) {
         }
     }
     t = tn;
+    kr = krn;
     buf ^= 1;
   }
 
@@ -182,7 +200,7 @@ __global__ __launch_bounds__(256, 2) void k_attention_fwd(AttentionParams p) {
           *reinterpret_cast<t4*>(orow + c) = w;
         }
       }
-    if (p.lse && h == 0) p.lse[(long)bh * p.Nq + i] = l > 0.f ? m + __log2f(l) : INFINITY;
+    if (p.lse && h == 0) p.lse[(long)bh * p.Nq + i] = l > 0.f ? m * c2 + __log2f(l) : INFINITY;
   }
 }
 

@@ -148,6 +148,14 @@ __device__ __forceinline__ void load_own(const T* row, int D, int h, typename At
   }
 }
 
+// Loads into registers have arrived behind this.  The compiler waits for a load where its value is first used; inside a loop that copies by LDS-DMA
+// (which it does not know of, and which its counter counts) such a wait would be for the copies just started as well.
+template <typename F, int N>
+__device__ __forceinline__ void arrived(F (&f)[N]) {
+#pragma unroll
+  for (int i = 0; i < N; ++i) asm volatile("" : "+v"(f[i]));
+}
+
 // LDS-DMA of ROWS rows (those from `valid` on repeat the last valid one; the chunks behind D repeat the last real one: both are only ever
 // multiplied by zeros or masked) by WAVES waves; this wave's share.  Issues only: wait for vmcnt and pass a barrier before reading.
 template <typename T, int DP, int ROWS, int WAVES>
@@ -221,6 +229,10 @@ __device__ __forceinline__ int4 join_ranges(const int4* r, int g0, int g1) {
     a.x = min(a.x, b.x); a.y = max(a.y, b.y); a.z |= b.z;
   }
   return a;
+}
+// the same as scalars: a range read inside the walk is read before the next tile's copies are started
+__device__ __forceinline__ int4 uniform_range(const int4& a) {
+  return make_int4(__builtin_amdgcn_readfirstlane(a.x), __builtin_amdgcn_readfirstlane(a.y), __builtin_amdgcn_readfirstlane(a.z), 0);
 }
 __device__ __forceinline__ bool ranges_meet(const int4& a, const int4& b) { return a.x <= b.y && b.x <= a.y; }
 __device__ __forceinline__ bool one_document(const int4& a, const int4& b) { return !a.z && !b.z && a.x == a.y && b.x == b.y && a.x == b.x; }

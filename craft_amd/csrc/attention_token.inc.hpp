@@ -40,7 +40,10 @@ __global__ __launch_bounds__((TokenShape<T, DP>::WAVES * 64)) void k_attention_t
   lim_lo = __builtin_amdgcn_readfirstlane(lim_lo); lim_hi = __builtin_amdgcn_readfirstlane(lim_hi);
   frag_t qf[DP / 16];
   load_own<T, DP>(reinterpret_cast<const T*>(p.q) + b * p.q_b + (long)i * p.q_n + head * p.q_h, p.D, h, qf);
-  const float slope2 = BIAS ? p.slopes[head] * 1.44269504088896f : 0.f;
+  float sl[1] = {BIAS ? p.slopes[head] * 1.44269504088896f : 0.f};
+  arrived(qf);
+  arrived(sl);
+  const float slope2 = sl[0];
 
   // tiles of this split: [a0, a1); of this wave: a0 + wave, + W, ...
   const int tiles = (p.Nk + 31) >> 5, per = (tiles + p.splits - 1) / p.splits;
