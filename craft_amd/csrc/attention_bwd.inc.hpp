@@ -45,7 +45,9 @@ __global__ __launch_bounds__(256) void k_attention_dq(AttentionParams p) {
   const unsigned lds0 = (unsigned)(size_t)(CRAFT_LDS unsigned char*)lds;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int nqt = (p.Nq + 127) >> 7;
-  const int id = xcd_chunk(blockIdx.x, gridDim.x), bh = id / nqt, qt = nqt - 1 - (id - bh * nqt);
+  int bh, qt;
+  block_of(p.B * p.H, nqt, bh, qt);
+  qt = nqt - 1 - qt;
   const int b = bh / p.H, head = bh - b * p.H, kvh = head / (p.H / p.Hk);
   const int off = p.Nk - p.Nq, i0 = qt * 128, i_last = min(i0 + 127, p.Nq - 1);
   const int prefix = p.prefix ? p.prefix[b] : 0;
@@ -205,7 +207,8 @@ __global__ __launch_bounds__(256) void k_attention_dkv(AttentionParams p) {
   const int nkt = (p.Nk + 127) >> 7, G = p.H / p.Hk;
   // part_k: one block per query head, whose results a second kernel sums over the group; else one block walks over the heads of its group
   const int heads = p.part_k ? p.H : p.Hk;
-  const int id = xcd_chunk(blockIdx.x, gridDim.x), bx = id / nkt, kt = id - bx * nkt;       // (the first keys of a causal row are the heaviest: first)
+  int bx, kt;
+  block_of(p.B * heads, nkt, bx, kt);           // (the first keys of a causal row are the heaviest)
   const int b = bx / heads, hx = bx - b * heads, kvh = p.part_k ? hx / G : hx;
   const int head0 = p.part_k ? hx : hx * G, head1 = p.part_k ? hx + 1 : hx * G + G;
   const int off = p.Nk - p.Nq, j0 = kt * 128, jw = j0 + wave * 32;

@@ -21,7 +21,9 @@ __global__ __launch_bounds__(256, 2) void k_attention_fwd(AttentionParams p) {
   const unsigned lds0 = (unsigned)(size_t)(CRAFT_LDS unsigned char*)lds;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int nqt = (p.Nq + 127) >> 7;
-  const int id = xcd_chunk(blockIdx.x, gridDim.x), bh = id / nqt, qt = nqt - 1 - (id - bh * nqt);     // (the last queries of a causal row are the heaviest: first)
+  int bh, qt;
+  block_of(p.B * p.H, nqt, bh, qt);
+  qt = nqt - 1 - qt;                            // (the last queries of a causal row are the heaviest)
   const int b = bh / p.H, head = bh - b * p.H, kvh = head / (p.H / p.Hk);
   const int off = p.Nk - p.Nq, i0 = qt * 128, i_last = min(i0 + 127, p.Nq - 1);
   const int prefix = p.prefix ? p.prefix[b] : 0;

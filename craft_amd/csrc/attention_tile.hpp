@@ -246,6 +246,22 @@ __device__ __forceinline__ float at_score(const AttentionParams& p, float s, flo
   return th * p.cap2;
 }
 
+// Which (head of the batch, tile) a block takes.  The blocks of a head share an XCD, whose L2 then holds that head's keys; and the tiles of all the heads
+// of an XCD come with the heaviest first (tile 0 is the heaviest): under a causal mask the last blocks to start are the shortest, and no compute unit is
+// left with a long one at the end.  Heads that do not divide by the 8 XCDs: head by head, in contiguous eighths of the list.
+__device__ __forceinline__ void block_of(int heads, int tiles, int& head, int& tile) {
+  const int total = heads * tiles, id = blockIdx.x;
+  if ((heads & 7) == 0) {
+    const int per = heads >> 3, slot = id >> 3;
+    tile = slot / per;
+    head = (id & 7) * per + slot - tile * per;
+  } else {
+    const int at = xcd_chunk(id, total);
+    head = at / tiles;
+    tile = at - head * tiles;
+  }
+}
+
 // token range of a walk: the first and the last tile of [t0, t1) whose documents meet `own`, over the whole block
 template <int THREADS>
 __device__ __forceinline__ void tiles_of_documents(const int4* r, int groups, int gpt, const int4& own, int& t0, int& t1, int tid, int* red) {
