@@ -29,15 +29,25 @@ __global__ __launch_bounds__(256) void k_attention_delta(AttentionParams p, floa
 }
 
 template <typename T, int DP> struct BwdShape {
-  static constexpr int TR = sizeof(T) == 2 ? 64 : 32;                     // rows of a tile
+  static constexpr int TR = sizeof(T) == 2 && DP < 128 ? 64 : 32;         // rows of a tile (128 columns in 64-row tiles: registers spill)
   static constexpr int TILE = TR * DP * (int)sizeof(T);
   static constexpr int STAGE = 2 * TILE + 3 * 256;                        // two operands; lse, delta, documents of 64 rows
   static constexpr int LDS = 2 * STAGE + 64;
 };
 
+// the key / value kernel's tiles.  Two 16-bit operands and two fp32 results of 128 columns leave no room for two waves to a SIMD in registers: there V is
+// read from LDS (the block's 128 keys stay there), and tiles are 32 rows so that two blocks share a compute unit (558 -> XXX us for the capped 4096-token step)
+template <typename T, int DP> struct DkvShape {
+  static constexpr bool VL = sizeof(T) == 2 && DP == 128;
+  static constexpr int TR = VL ? 32 : BwdShape<T, DP>::TR;
+  static constexpr int TILE = TR * DP * (int)sizeof(T);
+  static constexpr int STAGE = 2 * TILE + 3 * 256;
+  static constexpr int V = 2 * STAGE + 64, LDS = V + (VL ? 128 * DP * (int)sizeof(T) : 0);
+};
+
 // dq: lane = query
 template <typename T, int DP, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256) void k_attention_dq(AttentionParams p) {
+__global__ __launch_bounds__(256, (sizeof(T) == 2 || DP < 128 ? 2 : 1)) void k_attention_dq(AttentionParams p) {
   typedef BwdShape<T, DP> S;
   typedef typename AtFrag<T>::type frag_t;
   constexpr int TK = S::TR, NB = TK / 32;
@@ -197,8 +207,8 @@ __global__ __launch_bounds__(256) void k_attention_dq(AttentionParams p) {
 
 // dk, dv: lane = key
 template <typename T, int DP, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256) void k_attention_dkv(AttentionParams p) {
-  typedef BwdShape<T, DP> S;
+__global__ __launch_bounds__(256, (sizeof(T) == 2 || DP == 32 ? 2 : 1)) void k_attention_dkv(AttentionParams p) {
+  typedef DkvShape<T, DP> S;
   typedef typename AtFrag<T>::type frag_t;
   constexpr int TQ = S::TR, NB = TQ / 32;
   extern __shared__ __align__(16) unsigned char lds[];
@@ -217,11 +227,30 @@ __global__ __launch_bounds__(256) void k_attention_dkv(AttentionParams p) {
   const int first = !p.causal || key < prefix ? -0x40000000 : key - off;  // the first query that sees this key
   const int mydoc = p.dock ? p.dock[(long)b * p.Nk + key] : 0;
 
-  frag_t kf[DP / 16], vf[DP / 16];
+  frag_t kf[DP / 16], vf[S::VL ? 1 : DP / 16];
   load_own<T, DP>(reinterpret_cast<const T*>(p.k) + b * p.k_b + (long)key * p.k_n + kvh * p.k_h, p.D, h, kf);
-  load_own<T, DP>(reinterpret_cast<const T*>(p.v) + b * p.v_b + (long)key * p.v_n + kvh * p.v_h, p.D, h, vf);
+  const int nchunk = p.D * (int)sizeof(T) / 16;
+  const unsigned char* VT = lds + S::V;
+  if constexpr (S::VL) {
+    typedef TileCopy<T, DP, 128, 4> Copy;
+    Copy vc;
+    const unsigned vst = (unsigned)(p.v_n * (long)sizeof(T));
+    vc.init(wave, lane, vst, nchunk);
+    vc.issue(reinterpret_cast<const unsigned char*>(p.v) + (b * p.v_b + kvh * p.v_h + (long)j0 * p.v_n) * (long)sizeof(T), vst, nchunk, p.Nk - j0,
+             lds0 + (unsigned)S::V, wave, lane);
+    if (nchunk < Copy::CPR) {                           // both operands of go v come out of LDS: behind D one of them has to be zero
+      wait_copies();
+      __syncthreads();
+      for (int c = tid; c < 128 * Copy::CPR; c += 256) {
+        const int row = c / Copy::CPR;
+        if (((c % Copy::CPR) ^ tile_swz<Copy::CPR>(row)) >= nchunk) *reinterpret_cast<f32x4*>(lds + S::V + c * 16) = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
+    }
+  } else {
+    load_own<T, DP>(reinterpret_cast<const T*>(p.v) + b * p.v_b + (long)key * p.v_n + kvh * p.v_h, p.D, h, vf);
+    arrived(vf);
+  }
   arrived(kf);
-  arrived(vf);
 
   int t0 = !p.causal || prefix > j0 ? 0 : min(max(j0 - off, 0), p.Nq) / TQ, t1 = (p.Nq + TQ - 1) / TQ;
   int4 kr = make_int4(0, 0, 0, 0), krw = kr;
@@ -235,7 +264,6 @@ __global__ __launch_bounds__(256) void k_attention_dkv(AttentionParams p) {
     krw = rk[min((j0 >> 5) + wave, kgroups - 1)];
     tiles_of_documents<256>(rq, qgroups, NB, kr, t0, t1, tid, reinterpret_cast<int*>(lds + 2 * S::STAGE));
   }
-  const int nchunk = p.D * (int)sizeof(T) / 16;
   const unsigned qst = (unsigned)(p.q_n * (long)sizeof(T)), gst = (unsigned)(p.go_n * (long)sizeof(T));
   TileCopy<T, DP, TQ, 4> qc, gc;
   qc.init(wave, lane, qst, nchunk);
@@ -301,7 +329,7 @@ __global__ __launch_bounds__(256) void k_attention_dkv(AttentionParams p) {
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks) at_mma(tile_row<T, DP>(Q, 32 * ib + (lane & 31), ks, h), kf[ks], x);
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) at_mma(tile_row<T, DP>(GO, 32 * ib + (lane & 31), ks, h), vf[ks], y);
+        for (int ks = 0; ks < DP / 16; ++ks) at_mma(tile_row<T, DP>(GO, 32 * ib + (lane & 31), ks, h), S::VL ? tile_row<T, DP>(VT, wave * 32 + (lane & 31), ks, h) : vf[S::VL ? 0 : ks], y);
         const float away = BIAS ? (float)(key - off - i0 - 32 * ib - 4 * h) : 0.f;
         const int need = max(first, -0x20000000) - i0 - 32 * ib - 4 * h, room = p.Nq - i0 - 32 * ib - 4 * h;
 #pragma unroll
@@ -400,15 +428,15 @@ int attention_bwd_launch(const AttentionParams& p, hipStream_t s) {
   if (bq > 0x7fffffffL || bk > 0x7fffffffL || (rows + 15) / 16 > 0x7fffffffL) return CRAFT_ERR_UNSUPPORTED;
   hipLaunchKernelGGL(k_attention_delta<T>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, p, const_cast<float*>(p.delta));
   HIP_CHECK_RET(hipGetLastError());
-  auto go = [&](auto tag, long blocks) {
+  auto go = [&](auto tag, long blocks, int bytes) {
     constexpr auto kernel = decltype(tag)::value;
-    if (const int rc = allow_lds<kernel>(S::LDS)) return rc;
-    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), S::LDS, s, p);
+    if (const int rc = allow_lds<kernel>(bytes)) return rc;
+    hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), bytes, s, p);
     return (int)hipGetLastError();
   };
   int rc;
-  if (p.cap > 0.f) rc = p.slopes ? go(KernelTag<k_attention_dkv<T, DP, true, true>>(), bk) : go(KernelTag<k_attention_dkv<T, DP, true, false>>(), bk);
-  else rc = p.slopes ? go(KernelTag<k_attention_dkv<T, DP, false, true>>(), bk) : go(KernelTag<k_attention_dkv<T, DP, false, false>>(), bk);
+  if (p.cap > 0.f) rc = p.slopes ? go(KernelTag<k_attention_dkv<T, DP, true, true>>(), bk, DkvShape<T, DP>::LDS) : go(KernelTag<k_attention_dkv<T, DP, true, false>>(), bk, DkvShape<T, DP>::LDS);
+  else rc = p.slopes ? go(KernelTag<k_attention_dkv<T, DP, false, true>>(), bk, DkvShape<T, DP>::LDS) : go(KernelTag<k_attention_dkv<T, DP, false, false>>(), bk, DkvShape<T, DP>::LDS);
   if (rc) return rc;
   if (p.part_k) {
     const long n4 = (long)p.B * p.Nk * p.Hk * (p.D / 4);
@@ -417,8 +445,8 @@ int attention_bwd_launch(const AttentionParams& p, hipStream_t s) {
                        reinterpret_cast<T*>(p.dv), n4, p.H / p.Hk, p.D / 4);
     HIP_CHECK_RET(hipGetLastError());
   }
-  if (p.cap > 0.f) return p.slopes ? go(KernelTag<k_attention_dq<T, DP, true, true>>(), bq) : go(KernelTag<k_attention_dq<T, DP, true, false>>(), bq);
-  return p.slopes ? go(KernelTag<k_attention_dq<T, DP, false, true>>(), bq) : go(KernelTag<k_attention_dq<T, DP, false, false>>(), bq);
+  if (p.cap > 0.f) return p.slopes ? go(KernelTag<k_attention_dq<T, DP, true, true>>(), bq, S::LDS) : go(KernelTag<k_attention_dq<T, DP, true, false>>(), bq, S::LDS);
+  return p.slopes ? go(KernelTag<k_attention_dq<T, DP, false, true>>(), bq, S::LDS) : go(KernelTag<k_attention_dq<T, DP, false, false>>(), bq, S::LDS);
 }
 
 }  // namespace craft
