@@ -7,7 +7,7 @@
 
 namespace craft {
 
-// delta, 16 lanes to a row
+// -delta (the sums of dp start there), 16 lanes to a row
 template <typename T>
 __global__ __launch_bounds__(256) void k_attention_delta(AttentionParams p, float* delta) {
   const long row = (long)blockIdx.x * 16 + (threadIdx.x >> 4), rows = (long)p.B * p.Nq * p.H;
@@ -25,7 +25,7 @@ __global__ __launch_bounds__(256) void k_attention_delta(AttentionParams p, floa
   }
 #pragma unroll
   for (int k = 8; k > 0; k >>= 1) s += __shfl_xor(s, k);
-  if ((threadIdx.x & 15) == 0) delta[(b * p.H + head) * p.Nq + i] = s;
+  if ((threadIdx.x & 15) == 0) delta[(b * p.H + head) * p.Nq + i] = -s;
 }
 
 template <typename T, int DP> struct BwdShape {
@@ -77,7 +77,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP < 128 ? 2 : 1)) void k_a
   arrived(qf);
   arrived(gf);
   arrived(row);
-  const float lse = row[0], delta = row[1];
+  const float lse = row[0], delta = row[1], mul = at_mul<T, CAP>(p);
 
   int t0 = 0, t1 = p.causal ? (max(min(max(i_last + off + 1, prefix), p.Nk), 0) + TK - 1) / TK : (p.Nk + TK - 1) / TK;
   int4 qr = make_int4(0, 0, 0, 0), qrw = qr;
@@ -145,20 +145,28 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP < 128 ? 2 : 1)) void k_a
       for (int kbk = 0; kbk < NB; ++kbk) {
         f32x16 x, y;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] = y[r] = 0.f;
+        for (int r = 0; r < 16; ++r) { x[r] = 0.f; y[r] = delta; }                // dp - delta: the sum starts at -delta, which is what is stored
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) at_mma(tile_row<T, DP>(K, 32 * kbk + (lane & 31), ks, h), qf[ks], x);
-#pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) at_mma(tile_row<T, DP>(V, 32 * kbk + (lane & 31), ks, h), gf[ks], y);
+        for (int ks = 0; ks < DP / 16; ++ks) {
+          at_mma(tile_row<T, DP>(K, 32 * kbk + (lane & 31), ks, h), qf[ks], x);
+          at_mma(tile_row<T, DP>(V, 32 * kbk + (lane & 31), ks, h), gf[ks], y);
+        }
         const float away = BIAS ? (float)(pos - k0 - 32 * kbk - 4 * h) : 0.f;
+        {                                                                 // in steps over all 16 scores: a score's own steps wait for one another
+          if constexpr (CAP) {
+            at_raws<T>(p, x);
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-          float th = 0.f;
-          float z = at_score<T, CAP>(p, x[r], th);
-          if constexpr (BIAS) z -= slope2 * fabsf(away - (float)acc_row(r));
-          float ds = __builtin_amdgcn_exp2f(z - lse) * (y[r] - delta);
-          if constexpr (CAP) ds *= 1.f - th * th;
-          x[r] = ds;
+            for (int q = 0; q < 16; ++q) y[q] *= at_slope<T>(x[q]);
+          }
+#pragma unroll
+          for (int q = 0; q < 16; ++q)
+            x[q] = BIAS ? fmaf(-slope2, fabsf(away - (float)acc_row(q)), fmaf(x[q], mul, -lse)) : fmaf(x[q], mul, -lse);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int q = 0; q < 16; ++q) x[q] = __builtin_amdgcn_exp2f(x[q]);
+          __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+          for (int q = 0; q < 16; ++q) x[q] *= y[q];
         }
         if (masked) {                                                     // a choice, not a product: what the mask hides may be inf or NaN
           const int room = lim - k0 - 32 * kbk - 4 * h;
@@ -319,42 +327,60 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP == 32 ? 2 : 1)) void k_a
       skip |= !ranges_meet(qr, krw);
     }
     if (!skip) {
-      const float slope2 = BIAS ? p.slopes[head] * 1.44269504088896f : 0.f;
+      const float mul = at_mul<T, CAP>(p), slope2 = BIAS ? p.slopes[head] * 1.44269504088896f : 0.f;
       const bool masked = docmask || i0 + TQ > p.Nq || (p.causal && i0 + off < jw + 31 && prefix < jw + 32);
 #pragma unroll
       for (int ib = 0; ib < NB; ++ib) {
         f32x16 x, y;
 #pragma unroll
-        for (int r = 0; r < 16; ++r) x[r] = y[r] = 0.f;
+        for (int r = 0; r < 16; ++r) x[r] = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) at_mma(tile_row<T, DP>(Q, 32 * ib + (lane & 31), ks, h), kf[ks], x);
+        for (int g = 0; g < 4; ++g) {                                     // dp - delta: the sum starts at -delta
+          const f32x4 de = *reinterpret_cast<const f32x4*>(delta + 32 * ib + 8 * g + 4 * h);
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) at_mma(tile_row<T, DP>(GO, 32 * ib + (lane & 31), ks, h), S::VL ? tile_row<T, DP>(VT, wave * 32 + (lane & 31), ks, h) : vf[S::VL ? 0 : ks], y);
+          for (int e = 0; e < 4; ++e) y[4 * g + e] = de[e];
+        }
+#pragma unroll
+        for (int ks = 0; ks < DP / 16; ++ks) {
+          at_mma(tile_row<T, DP>(Q, 32 * ib + (lane & 31), ks, h), kf[ks], x);
+          at_mma(tile_row<T, DP>(GO, 32 * ib + (lane & 31), ks, h), S::VL ? tile_row<T, DP>(VT, wave * 32 + (lane & 31), ks, h) : vf[S::VL ? 0 : ks], y);
+        }
         const float away = BIAS ? (float)(key - off - i0 - 32 * ib - 4 * h) : 0.f;
-        const int need = max(first, -0x20000000) - i0 - 32 * ib - 4 * h, room = p.Nq - i0 - 32 * ib - 4 * h;
+        // in steps over all 16 scores: a score's own steps wait for one another
+        if constexpr (CAP) {
+          at_raws<T>(p, x);
+#pragma unroll
+          for (int r = 0; r < 16; ++r) y[r] *= at_slope<T>(x[r]);
+        }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
           const f32x4 le = *reinterpret_cast<const f32x4*>(lse + 32 * ib + 8 * g + 4 * h);
-          const f32x4 de = *reinterpret_cast<const f32x4*>(delta + 32 * ib + 8 * g + 4 * h);
-          int4 di = make_int4(mydoc, mydoc, mydoc, mydoc);
-          if (docmask) di = *reinterpret_cast<const int4*>(ids + 32 * ib + 8 * g + 4 * h);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int r = 4 * g + e;
-            float th = 0.f;
-            float z = at_score<T, CAP>(p, x[r], th);
-            if constexpr (BIAS) z -= slope2 * fabsf(away - (float)acc_row(r));
-            float pr = __builtin_amdgcn_exp2f(z - le[e]);
-            float ds = pr * (y[r] - de[e]);
-            if constexpr (CAP) ds *= 1.f - th * th;
-            if (masked) {
-              const int dr = e == 0 ? di.x : e == 1 ? di.y : e == 2 ? di.z : di.w;
+            x[r] = BIAS ? fmaf(-slope2, fabsf(away - (float)acc_row(r)), fmaf(x[r], mul, -le[e])) : fmaf(x[r], mul, -le[e]);
+          }
+        }
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(x[r]);
+        __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) y[r] *= x[r];
+        if (masked) {                                                     // a choice, not a product: what the mask hides may be inf or NaN
+          asm volatile("" ::: "memory");                                  // (a branch of its own, not a branch or a selection per score)
+          const int need = max(first, -0x20000000) - i0 - 32 * ib - 4 * h, room = p.Nq - i0 - 32 * ib - 4 * h;
+#pragma unroll
+          for (int g = 0; g < 4; ++g) {
+            int4 di = make_int4(0, 0, 0, 0);
+            if (docmask) di = *reinterpret_cast<const int4*>(ids + 32 * ib + 8 * g + 4 * h);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int r = 4 * g + e, dr = e == 0 ? di.x : e == 1 ? di.y : e == 2 ? di.z : di.w;
               const bool see = acc_row(r) >= need && acc_row(r) < room && (!docmask || (dr == mydoc && dr >= 0));
-              pr = see ? pr : 0.f;
-              ds = see ? ds : 0.f;
+              x[r] = see ? x[r] : 0.f;
+              y[r] = see ? y[r] : 0.f;
             }
-            x[r] = pr;
-            y[r] = ds;
           }
         }
 #pragma unroll

@@ -39,9 +39,9 @@ __global__ __launch_bounds__(256, 2) void k_attention_fwd(AttentionParams p) {
 
   frag_t qf[DP / 16];
   load_own<T, DP>(reinterpret_cast<const T*>(p.q) + b * p.q_b + (long)i * p.q_n + head * p.q_h, p.D, h, qf);
-  constexpr bool RAW = !CAP && !BIAS;           // scores stay products: the maximum is taken of them, the scale goes into the exponential's one fma
-  const float c2 = RAW ? fmaxf(fabsf(p.c2), 1e-30f) : 1.f;
-  if (RAW && p.c2 < 0.f) {
+  constexpr bool RAW = !BIAS;                   // the maximum is taken of at_raw, at_mul goes into the exponential's one fma
+  const float mul = at_mul<T, CAP>(p), c2 = RAW ? fmaxf(fabsf(mul), 1e-30f) : 1.f;
+  if (RAW && !CAP && mul < 0.f) {
 #pragma unroll
     for (int ks = 0; ks < DP / 16; ++ks) qf[ks] = -qf[ks];
   }
@@ -119,15 +119,14 @@ __global__ __launch_bounds__(256, 2) void k_attention_fwd(AttentionParams p) {
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks) at_mma(tile_row<T, DP>(K, 32 * kbk + (lane & 31), ks, h), qf[ks], x[kbk]);
       }
-      if constexpr (!RAW) {
+      if constexpr (CAP || BIAS) {
         const float away = BIAS ? (float)(pos - k0 - 4 * h) : 0.f;
 #pragma unroll
         for (int kbk = 0; kbk < NB; ++kbk)
 #pragma unroll
           for (int r = 0; r < 16; ++r) {
-            float th;
-            float z = at_score<T, CAP>(p, x[kbk][r], th);
-            if constexpr (BIAS) z -= slope2 * fabsf(away - (float)(32 * kbk + acc_row(r)));
+            float z = at_raw<T, CAP>(p, x[kbk][r]);
+            if constexpr (BIAS) z = fmaf(-slope2, fabsf(away - (float)(32 * kbk + acc_row(r))), z * mul);
             x[kbk][r] = z;
           }
       }

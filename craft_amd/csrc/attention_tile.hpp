@@ -37,7 +37,7 @@ struct AttentionParams {
   const int4 *rq, *rk;                         // per 32 tokens: {least document, greatest document, any negative one, 0}
   int causal;
   float* lse;                                  // [B][H][Nq] log2 of the sum of 2^z; +inf for a query that sees nothing (so that 2^(z - lse) = 0)
-  const float* delta;                          // [B][H][Nq] sum_d go * o
+  const float* delta;                          // [B][H][Nq] -sum_d go * o
   float *part_o, *part_ml;                     // token kernel: partial results of the splits
   int splits;
   float *part_k, *part_v;                      // backward: per query head partial key / value gradients (null: written directly)
@@ -237,13 +237,42 @@ __device__ __forceinline__ int4 uniform_range(const int4& a) {
 __device__ __forceinline__ bool ranges_meet(const int4& a, const int4& b) { return a.x <= b.y && b.x <= a.y; }
 __device__ __forceinline__ bool one_document(const int4& a, const int4& b) { return !a.z && !b.z && a.x == a.y && b.x == b.y && a.x == b.x; }
 
-// the score of a product, as a power of two; th: tanh, for the gradient.  fp32 tensors take the library's tanh (the quick form is off by 1e-7 of the cap).
+// A score is at_mul * at_raw(q . k) (+ the bias), as a power of two and up to a constant of the whole row, which the softmax drops (the kept log-sums drop
+// it too): the product itself; capped, with tanh(u) = 1 - 2 r, r = 1 / (1 + e^2u): -r.  fp32 tensors take the library's tanh (r is off by 2^-23 of 1).
 template <typename T, bool CAP>
-__device__ __forceinline__ float at_score(const AttentionParams& p, float s, float& th) {
-  if constexpr (!CAP) return s * p.c2;
-  if constexpr (std::is_same<T, float>::value) th = tanhf(s * p.scale / p.cap);
-  else th = 1.f - 2.f * __builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * p.ca) + 1.f);      // (exp2 = inf: 1;  exp2 = 0: -1)
-  return th * p.cap2;
+__device__ __forceinline__ float at_raw(const AttentionParams& p, float s) {
+  if constexpr (!CAP) return s;
+  else if constexpr (std::is_same<T, float>::value) return tanhf(s * p.scale / p.cap);
+  else return -__builtin_amdgcn_rcpf(__builtin_amdgcn_exp2f(s * p.ca) + 1.f);                // (exp2 = inf: 0;  exp2 = 0: -1)
+}
+// at_raw with a cap of 16 scores, step by step
+template <typename T>
+__device__ __forceinline__ void at_raws(const AttentionParams& p, f32x16& x) {
+  if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = at_raw<T, true>(p, x[r]);
+  } else {
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] *= p.ca;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = __builtin_amdgcn_exp2f(x[r]);
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] += 1.f;
+    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) x[r] = -__builtin_amdgcn_rcpf(x[r]);
+    __builtin_amdgcn_sched_barrier(0);
+  }
+}
+template <typename T, bool CAP>
+__device__ __forceinline__ float at_mul(const AttentionParams& p) { return !CAP ? p.c2 : std::is_same<T, float>::value ? p.cap2 : 2.f * p.cap2; }
+// 1 - tanh^2 from at_raw
+template <typename T>
+__device__ __forceinline__ float at_slope(float x) {
+  const float th = std::is_same<T, float>::value ? x : fmaf(2.f, x, 1.f);
+  return fmaf(-th, th, 1.f);
 }
 
 // Which (head of the batch, tile) a block takes.  The blocks of a head share an XCD, whose L2 then holds that head's keys; and the tiles of all the heads

@@ -43,7 +43,7 @@ __global__ __launch_bounds__((TokenShape<T, DP>::WAVES * 64)) void k_attention_t
   float sl[1] = {BIAS ? p.slopes[head] * 1.44269504088896f : 0.f};
   arrived(qf);
   arrived(sl);
-  const float slope2 = sl[0];
+  const float slope2 = sl[0], mul = at_mul<T, CAP>(p);
 
   // tiles of this split: [a0, a1); of this wave: a0 + wave, + W, ...
   const int tiles = (p.Nk + 31) >> 5, per = (tiles + p.splits - 1) / p.splits;
@@ -93,9 +93,8 @@ __global__ __launch_bounds__((TokenShape<T, DP>::WAVES * 64)) void k_attention_t
       const float away = BIAS ? (float)(pos - k0 - 4 * h) : 0.f;
 #pragma unroll
       for (int q = 0; q < 16; ++q) {
-        float th;
-        float z = at_score<T, CAP>(p, x[q], th);
-        if constexpr (BIAS) z -= slope2 * fabsf(away - (float)acc_row(q));
+        float z = at_raw<T, CAP>(p, x[q]) * mul;
+        if constexpr (BIAS) z = fmaf(-slope2, fabsf(away - (float)acc_row(q)), z);
         x[q] = z;
       }
       if (k0 + 32 > lim_lo) {
