@@ -31,7 +31,7 @@ __global__ __launch_bounds__(256) void k_attention_delta(AttentionParams p, floa
 template <typename T, int DP> struct BwdShape {
   static constexpr int TR = sizeof(T) == 2 && DP < 128 ? 64 : 32;         // rows of a tile (128 columns in 64-row tiles: registers spill)
   static constexpr int TILE = TR * DP * (int)sizeof(T);
-  static constexpr int STAGE = 2 * TILE + 3 * 256;                        // two operands; lse, delta, documents of 64 rows
+  static constexpr int STAGE = 2 * TILE + 1024;                        // two operands; lse, delta, documents of 64 rows
   static constexpr int LDS = 2 * STAGE + 64;
 };
 
@@ -41,8 +41,8 @@ template <typename T, int DP> struct DkvShape {
   static constexpr bool VL = sizeof(T) == 2 && DP == 128;
   static constexpr int TR = VL ? 32 : BwdShape<T, DP>::TR;
   static constexpr int TILE = TR * DP * (int)sizeof(T);
-  static constexpr int STAGE = 2 * TILE + 3 * 256;
-  static constexpr int V = 2 * STAGE + 64, LDS = V + (VL ? 128 * DP * (int)sizeof(T) : 0);
+  static constexpr int STAGE = 2 * TILE + 1024;
+  static constexpr int V = 2 * STAGE + 512, LDS = V + (VL ? 128 * DP * (int)sizeof(T) : 0);
 };
 
 // dq: lane = query
@@ -51,7 +51,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP < 128 ? 2 : 1)) void k_a
   typedef BwdShape<T, DP> S;
   typedef typename AtFrag<T>::type frag_t;
   constexpr int TK = S::TR, NB = TK / 32;
-  extern __shared__ __align__(16) unsigned char lds[];
+  extern __shared__ __align__(512) unsigned char lds[];
   const unsigned lds0 = (unsigned)(size_t)(CRAFT_LDS unsigned char*)lds;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int nqt = (p.Nq + 127) >> 7;
@@ -132,6 +132,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP < 128 ? 2 : 1)) void k_a
     unsigned char* K = lds + buf * S::STAGE;
     unsigned char* V = K + S::TILE;
     const int* ids = reinterpret_cast<const int*>(V + S::TILE);
+    const unsigned at = lds0 + (unsigned)(buf * S::STAGE), Kr = row_addr<T, DP>(at, lane), Vr = row_addr<T, DP>(at + S::TILE, lane), Kc = col_addr<T, DP>(at, lane);
     const int k0 = t * TK;
     bool docmask = false, skip = k0 >= lim_hi;
     if (rk) {
@@ -148,8 +149,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP < 128 ? 2 : 1)) void k_a
         for (int r = 0; r < 16; ++r) { x[r] = 0.f; y[r] = delta; }                // dp - delta: the sum starts at -delta, which is what is stored
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks) {
-          at_mma(tile_row<T, DP>(K, 32 * kbk + (lane & 31), ks, h), qf[ks], x);
-          at_mma(tile_row<T, DP>(V, 32 * kbk + (lane & 31), ks, h), gf[ks], y);
+          at_mma(row_read<T, DP>(Kr, kbk, ks), qf[ks], x);
+          at_mma(row_read<T, DP>(Vr, kbk, ks), gf[ks], y);
         }
         const float away = BIAS ? (float)(pos - k0 - 32 * kbk - 4 * h) : 0.f;
         {                                                                 // in steps over all 16 scores: a score's own steps wait for one another
@@ -187,7 +188,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP < 128 ? 2 : 1)) void k_a
         for (int s2 = 0; s2 < 2; ++s2) {
           const frag_t sf = at_pack<T>(x, s2);
 #pragma unroll
-          for (int d = 0; d < DP / 32; ++d) at_mma(tile_col<T, DP>(K, 32 * kbk + 16 * s2, d, lane), sf, dq[d]);
+          for (int d = 0; d < DP / 32; ++d) at_mma(col_read<T, DP>(Kc, 32 * kbk + 16 * s2, d), sf, dq[d]);
         }
       }
     }
@@ -219,7 +220,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP == 32 ? 2 : 1)) void k_a
   typedef DkvShape<T, DP> S;
   typedef typename AtFrag<T>::type frag_t;
   constexpr int TQ = S::TR, NB = TQ / 32;
-  extern __shared__ __align__(16) unsigned char lds[];
+  extern __shared__ __align__(512) unsigned char lds[];
   const unsigned lds0 = (unsigned)(size_t)(CRAFT_LDS unsigned char*)lds;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int nkt = (p.Nk + 127) >> 7, G = p.H / p.Hk;
@@ -238,7 +239,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP == 32 ? 2 : 1)) void k_a
   frag_t kf[DP / 16], vf[S::VL ? 1 : DP / 16];
   load_own<T, DP>(reinterpret_cast<const T*>(p.k) + b * p.k_b + (long)key * p.k_n + kvh * p.k_h, p.D, h, kf);
   const int nchunk = p.D * (int)sizeof(T) / 16;
-  const unsigned char* VT = lds + S::V;
+  const unsigned VTr = row_addr<T, DP>(lds0 + (unsigned)(S::V + wave * 32 * at_rowb<T, DP>()), lane);
   if constexpr (S::VL) {
     typedef TileCopy<T, DP, 128, 4> Copy;
     Copy vc;
@@ -295,6 +296,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP == 32 ? 2 : 1)) void k_a
     if (wave == 0) copy_words(p.lse + row, (long)t * TQ, p.Nq - 1, at + 2 * S::TILE, lane);
     if (wave == 1) copy_words(p.delta + row, (long)t * TQ, p.Nq - 1, at + 2 * S::TILE + 256, lane);
     if (rq && wave == 2) copy_words(p.docq + (long)b * p.Nq, (long)t * TQ, p.Nq - 1, at + 2 * S::TILE + 512, lane);
+    if (BIAS && wave == 3) copy_words(p.slopes, head, head, at + 2 * S::TILE + 768, lane);
   };
 
   f32x16 dk[DP / 32], dv[DP / 32];
@@ -319,6 +321,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP == 32 ? 2 : 1)) void k_a
     const float* lse = reinterpret_cast<const float*>(GO + S::TILE);
     const float* delta = lse + 64;
     const int* ids = reinterpret_cast<const int*>(delta + 64);
+    const unsigned at = lds0 + (unsigned)(buf * S::STAGE), Qr = row_addr<T, DP>(at, lane), GOr = row_addr<T, DP>(at + S::TILE, lane),
+                   Qc = col_addr<T, DP>(at, lane), GOc = col_addr<T, DP>(at + S::TILE, lane);
     const int i0 = t * TQ;
     bool docmask = false, skip = p.causal && prefix <= jw && i0 + TQ - 1 + off < jw;
     if (rq) {
@@ -327,7 +331,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP == 32 ? 2 : 1)) void k_a
       skip |= !ranges_meet(qr, krw);
     }
     if (!skip) {
-      const float mul = at_mul<T, CAP>(p), slope2 = BIAS ? p.slopes[head] * 1.44269504088896f : 0.f;
+      const float mul = at_mul<T, CAP>(p), slope2 = BIAS ? delta[128] * 1.44269504088896f : 0.f;      // (behind the documents)
       const bool masked = docmask || i0 + TQ > p.Nq || (p.causal && i0 + off < jw + 31 && prefix < jw + 32);
 #pragma unroll
       for (int ib = 0; ib < NB; ++ib) {
@@ -342,8 +346,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP == 32 ? 2 : 1)) void k_a
         }
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks) {
-          at_mma(tile_row<T, DP>(Q, 32 * ib + (lane & 31), ks, h), kf[ks], x);
-          at_mma(tile_row<T, DP>(GO, 32 * ib + (lane & 31), ks, h), S::VL ? tile_row<T, DP>(VT, wave * 32 + (lane & 31), ks, h) : vf[S::VL ? 0 : ks], y);
+          at_mma(row_read<T, DP>(Qr, ib, ks), kf[ks], x);
+          at_mma(row_read<T, DP>(GOr, ib, ks), S::VL ? row_read<T, DP>(VTr, 0, ks) : vf[S::VL ? 0 : ks], y);
         }
         const float away = BIAS ? (float)(key - off - i0 - 32 * ib - 4 * h) : 0.f;
         // in steps over all 16 scores: a score's own steps wait for one another
@@ -388,8 +392,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP == 32 ? 2 : 1)) void k_a
           const frag_t pf = at_pack<T>(x, s2), sf = at_pack<T>(y, s2);
 #pragma unroll
           for (int d = 0; d < DP / 32; ++d) {
-            at_mma(tile_col<T, DP>(GO, 32 * ib + 16 * s2, d, lane), pf, dv[d]);
-            at_mma(tile_col<T, DP>(Q, 32 * ib + 16 * s2, d, lane), sf, dk[d]);
+            at_mma(col_read<T, DP>(GOc, 32 * ib + 16 * s2, d), pf, dv[d]);
+            at_mma(col_read<T, DP>(Qc, 32 * ib + 16 * s2, d), sf, dk[d]);
           }
         }
       }

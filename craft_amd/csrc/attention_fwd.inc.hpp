@@ -8,7 +8,7 @@ namespace craft {
 template <typename T, int DP> struct FwdShape {
   static constexpr int TK = sizeof(T) == 2 ? 64 : 32;                     // keys of a tile
   static constexpr int TILE = TK * DP * (int)sizeof(T);
-  static constexpr int STAGE = 2 * TILE + 256;                            // K, V, document ids
+  static constexpr int STAGE = 2 * TILE + 512;                            // K, V, document ids
   static constexpr int LDS = 2 * STAGE + 64;
 };
 
@@ -17,7 +17,7 @@ __global__ __launch_bounds__(256, 2) void k_attention_fwd(AttentionParams p) {
   typedef FwdShape<T, DP> S;
   typedef typename AtFrag<T>::type frag_t;
   constexpr int TK = S::TK, NB = TK / 32;
-  extern __shared__ __align__(16) unsigned char lds[];
+  extern __shared__ __align__(512) unsigned char lds[];
   const unsigned lds0 = (unsigned)(size_t)(CRAFT_LDS unsigned char*)lds;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int nqt = (p.Nq + 127) >> 7;
@@ -100,9 +100,9 @@ __global__ __launch_bounds__(256, 2) void k_attention_fwd(AttentionParams p) {
     __syncthreads();                            // the tile is whole; everybody has left the other buffer
     const int tn = next(t + 1, krn);
     if (tn < t1) stage(buf ^ 1, tn);
-    unsigned char* K = lds + buf * S::STAGE;
-    unsigned char* V = K + S::TILE;
+    unsigned char* V = lds + buf * S::STAGE + S::TILE;
     const int* ids = reinterpret_cast<const int*>(V + S::TILE);
+    const unsigned at = lds0 + (unsigned)(buf * S::STAGE), Kr = row_addr<T, DP>(at, lane), Vc = col_addr<T, DP>(at + S::TILE, lane);
     const int k0 = t * TK;
     bool docmask = false, skip = k0 >= lim_hi;
     if (rk) {
@@ -117,7 +117,7 @@ __global__ __launch_bounds__(256, 2) void k_attention_fwd(AttentionParams p) {
 #pragma unroll
         for (int r = 0; r < 16; ++r) x[kbk][r] = 0.f;
 #pragma unroll
-        for (int ks = 0; ks < DP / 16; ++ks) at_mma(tile_row<T, DP>(K, 32 * kbk + (lane & 31), ks, h), qf[ks], x[kbk]);
+        for (int ks = 0; ks < DP / 16; ++ks) at_mma(row_read<T, DP>(Kr, kbk, ks), qf[ks], x[kbk]);
       }
       if constexpr (CAP || BIAS) {
         const float away = BIAS ? (float)(pos - k0 - 4 * h) : 0.f;
@@ -176,7 +176,7 @@ __global__ __launch_bounds__(256, 2) void k_attention_fwd(AttentionParams p) {
         for (int s2 = 0; s2 < 2; ++s2) {
           const frag_t pf = at_pack<T>(x[kbk], s2);
 #pragma unroll
-          for (int d = 0; d < DP / 32; ++d) at_mma(tile_col<T, DP>(V, 32 * kbk + 16 * s2, d, lane), pf, o[d]);
+          for (int d = 0; d < DP / 32; ++d) at_mma(col_read<T, DP>(Vc, 32 * kbk + 16 * s2, d), pf, o[d]);
         }
     }
     t = tn;

@@ -65,54 +65,69 @@ __device__ __forceinline__ int tile_swz(int r) {
 }
 template <typename T, int DP> constexpr int at_cpr() { return DP * (int)sizeof(T) / 16; }
 
-// row read: 8 consecutive columns 16 ks + 8 h .. of row `row`
+// LDS addresses.  The swizzle is an exclusive or of a chunk's number, so a lane's addresses within a tile (whose base is a multiple of its row, 512 bytes at
+// most) differ from one of them by an exclusive or with a constant and an offset that the instruction adds: one register for the row reads of a tile and
+// one for its transposing reads, in place of one for each column step (the gradients' kernels spilled for them).
+template <typename T, int DP> constexpr int at_rowb() { return DP * (int)sizeof(T); }
+// of lane's row lane & 31, columns 8 h ..
 template <typename T, int DP>
-__device__ __forceinline__ typename AtFrag<T>::type tile_row(const unsigned char* t, int row, int ks, int h) {
-  constexpr int CPR = at_cpr<T, DP>();
-  const int f = tile_swz<CPR>(row);
-  const unsigned char* r = t + row * (DP * (int)sizeof(T));
+__device__ __forceinline__ unsigned row_addr(unsigned tile, int lane) {
+  const int row = lane & 31, h = lane >> 5, f = tile_swz<at_cpr<T, DP>()>(row);
+  return tile + (unsigned)(row * at_rowb<T, DP>() + (((sizeof(T) == 2 ? h : 2 * h) ^ f) << 4));
+}
+// row read: columns 16 ks + 8 h .. + 7 of row 32 blk + (lane & 31)
+template <typename T, int DP>
+__device__ __forceinline__ typename AtFrag<T>::type row_read(unsigned addr, int blk, int ks) {
   if constexpr (sizeof(T) == 2) {
-    return *reinterpret_cast<const typename AtFrag<T>::type*>(r + (((2 * ks + h) ^ f) << 4));
+    return *reinterpret_cast<CRAFT_LDS typename AtFrag<T>::type*>((addr ^ (unsigned)(ks << 5)) + (unsigned)(blk * 32 * at_rowb<T, DP>()));
   } else {
-    const f32x4 a = *reinterpret_cast<const f32x4*>(r + (((4 * ks + 2 * h) ^ f) << 4));
-    const f32x4 b = *reinterpret_cast<const f32x4*>(r + (((4 * ks + 2 * h + 1) ^ f) << 4));
+    const f32x4 a = *reinterpret_cast<CRAFT_LDS f32x4*>((addr ^ (unsigned)(ks << 6)) + (unsigned)(blk * 32 * at_rowb<T, DP>()));
+    const f32x4 b = *reinterpret_cast<CRAFT_LDS f32x4*>((addr ^ (unsigned)(ks << 6) ^ 16u) + (unsigned)(blk * 32 * at_rowb<T, DP>()));
     f32x8 v;
 #pragma unroll
     for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
     return v;
   }
 }
-
+// of lane's part of the transposing reads
+template <typename T, int DP>
+__device__ __forceinline__ unsigned col_addr(unsigned tile, int lane) {
+  const int h = lane >> 5;
+  if constexpr (sizeof(T) == 2) {
+    const int j = lane & 15, mh = (lane >> 4) & 1, row = 4 * h + (j >> 2), c = 2 * mh + ((j & 3) >> 1);
+    return tile + (unsigned)(row * at_rowb<T, DP>() + ((c ^ tile_swz<at_cpr<T, DP>()>(row)) << 4) + ((j & 1) << 3));
+  } else {
+    const int col = lane & 31, row = 4 * h;
+    return tile + (unsigned)(row * at_rowb<T, DP>() + (((col >> 2) ^ tile_swz<at_cpr<T, DP>()>(row)) << 4) + ((col & 3) << 2));
+  }
+}
 // transposing read: column 32 db + (lane & 31) of rows row0 + 4 h + {0..3} and row0 + 8 + 4 h + {0..3} (accumulator order), row0 a multiple of 16
 template <typename T, int DP>
-__device__ __forceinline__ typename AtFrag<T>::type tile_col(const unsigned char* t, int row0, int db, int lane) {
-  constexpr int CPR = at_cpr<T, DP>();
-  const int h = lane >> 5;
+__device__ __forceinline__ typename AtFrag<T>::type col_read(unsigned addr, int row0, int db) {
+  constexpr int ROWB = at_rowb<T, DP>();
   typename AtFrag<T>::type v;
   if constexpr (sizeof(T) == 2) {
-    const int j = lane & 15, mh = (lane >> 4) & 1, c = 4 * db + 2 * mh + ((j & 3) >> 1);
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const int row = row0 + 8 * u + 4 * h + (j >> 2);
-      const int off = row * (DP * 2) + ((c ^ tile_swz<CPR>(row)) << 4) + ((j & 1) << 3);
+    for (int u = 0; u < 2; ++u) {                       // 8 rows on: the swizzle's bit 1
+      const unsigned at = (addr ^ (unsigned)((db << 6) | (u << 5))) + (unsigned)((row0 + 8 * u) * ROWB);
       if constexpr (std::is_same<T, __bf16>::value) {
-        const at_bf16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((CRAFT_LDS at_bf16x4*)((CRAFT_LDS unsigned char*)t + off));
+        const at_bf16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((CRAFT_LDS at_bf16x4*)at);
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[4 * u + i] = x[i];
       } else {
-        const at_fp16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4f16((CRAFT_LDS at_fp16x4*)((CRAFT_LDS unsigned char*)t + off));
+        const at_fp16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4f16((CRAFT_LDS at_fp16x4*)at);
 #pragma unroll
         for (int i = 0; i < 4; ++i) v[4 * u + i] = (_Float16)x[i];
       }
     }
   } else {
-    const int col = 32 * db + (lane & 31);
 #pragma unroll
     for (int u = 0; u < 2; ++u)
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const int row = row0 + 8 * u + 4 * h + i;
-        v[4 * u + i] = *reinterpret_cast<const float*>(t + row * (DP * 4) + ((((col >> 2) ^ tile_swz<CPR>(row)) << 4) | ((col & 3) << 2)));
+        const int f = at_cpr<T, DP>() >= 16 ? (i << 2) : ((i >> 1) & 1) << 2;          // tile_swz of row 8 u + 4 h + i, less that of 4 h
+        const unsigned at = (addr ^ (unsigned)((db << 7) ^ (f << 4) ^ (u << 5))) + (unsigned)((row0 + 8 * u + i) * ROWB);
+        v[4 * u + i] = *reinterpret_cast<CRAFT_LDS float*>(at);
       }
   }
   return v;

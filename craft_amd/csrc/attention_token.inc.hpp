@@ -10,9 +10,9 @@ namespace craft {
 
 template <typename T, int DP> struct TokenShape {
   static constexpr int TILE = 32 * DP * (int)sizeof(T);
-  static constexpr int STAGE = 2 * TILE + 256;
-  static constexpr int WAVES = STAGE > 17 * 1024 ? 2 : 4;
-  static constexpr int NST = STAGE * WAVES * 4 <= 132 * 1024 ? 4 : 2;     // about 64 KB of copies in flight per CU either way
+  static constexpr int STAGE = 2 * TILE + 512;
+  static constexpr int WAVES = STAGE > 20 * 1024 ? 2 : 4;
+  static constexpr int NST = STAGE * WAVES * 4 <= 144 * 1024 ? 4 : 2;     // about 64 KB of copies in flight per CU either way
   static constexpr int JOIN = WAVES * 32 * ((DP + 4) * 4 + 8);
   static constexpr int RING = WAVES * NST * STAGE;
   static constexpr int LDS = RING > JOIN ? RING : JOIN;
@@ -23,7 +23,7 @@ __global__ __launch_bounds__((TokenShape<T, DP>::WAVES * 64)) void k_attention_t
   typedef TokenShape<T, DP> S;
   typedef typename AtFrag<T>::type frag_t;
   constexpr int W = S::WAVES, NST = S::NST;
-  extern __shared__ __align__(16) unsigned char lds[];
+  extern __shared__ __align__(512) unsigned char lds[];
   const unsigned lds0 = (unsigned)(size_t)(CRAFT_LDS unsigned char*)lds;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
   const int G = p.H / p.Hk, R = p.Nq * G, nrt = (R + 31) >> 5;
@@ -81,15 +81,15 @@ __global__ __launch_bounds__((TokenShape<T, DP>::WAVES * 64)) void k_attention_t
       stage(st == 0 ? NST - 1 : st - 1, t + (NST - 1) * W);
       if (p.dock) asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 1) * (2 * Copy::PER + 1)) : "memory");
       else asm volatile("s_waitcnt vmcnt(%0)" ::"n"((NST - 1) * 2 * Copy::PER) : "memory");
-      unsigned char* K = lds + (wave * NST + st) * S::STAGE;
-      unsigned char* V = K + S::TILE;
+      unsigned char* V = lds + (wave * NST + st) * S::STAGE + S::TILE;
+      const unsigned at = ring + (unsigned)st * S::STAGE, Kr = row_addr<T, DP>(at, lane), Vc = col_addr<T, DP>(at + S::TILE, lane);
       const int* ids = reinterpret_cast<const int*>(V + S::TILE);
       const int k0 = t * 32;
       f32x16 x;
 #pragma unroll
       for (int q = 0; q < 16; ++q) x[q] = 0.f;
 #pragma unroll
-      for (int ks = 0; ks < DP / 16; ++ks) at_mma(tile_row<T, DP>(K, lane & 31, ks, h), qf[ks], x);
+      for (int ks = 0; ks < DP / 16; ++ks) at_mma(row_read<T, DP>(Kr, 0, ks), qf[ks], x);
       const float away = BIAS ? (float)(pos - k0 - 4 * h) : 0.f;
 #pragma unroll
       for (int q = 0; q < 16; ++q) {
@@ -139,7 +139,7 @@ __global__ __launch_bounds__((TokenShape<T, DP>::WAVES * 64)) void k_attention_t
       for (int s2 = 0; s2 < 2; ++s2) {
         const frag_t pf = at_pack<T>(x, s2);
 #pragma unroll
-        for (int d = 0; d < DP / 32; ++d) at_mma(tile_col<T, DP>(V, 16 * s2, d, lane), pf, o[d]);
+        for (int d = 0; d < DP / 32; ++d) at_mma(col_read<T, DP>(Vc, 16 * s2, d), pf, o[d]);
       }
       st = st == NST - 1 ? 0 : st + 1;
     }
