@@ -132,7 +132,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP < 128 ? 2 : 1)) void k_a
     unsigned char* K = lds + buf * S::STAGE;
     unsigned char* V = K + S::TILE;
     const int* ids = reinterpret_cast<const int*>(V + S::TILE);
-    const unsigned at = lds0 + (unsigned)(buf * S::STAGE), Kr = row_addr<T, DP>(at, lane), Vr = row_addr<T, DP>(at + S::TILE, lane), Kc = col_addr<T, DP>(at, lane);
+    const unsigned at = lds0 + (unsigned)(buf * S::STAGE), Kr = row_addr<T, DP>(at, lane), Kc = col_addr<T, DP>(at, lane);
     const int k0 = t * TK;
     bool docmask = false, skip = k0 >= lim_hi;
     if (rk) {
@@ -150,7 +150,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP < 128 ? 2 : 1)) void k_a
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks) {
           at_mma(row_read<T, DP>(Kr, kbk, ks), qf[ks], x);
-          at_mma(row_read<T, DP>(Vr, kbk, ks), gf[ks], y);
+          at_mma(row_read<T, DP>(Kr, kbk, ks, S::TILE), gf[ks], y);
         }
         const float away = BIAS ? (float)(pos - k0 - 32 * kbk - 4 * h) : 0.f;
         {                                                                 // in steps over all 16 scores: a score's own steps wait for one another
@@ -285,16 +285,22 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP == 32 ? 2 : 1)) void k_a
       }
     return t;
   };
+  // where the head being copied lies
+  const unsigned char *qb, *gb;
+  const float *lb, *db;
+  auto enter = [&](int head) {
+    qb = reinterpret_cast<const unsigned char*>(p.q) + (b * p.q_b + head * p.q_h) * (long)sizeof(T);
+    gb = reinterpret_cast<const unsigned char*>(p.go) + (b * p.go_b + head * p.go_h) * (long)sizeof(T);
+    lb = p.lse + ((long)b * p.H + head) * p.Nq;
+    db = p.delta + ((long)b * p.H + head) * p.Nq;
+  };
   auto stage = [&](int buf, int head, int t) {
     const int valid = p.Nq - t * TQ;
     const unsigned at = lds0 + (unsigned)buf * S::STAGE;
-    const unsigned char* qb = reinterpret_cast<const unsigned char*>(p.q) + (b * p.q_b + head * p.q_h) * (long)sizeof(T);
-    const unsigned char* gb = reinterpret_cast<const unsigned char*>(p.go) + (b * p.go_b + head * p.go_h) * (long)sizeof(T);
     qc.issue(qb + (long)t * TQ * qst, qst, nchunk, valid, at, wave, lane);
     gc.issue(gb + (long)t * TQ * gst, gst, nchunk, valid, at + S::TILE, wave, lane);
-    const long row = ((long)b * p.H + head) * p.Nq;
-    if (wave == 0) copy_words(p.lse + row, (long)t * TQ, p.Nq - 1, at + 2 * S::TILE, lane);
-    if (wave == 1) copy_words(p.delta + row, (long)t * TQ, p.Nq - 1, at + 2 * S::TILE + 256, lane);
+    if (wave == 0) copy_words(lb, (long)t * TQ, p.Nq - 1, at + 2 * S::TILE, lane);
+    if (wave == 1) copy_words(db, (long)t * TQ, p.Nq - 1, at + 2 * S::TILE + 256, lane);
     if (rq && wave == 2) copy_words(p.docq + (long)b * p.Nq, (long)t * TQ, p.Nq - 1, at + 2 * S::TILE + 512, lane);
     if (BIAS && wave == 3) copy_words(p.slopes, head, head, at + 2 * S::TILE + 768, lane);
   };
@@ -309,20 +315,20 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP == 32 ? 2 : 1)) void k_a
   int head = head0, t = next(t0, qr), buf = 0;
   const int tfirst = t;
   const int4 qrfirst = qr;
+  enter(head);
   if (t < t1) stage(0, head, t);
   while (t < t1) {
     wait_copies();
     __syncthreads();
     int tn = next(t + 1, qrn), headn = head;
-    if (tn >= t1 && head + 1 < head1) { tn = tfirst; qrn = qrfirst; headn = head + 1; }
+    if (tn >= t1 && head + 1 < head1) { tn = tfirst; qrn = qrfirst; headn = head + 1; enter(headn); }
     if (tn < t1) stage(buf ^ 1, headn, tn);
     unsigned char* Q = lds + buf * S::STAGE;
     unsigned char* GO = Q + S::TILE;
     const float* lse = reinterpret_cast<const float*>(GO + S::TILE);
     const float* delta = lse + 64;
     const int* ids = reinterpret_cast<const int*>(delta + 64);
-    const unsigned at = lds0 + (unsigned)(buf * S::STAGE), Qr = row_addr<T, DP>(at, lane), GOr = row_addr<T, DP>(at + S::TILE, lane),
-                   Qc = col_addr<T, DP>(at, lane), GOc = col_addr<T, DP>(at + S::TILE, lane);
+    const unsigned at = lds0 + (unsigned)(buf * S::STAGE), Qr = row_addr<T, DP>(at, lane), Qc = col_addr<T, DP>(at, lane);
     const int i0 = t * TQ;
     bool docmask = false, skip = p.causal && prefix <= jw && i0 + TQ - 1 + off < jw;
     if (rq) {
@@ -347,7 +353,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP == 32 ? 2 : 1)) void k_a
 #pragma unroll
         for (int ks = 0; ks < DP / 16; ++ks) {
           at_mma(row_read<T, DP>(Qr, ib, ks), kf[ks], x);
-          at_mma(row_read<T, DP>(GOr, ib, ks), S::VL ? row_read<T, DP>(VTr, 0, ks) : vf[S::VL ? 0 : ks], y);
+          at_mma(row_read<T, DP>(Qr, ib, ks, S::TILE), S::VL ? row_read<T, DP>(VTr, 0, ks) : vf[S::VL ? 0 : ks], y);
         }
         const float away = BIAS ? (float)(key - off - i0 - 32 * ib - 4 * h) : 0.f;
         // in steps over all 16 scores: a score's own steps wait for one another
@@ -392,7 +398,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP == 32 ? 2 : 1)) void k_a
           const frag_t pf = at_pack<T>(x, s2), sf = at_pack<T>(y, s2);
 #pragma unroll
           for (int d = 0; d < DP / 32; ++d) {
-            at_mma(col_read<T, DP>(GOc, 32 * ib + 16 * s2, d), pf, dv[d]);
+            at_mma(col_read<T, DP>(Qc, 32 * ib + 16 * s2, d, S::TILE), pf, dv[d]);
             at_mma(col_read<T, DP>(Qc, 32 * ib + 16 * s2, d), sf, dk[d]);
           }
         }

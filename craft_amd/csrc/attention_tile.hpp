@@ -75,14 +75,14 @@ __device__ __forceinline__ unsigned row_addr(unsigned tile, int lane) {
   const int row = lane & 31, h = lane >> 5, f = tile_swz<at_cpr<T, DP>()>(row);
   return tile + (unsigned)(row * at_rowb<T, DP>() + (((sizeof(T) == 2 ? h : 2 * h) ^ f) << 4));
 }
-// row read: columns 16 ks + 8 h .. + 7 of row 32 blk + (lane & 31)
+// row read: columns 16 ks + 8 h .. + 7 of row 32 blk + (lane & 31); `more`: in the tile that many bytes on (one exclusive or for both)
 template <typename T, int DP>
-__device__ __forceinline__ typename AtFrag<T>::type row_read(unsigned addr, int blk, int ks) {
+__device__ __forceinline__ typename AtFrag<T>::type row_read(unsigned addr, int blk, int ks, int more = 0) {
   if constexpr (sizeof(T) == 2) {
-    return *reinterpret_cast<CRAFT_LDS typename AtFrag<T>::type*>((addr ^ (unsigned)(ks << 5)) + (unsigned)(blk * 32 * at_rowb<T, DP>()));
+    return *reinterpret_cast<CRAFT_LDS typename AtFrag<T>::type*>((addr ^ (unsigned)(ks << 5)) + (unsigned)(blk * 32 * at_rowb<T, DP>() + more));
   } else {
-    const f32x4 a = *reinterpret_cast<CRAFT_LDS f32x4*>((addr ^ (unsigned)(ks << 6)) + (unsigned)(blk * 32 * at_rowb<T, DP>()));
-    const f32x4 b = *reinterpret_cast<CRAFT_LDS f32x4*>((addr ^ (unsigned)(ks << 6) ^ 16u) + (unsigned)(blk * 32 * at_rowb<T, DP>()));
+    const f32x4 a = *reinterpret_cast<CRAFT_LDS f32x4*>((addr ^ (unsigned)(ks << 6)) + (unsigned)(blk * 32 * at_rowb<T, DP>() + more));
+    const f32x4 b = *reinterpret_cast<CRAFT_LDS f32x4*>((addr ^ (unsigned)(ks << 6) ^ 16u) + (unsigned)(blk * 32 * at_rowb<T, DP>() + more));
     f32x8 v;
 #pragma unroll
     for (int j = 0; j < 4; ++j) { v[j] = a[j]; v[4 + j] = b[j]; }
@@ -103,13 +103,13 @@ __device__ __forceinline__ unsigned col_addr(unsigned tile, int lane) {
 }
 // transposing read: column 32 db + (lane & 31) of rows row0 + 4 h + {0..3} and row0 + 8 + 4 h + {0..3} (accumulator order), row0 a multiple of 16
 template <typename T, int DP>
-__device__ __forceinline__ typename AtFrag<T>::type col_read(unsigned addr, int row0, int db) {
+__device__ __forceinline__ typename AtFrag<T>::type col_read(unsigned addr, int row0, int db, int more = 0) {
   constexpr int ROWB = at_rowb<T, DP>();
   typename AtFrag<T>::type v;
   if constexpr (sizeof(T) == 2) {
 #pragma unroll
     for (int u = 0; u < 2; ++u) {                       // 8 rows on: the swizzle's bit 1
-      const unsigned at = (addr ^ (unsigned)((db << 6) | (u << 5))) + (unsigned)((row0 + 8 * u) * ROWB);
+      const unsigned at = (addr ^ (unsigned)((db << 6) | (u << 5))) + (unsigned)((row0 + 8 * u) * ROWB + more);
       if constexpr (std::is_same<T, __bf16>::value) {
         const at_bf16x4 x = __builtin_amdgcn_ds_read_tr16_b64_v4bf16((CRAFT_LDS at_bf16x4*)at);
 #pragma unroll
@@ -126,7 +126,7 @@ __device__ __forceinline__ typename AtFrag<T>::type col_read(unsigned addr, int 
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int f = at_cpr<T, DP>() >= 16 ? (i << 2) : ((i >> 1) & 1) << 2;          // tile_swz of row 8 u + 4 h + i, less that of 4 h
-        const unsigned at = (addr ^ (unsigned)((db << 7) ^ (f << 4) ^ (u << 5))) + (unsigned)((row0 + 8 * u + i) * ROWB);
+        const unsigned at = (addr ^ (unsigned)((db << 7) ^ (f << 4) ^ (u << 5))) + (unsigned)((row0 + 8 * u + i) * ROWB + more);
         v[4 * u + i] = *reinterpret_cast<CRAFT_LDS float*>(at);
       }
   }
@@ -205,9 +205,8 @@ struct TileCopy {
   }
   __device__ __forceinline__ static void one(const u32x4_at& d, unsigned v, unsigned lds) {
     const unsigned dst = __builtin_amdgcn_readfirstlane(lds);
-    unsigned keep;
-    asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
-                 : "=&s"(keep) : "v"(v), "s"(dst), "s"(d) : "memory");
+    // (m0 holds the LDS address; a copy may follow its setting after one wait state)
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %2, 0 offen lds" ::"v"(v), "s"(dst), "s"(d) : "memory", "m0");
   }
 };
 // 64 words base[min(first + lane, last)] -> LDS, by one wave
@@ -218,11 +217,9 @@ __device__ __forceinline__ void copy_words(const void* base, long first, long la
   d[1] = __builtin_amdgcn_readfirstlane((unsigned)(a >> 32));
   d[2] = 0xffffffffu;
   d[3] = 0x00020000u;
-  const unsigned v = 4u * (unsigned)min((long)lane, last - first);
+  const unsigned v = 4u * (unsigned)min(lane, (int)min(last - first, 63l));
   const unsigned dst = __builtin_amdgcn_readfirstlane(lds);
-  unsigned keep;
-  asm volatile("s_mov_b32 %0, m0\n\ts_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dword %1, %3, 0 offen lds\n\ts_mov_b32 m0, %0"
-               : "=&s"(keep) : "v"(v), "s"(dst), "s"(d) : "memory");
+  asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tbuffer_load_dword %0, %2, 0 offen lds" ::"v"(v), "s"(dst), "s"(d) : "memory", "m0");
 }
 __device__ __forceinline__ void wait_copies() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
