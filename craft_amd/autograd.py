@@ -1207,32 +1207,32 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 
 
 class Attention(Function):
-    """ops.attention with its gradients; keeps q, k, v, the output and one log-sum per query."""
+    """ops.attention with its gradients; keeps q, k, v, the output (16-bit types: and what its rounding left) and one log-sum per query."""
 
     @staticmethod
     def forward(ctx, q, k, v, scale, cap, slopes, causal, prefix, docs, docs_k):
         plan = ops.AttentionPlan(q, k, v, scale, cap, slopes, causal, prefix, docs, docs_k)
         B, Nq, Nk, H, Hk, D = plan.dims
         out = torch.empty(B, Nq, H, D, device=plan.device, dtype=q.dtype)
-        lse = torch.empty(B, H, Nq, device=plan.device, dtype=torch.float32)
+        lse, rest = plan.saved()
         if out.numel() and Nk:
-            plan.forward(out, lse)
+            plan.forward(out, lse, rest)
         else:
             out.zero_()
-        ctx.save_for_backward(q, k, v, out, lse, slopes, prefix, docs, docs_k)
+        ctx.save_for_backward(q, k, v, out, lse, rest, slopes, prefix, docs, docs_k)
         ctx.how = scale, cap, causal
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, go):
-        q, k, v, out, lse, slopes, prefix, docs, docs_k = ctx.saved_tensors
-        rest = (None,) * 7
+        q, k, v, out, lse, rest, slopes, prefix, docs, docs_k = ctx.saved_tensors
+        none = (None,) * 7
         if not out.numel() or not k.shape[1]:
-            return (torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), *rest)
+            return (torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), *none)
         scale, cap, causal = ctx.how
         with torch.no_grad():
-            return (*ops.AttentionPlan(q, k, v, scale, cap, slopes, causal, prefix, docs, docs_k).backward(out, lse, go), *rest)
+            return (*ops.AttentionPlan(q, k, v, scale, cap, slopes, causal, prefix, docs, docs_k).backward(out, lse, rest, go), *none)
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optional[float] = None, cap: float = 0.0, slopes: Optional[torch.Tensor] = None,

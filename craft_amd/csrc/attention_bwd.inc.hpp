@@ -22,6 +22,11 @@ __global__ __launch_bounds__(256) void k_attention_delta(AttentionParams p, floa
     const frag_t g = *reinterpret_cast<const frag_t*>(reinterpret_cast<const T*>(p.go) + b * p.go_b + i * p.go_n + head * p.go_h + c);
 #pragma unroll
     for (int j = 0; j < 8; ++j) s += (float)o[j] * (float)g[j];
+    if (sizeof(T) == 2 && p.o_rest) {
+      const frag_t r = *reinterpret_cast<const frag_t*>(reinterpret_cast<const T*>(p.o_rest) + row * p.D + c);
+#pragma unroll
+      for (int j = 0; j < 8; ++j) s += (float)r[j] * (float)g[j];
+    }
   }
 #pragma unroll
   for (int k = 8; k > 0; k >>= 1) s += __shfl_xor(s, k);
@@ -36,8 +41,9 @@ template <typename T, int DP> struct BwdShape {
 };
 
 // the key / value kernel's tiles.  Two 16-bit operands and two fp32 results of 128 columns leave no room for two waves to a SIMD in registers: there V is
-// read from LDS (the block's 128 keys stay there), and tiles are 32 rows so that two blocks share a compute unit (558 -> XXX us for the capped 4096-token step)
+// read from LDS (the block's 128 keys stay there), and tiles are 32 rows so that two blocks share a compute unit (558 -> 404 us for the capped 4096-token step)
 template <typename T, int DP> struct DkvShape {
+  static_assert(sizeof(T) == 2 || BwdShape<T, DP>::TR * at_lw<T>() <= 64, "a tile's log-sums are one copy");
   static constexpr bool VL = sizeof(T) == 2 && DP == 128;
   static constexpr int TR = VL ? 32 : BwdShape<T, DP>::TR;
   static constexpr int TILE = TR * DP * (int)sizeof(T);
@@ -73,7 +79,8 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP < 128 ? 2 : 1)) void k_a
   frag_t qf[DP / 16], gf[DP / 16];
   load_own<T, DP>(reinterpret_cast<const T*>(p.q) + b * p.q_b + (long)i * p.q_n + head * p.q_h, p.D, h, qf);
   load_own<T, DP>(reinterpret_cast<const T*>(p.go) + b * p.go_b + (long)i * p.go_n + head * p.go_h, p.D, h, gf);
-  float row[2] = {p.lse[(long)bh * p.Nq + i], p.delta[(long)bh * p.Nq + i]};
+  const float* lp = p.lse + ((long)bh * p.Nq + i) * at_lw<T>();
+  float row[3] = {lp[0], p.delta[(long)bh * p.Nq + i], at_lw<T>() == 2 ? lp[1] : 0.f};
   arrived(qf);
   arrived(gf);
   arrived(row);
@@ -161,7 +168,11 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP < 128 ? 2 : 1)) void k_a
           }
 #pragma unroll
           for (int q = 0; q < 16; ++q)
-            x[q] = BIAS ? fmaf(-slope2, fabsf(away - (float)acc_row(q)), fmaf(x[q], mul, -lse)) : fmaf(x[q], mul, -lse);
+          {
+            float z = fmaf(x[q], mul, -lse);
+            if constexpr (BIAS) z = fmaf(-slope2, fabsf(away - (float)acc_row(q)), z);
+            x[q] = at_lw<T>() == 2 ? z - row[2] : z;
+          }
           __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int q = 0; q < 16; ++q) x[q] = __builtin_amdgcn_exp2f(x[q]);
@@ -291,7 +302,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP == 32 ? 2 : 1)) void k_a
   auto enter = [&](int head) {
     qb = reinterpret_cast<const unsigned char*>(p.q) + (b * p.q_b + head * p.q_h) * (long)sizeof(T);
     gb = reinterpret_cast<const unsigned char*>(p.go) + (b * p.go_b + head * p.go_h) * (long)sizeof(T);
-    lb = p.lse + ((long)b * p.H + head) * p.Nq;
+    lb = p.lse + ((long)b * p.H + head) * p.Nq * at_lw<T>();
     db = p.delta + ((long)b * p.H + head) * p.Nq;
   };
   auto stage = [&](int buf, int head, int t) {
@@ -299,7 +310,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP == 32 ? 2 : 1)) void k_a
     const unsigned at = lds0 + (unsigned)buf * S::STAGE;
     qc.issue(qb + (long)t * TQ * qst, qst, nchunk, valid, at, wave, lane);
     gc.issue(gb + (long)t * TQ * gst, gst, nchunk, valid, at + S::TILE, wave, lane);
-    if (wave == 0) copy_words(lb, (long)t * TQ, p.Nq - 1, at + 2 * S::TILE, lane);
+    if (wave == 0) copy_words(lb, (long)t * TQ * at_lw<T>(), (long)p.Nq * at_lw<T>() - 1, at + 2 * S::TILE, lane);
     if (wave == 1) copy_words(db, (long)t * TQ, p.Nq - 1, at + 2 * S::TILE + 256, lane);
     if (rq && wave == 2) copy_words(p.docq + (long)b * p.Nq, (long)t * TQ, p.Nq - 1, at + 2 * S::TILE + 512, lane);
     if (BIAS && wave == 3) copy_words(p.slopes, head, head, at + 2 * S::TILE + 768, lane);
@@ -364,11 +375,21 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP == 32 ? 2 : 1)) void k_a
         }
 #pragma unroll
         for (int g = 0; g < 4; ++g) {
-          const f32x4 le = *reinterpret_cast<const f32x4*>(lse + 32 * ib + 8 * g + 4 * h);
+          float le[4], rest[4];
+          if constexpr (at_lw<T>() == 2) {
+            const f32x4 u = *reinterpret_cast<const f32x4*>(lse + 2 * (32 * ib + 8 * g + 4 * h)), v = *reinterpret_cast<const f32x4*>(lse + 2 * (32 * ib + 8 * g + 4 * h) + 4);
+            le[0] = u[0]; rest[0] = u[1]; le[1] = u[2]; rest[1] = u[3]; le[2] = v[0]; rest[2] = v[1]; le[3] = v[2]; rest[3] = v[3];
+          } else {
+            const f32x4 u = *reinterpret_cast<const f32x4*>(lse + 32 * ib + 8 * g + 4 * h);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) { le[e] = u[e]; rest[e] = 0.f; }
+          }
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int r = 4 * g + e;
-            x[r] = BIAS ? fmaf(-slope2, fabsf(away - (float)acc_row(r)), fmaf(x[r], mul, -le[e])) : fmaf(x[r], mul, -le[e]);
+            float z = fmaf(x[r], mul, -le[e]);
+            if constexpr (BIAS) z = fmaf(-slope2, fabsf(away - (float)acc_row(r)), z);
+            x[r] = at_lw<T>() == 2 ? z - rest[e] : z;
           }
         }
         __builtin_amdgcn_sched_barrier(0);

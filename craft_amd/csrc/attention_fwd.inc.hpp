@@ -195,13 +195,23 @@ __global__ __launch_bounds__(256, 2) void k_attention_fwd(AttentionParams p) {
       for (int g = 0; g < 4; ++g) {
         const int c = 32 * d + 8 * g + 4 * h;
         if (c < p.D) {
-          t4 w;
+          t4 w, rest;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) w[j] = (T)(o[d][4 * g + j] * inv);
+          for (int j = 0; j < 4; ++j) {
+            const float v = o[d][4 * g + j] * inv;
+            w[j] = (T)v;
+            rest[j] = (T)(v - (float)w[j]);
+          }
           *reinterpret_cast<t4*>(orow + c) = w;
+          if (sizeof(T) == 2 && p.rest) *reinterpret_cast<t4*>(reinterpret_cast<T*>(p.rest) + (((long)b * p.Nq + i) * p.H + head) * p.D + c) = rest;
         }
       }
-    if (p.lse && h == 0) p.lse[(long)bh * p.Nq + i] = l > 0.f ? m * c2 + __log2f(l) : INFINITY;
+    if (p.lse && h == 0) {
+      float* lse = p.lse + ((long)bh * p.Nq + i) * at_lw<T>();
+      const float big = m * c2, small = __log2f(l), sum = big + small;
+      lse[0] = l > 0.f ? sum : INFINITY;
+      if (at_lw<T>() == 2) lse[1] = l > 0.f ? small - (sum - big) : 0.f;
+    }
   }
 }
 

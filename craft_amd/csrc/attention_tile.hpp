@@ -36,7 +36,10 @@ struct AttentionParams {
   const int *prefix, *docq, *dock;             // [B], [B][Nq], [B][Nk]; each may be null
   const int4 *rq, *rk;                         // per 32 tokens: {least document, greatest document, any negative one, 0}
   int causal;
-  float* lse;                                  // [B][H][Nq] log2 of the sum of 2^z; +inf for a query that sees nothing (so that 2^(z - lse) = 0)
+  float* lse;                                  // [B][H][Nq] log2 of the sum of 2^z; +inf for a query that sees nothing (so that 2^(z - lse) = 0).  fp32 tensors:
+                                               // [B][H][Nq][2], with what its rounding left (a log-sum of 20 is rounded by 1e-6, the whole row's gradients with it)
+  void* rest; const void* o_rest;              // 16-bit: what o's rounding left, like o contiguous [B][Nq][H][D]: delta is a difference of sums that the
+                                               // rounding of o would disturb as much as the gradients' own (written with lse, read for delta; may be null)
   const float* delta;                          // [B][H][Nq] -sum_d go * o
   float *part_o, *part_ml;                     // token kernel: partial results of the splits
   int splits;
@@ -142,6 +145,8 @@ __device__ __forceinline__ typename AtFrag<T>::type at_pack(const f32x16& x, int
   for (int j = 0; j < 8; ++j) v[j] = (T)x[8 * s + j];
   return v;
 }
+
+template <typename T> constexpr int at_lw() { return sizeof(T) == 4 ? 2 : 1; }       // words of a log-sum
 
 // the row of a 32-row block that register r of a lane holds, less 4 h
 __device__ __forceinline__ constexpr int acc_row(int r) { return 8 * (r >> 2) + (r & 3); }

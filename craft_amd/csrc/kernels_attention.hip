@@ -81,14 +81,15 @@ using namespace craft;
 extern "C" {
 
 int craft_attention_fwd(const void* q, const void* k, const void* v, const long* shape, const float* slopes, const int* prefix, const int* doc_q,
-                        const int* doc_k, float scale, float cap, int causal, int dtype, int splits, void* out, float* lse, void* ws, long ws_bytes, void* stream) {
+                        const int* doc_k, float scale, float cap, int causal, int dtype, int splits, void* out, float* lse, void* out_rest, void* ws,
+                        long ws_bytes, void* stream) {
   AttentionParams p;
   const int rc = fill(p, shape, 4, slopes, prefix, doc_q, doc_k, scale, cap, causal, dtype);
   if (rc) return rc;
   if (!aligned(q) || !aligned(k) || !aligned(v) || !aligned(out)) return CRAFT_ERR_ALIGN;
-  if (splits < 0 || splits > 65535 || (splits && lse)) return CRAFT_ERR_ARG;
+  if (splits < 0 || splits > 65535 || (splits && (lse || out_rest)) || (reinterpret_cast<uintptr_t>(out_rest) & 15)) return CRAFT_ERR_ARG;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  p.q = q; p.k = k; p.v = v; p.out = out; p.lse = lse;
+  p.q = q; p.k = k; p.v = v; p.out = out; p.lse = lse; p.rest = out_rest;
   if (splits) {
     p.splits = splits;
     if (splits > 1) {
@@ -104,18 +105,19 @@ int craft_attention_fwd(const void* q, const void* k, const void* v, const long*
   return rr ? rr : dispatch(p, dtype, 0, s);
 }
 
-int craft_attention_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse, const void* grad_out, const long* shape,
+int craft_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* out_rest, const float* lse, const void* grad_out,
+                        const long* shape,
                         const float* slopes, const int* prefix, const int* doc_q, const int* doc_k, float scale, float cap, int causal, int dtype,
                         int split_group, void* dq, void* dk, void* dv, void* ws, long ws_bytes, void* stream) {
   AttentionParams p;
   const int rc = fill(p, shape, 5, slopes, prefix, doc_q, doc_k, scale, cap, causal, dtype);
   if (rc) return rc;
   if (!aligned(q) || !aligned(k) || !aligned(v) || !aligned(out) || !aligned(grad_out) || !aligned(dq) || !aligned(dk) || !aligned(dv)) return CRAFT_ERR_ALIGN;
-  if (!lse) return CRAFT_ERR_ARG;
+  if (!lse || (reinterpret_cast<uintptr_t>(out_rest) & 15)) return CRAFT_ERR_ARG;
   const long ranges = range_bytes(p), delta = ((long)p.B * p.H * p.Nq * 4 + 15) / 16 * 16, part = split_group ? (long)p.B * p.Nk * p.H * p.D * 4 : 0;
   if (!aligned(ws) || ws_bytes < ranges + delta + 2 * part) return CRAFT_ERR_ARG;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
-  p.q = q; p.k = k; p.v = v; p.o = out; p.go = grad_out; p.lse = const_cast<float*>(lse); p.dq = dq; p.dk = dk; p.dv = dv;
+  p.q = q; p.k = k; p.v = v; p.o = out; p.o_rest = out_rest; p.go = grad_out; p.lse = const_cast<float*>(lse); p.dq = dq; p.dk = dk; p.dv = dv;
   char* w = reinterpret_cast<char*>(ws) + ranges;
   p.delta = reinterpret_cast<float*>(w);
   if (split_group) { p.part_k = reinterpret_cast<float*>(w + delta); p.part_v = reinterpret_cast<float*>(w + delta + part); }

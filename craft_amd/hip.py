@@ -124,8 +124,8 @@ _SIGS = {
     # ---- LayerNorm with weights, attention, orthogonalisation
     "craft_layer_norm_fwd": [P, L, P, P, L, I, F, I, I, P, L, P, P, P],
     "craft_layer_norm_bwd": [P, L, P, L, P, P, P, L, I, I, I, P, L, P, P, P, I, P],
-    "craft_attention_fwd": [P, P, P, P, P, P, P, P, F, F, I, I, I, P, P, P, L, P],
-    "craft_attention_bwd": [P, P, P, P, P, P, P, P, P, P, P, F, F, I, I, I, P, P, P, P, L, P],
+    "craft_attention_fwd": [P, P, P, P, P, P, P, P, F, F, I, I, I, P, P, P, P, L, P],
+    "craft_attention_bwd": [P, P, P, P, P, P, P, P, P, P, P, P, F, F, I, I, I, P, P, P, P, L, P],
     "craft_orthogonalize": [P, I, P, I, F, F, F, F, I, P, L, P],
     "craft_muon_momentum": [P, P, P, P, I, F, I, P, P],
     "craft_muon_apply": [P, P, P, P, I, F, F, P, P],

@@ -939,15 +939,22 @@ class AttentionPlan:
             return 0
         return max(1, min(512 // (B * Hk * ((rows + 31) // 32)), (Nk + 255) // 256))
 
-    def forward(self, out: torch.Tensor, lse: Optional[torch.Tensor]):
+    def forward(self, out: torch.Tensor, lse: Optional[torch.Tensor] = None, rest: Optional[torch.Tensor] = None):
         B, Nq, Nk, H, Hk, D = self.dims
         splits = 0 if lse is not None else self.splits()
         nbytes = self.range_bytes() if not splits else 4 * B * Nq * H * splits * (D + 2) if splits > 1 else 0
         with _on(self.device):
             call("craft_attention_fwd", self.q, self.k, self.v, self.shape(out), *self.masks(), self.scale, self.cap, self.causal, self.code, splits, out,
-                 lse, self.new(nbytes), nbytes)
+                 lse, rest, self.new(nbytes), nbytes)
 
-    def backward(self, out: torch.Tensor, lse: torch.Tensor, go: torch.Tensor):
+    def saved(self):
+        """(log-sums, the rest of the output's rounding or None) for the forward pass to fill and the backward pass to read."""
+        B, Nq, Nk, H, Hk, D = self.dims
+        if self.code == PREC_F32:
+            return torch.empty(B, H, Nq, 2, device=self.device, dtype=torch.float32), None
+        return torch.empty(B, H, Nq, device=self.device, dtype=torch.float32), torch.empty(B, Nq, H, D, device=self.device, dtype=self.q.dtype)
+
+    def backward(self, out: torch.Tensor, lse: torch.Tensor, rest: Optional[torch.Tensor], go: torch.Tensor):
         B, Nq, Nk, H, Hk, D = self.dims
         go = _strided(go.to(self.q.dtype))
         dq = torch.empty(B, Nq, H, D, device=self.device, dtype=self.q.dtype)
@@ -956,7 +963,7 @@ class AttentionPlan:
         split_group = int(H > Hk and B * Hk * ((Nk + 127) // 128) < 512)
         nbytes = self.range_bytes() + (4 * B * H * Nq + 15) // 16 * 16 + split_group * 8 * B * Nk * H * D
         with _on(self.device):
-            call("craft_attention_bwd", self.q, self.k, self.v, out, lse, go, self.shape(out, go), *self.masks(), self.scale, self.cap, self.causal, self.code,
+            call("craft_attention_bwd", self.q, self.k, self.v, out, rest, lse, go, self.shape(out, go), *self.masks(), self.scale, self.cap, self.causal, self.code,
                  split_group, dq, dk, dv, self.new(nbytes), nbytes)
         return dq, dk, dv
 
@@ -982,5 +989,5 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optio
         if out.numel() and not k.shape[1]:
             return out.zero_()
         if out.numel():
-            plan.forward(out, None)
+            plan.forward(out)
         return out

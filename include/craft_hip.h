@@ -669,16 +669,18 @@ int craft_layer_norm_bwd(const void* x, long ldx, const void* dy, long lddy, con
  *   cap 0: no cap;  slopes: [H] fp32, NULL: no bias.
  * shape: 18 host longs B, Nq, Nk, H, Hk, D, then the (batch, token, head) strides in elements of q, k, v, out.  H % Hk == 0 (query head h reads key head
  * h / (H / Hk)), D % 8 == 0, D <= 128, strides multiples of 16 bytes, pointers 16-byte aligned, the last axis contiguous.
- * splits 0: blocks of 128 queries, whose log2-sums go to lse ([B][H][Nq], NULL: not wanted; +inf where nothing is seen).  splits >= 1: for a few rows
- * (Nq * H / Hk up to about 64): the keys split over so many blocks; no lse.
+ * splits 0: blocks of 128 queries.  For the backward pass they leave the log2-sums in lse ([B][H][Nq]; fp32: [B][H][Nq][2] with their rounding's rest; +inf
+ * where nothing is seen) and, 16-bit types, the rest of out's rounding in out_rest (contiguous [B][Nq][H][D], 16-byte aligned); either may be NULL.
+ * splits >= 1: for a few rows (Nq * H / Hk up to about 64): the keys split over so many blocks; no lse, no out_rest.
  * ws (16-byte aligned): splits 0 with documents: 16 * B * (ceil(Nq / 32) + ceil(Nk / 32)) bytes;  splits > 1: B * Nq * H * splits * (D + 2) floats. */
 int craft_attention_fwd(const void* q, const void* k, const void* v, const long* shape, const float* slopes, const int* prefix, const int* doc_q,
-                        const int* doc_k, float scale, float cap, int causal, int dtype, int splits, void* out, float* lse, void* ws, long ws_bytes, void* stream);
-/* gradients of q [B][Nq][H][D], k and v [B][Nk][Hk][D], contiguous.  shape: 21 host longs, as above with the strides of grad_out last.
+                        const int* doc_k, float scale, float cap, int causal, int dtype, int splits, void* out, float* lse, void* out_rest, void* ws,
+                        long ws_bytes, void* stream);
+/* gradients of q [B][Nq][H][D], k and v [B][Nk][Hk][D], contiguous.  out_rest may be NULL (the gradients are then off by out's rounding too).  shape: 21 host longs, as above with the strides of grad_out last.
  * split_group 1: a block per query head for the key / value gradients and a sum over the heads of a group behind it (more blocks, fp32 partial results).
  * ws (16-byte aligned): the documents' ranges as above, then B * H * Nq floats rounded up to 16 bytes, then with split_group 2 * B * Nk * H * D floats.
  * The result does not depend on the order in which blocks run. */
-int craft_attention_bwd(const void* q, const void* k, const void* v, const void* out, const float* lse, const void* grad_out, const long* shape,
+int craft_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* out_rest, const float* lse, const void* grad_out, const long* shape,
                         const float* slopes, const int* prefix, const int* doc_q, const int* doc_k, float scale, float cap, int causal, int dtype,
                         int split_group, void* dq, void* dk, void* dv, void* ws, long ws_bytes, void* stream);
 

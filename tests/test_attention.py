@@ -102,9 +102,9 @@ def test_entry_points_check_their_arguments():
     buf = 4096                                                             # an aligned address that is never read: every call below is refused first
     good = [1, 4, 4, 2, 2, 16] + [128, 32, 16] * 4
 
-    def fwd(shape=good, q=buf, k=buf, v=buf, out=buf, scale=1.0, cap=0.0, causal=0, dtype=2, splits=0, docs=(None, None), prefix=None, ws=None, ws_bytes=0, lse=None):
+    def fwd(shape=good, q=buf, k=buf, v=buf, out=buf, scale=1.0, cap=0.0, causal=0, dtype=2, splits=0, docs=(None, None), prefix=None, ws=None, ws_bytes=0, lse=None, rest=None):
         return lib.craft_attention_fwd(q, k, v, (ctypes.c_long * len(shape))(*shape), None, prefix, docs[0], docs[1], scale, cap, causal, dtype, splits, out, lse,
-                                       ws, ws_bytes, None)
+                                       rest, ws, ws_bytes, None)
 
     def with_(i, x):
         s = list(good)
@@ -117,9 +117,9 @@ def test_entry_points_check_their_arguments():
     assert fwd(q=buf + 8) == ALIGN and fwd(k=None) == ALIGN and fwd(out=buf + 2) == ALIGN
     assert fwd(dtype=3) == ARG and fwd(cap=-1.0) == ARG and fwd(cap=float("nan")) == ARG and fwd(scale=float("nan")) == ARG
     assert fwd(docs=(buf, None)) == ARG and fwd(docs=(buf, buf)) == ARG                      # (no workspace for the ranges)
-    assert fwd(prefix=buf) == ARG and fwd(splits=-1) == ARG and fwd(splits=2) == ARG and fwd(splits=1, lse=buf) == ARG
+    assert fwd(prefix=buf) == ARG and fwd(splits=-1) == ARG and fwd(splits=2) == ARG and fwd(splits=1, lse=buf) == ARG and fwd(splits=1, rest=buf) == ARG and fwd(rest=buf + 8) == ARG
     shape5 = (ctypes.c_long * 21)(*(good + [128, 32, 16]))
-    bwd = lambda ws, n, lse=buf, dk=buf: lib.craft_attention_bwd(buf, buf, buf, buf, lse, buf, shape5, None, None, None, None, 1.0, 0.0, 0, 2, 1, buf, dk, buf, ws, n, None)  # noqa: E731
+    bwd = lambda ws, n, lse=buf, dk=buf: lib.craft_attention_bwd(buf, buf, buf, buf, None, lse, buf, shape5, None, None, None, None, 1.0, 0.0, 0, 2, 1, buf, dk, buf, ws, n, None)  # noqa: E731
     assert bwd(None, 0) == ARG and bwd(buf, 31) == ARG and bwd(buf, 1 << 20, lse=None) == ARG and bwd(buf, 1 << 20, dk=buf + 4) == ALIGN
 
 
