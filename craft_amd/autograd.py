@@ -1191,18 +1191,20 @@ class LayerNorm(Function):
     def forward(ctx, x, weight, bias, eps):
         y, mean, rstd = ops._layer_norm(x, weight, bias, eps, None, True)
         ctx.save_for_backward(x, weight, mean, rstd)
-        ctx.bias_type = None if bias is None else bias.dtype
+        ctx.weight_type = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
         x, weight, mean, rstd = ctx.saved_tensors
-        return (*ops.layer_norm_bwd(x, weight, ctx.bias_type, dy, mean, rstd, ctx.needs_input_grad[:3]), None)
+        return (*ops._layer_norm_bwd(x, weight, ctx.weight_type, dy, mean, rstd, ctx.needs_input_grad[:3]), None)
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
     """Differentiable ``ops.layer_norm`` (gradients of x, weight and bias; the weight's and bias' sums over the rows in fp32, in a fixed order)."""
+    if not torch.is_grad_enabled():
+        return ops.layer_norm(x, weight, bias, eps)
     return LayerNorm.apply(x, weight, bias, eps)
 
 
@@ -1242,4 +1244,6 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optio
     the cap have none.  The scores are computed again in the backward pass; no N x N tensor is kept."""
     if slopes is not None and slopes.requires_grad:
         raise hip.CraftHipError("attention: slopes have no gradient here")
+    if not torch.is_grad_enabled():                                        # (a few query rows: the single-token kernel, which keeps no log-sums)
+        return ops.attention(q, k, v, scale=scale, cap=cap, slopes=slopes, causal=causal, prefix=prefix, docs=docs, docs_k=docs_k)
     return Attention.apply(q, k, v, scale, cap, slopes, causal, prefix, docs, docs_k)

@@ -39,6 +39,10 @@ static int fill(AttentionParams& p, const long* shape, int nt, const float* slop
                 int causal, int dtype) {
   if (!shape || dtype < 0 || dtype > 2 || (doc_q == nullptr) != (doc_k == nullptr) || (prefix && !causal)) return CRAFT_ERR_ARG;
   if (!(cap >= 0.f) || !(cap <= 1e30f) || !(fabsf(scale) <= 1e30f)) return CRAFT_ERR_ARG;
+  // 16-bit types take tanh from 1 / (1 + e^2u), off by 2^-23 of 1 however small u is: a capped score is off by cap 2^-22, 2^-10 here.  And a score
+  // of zero times 2 scale / cap has to be zero, which it is not where that overflows.
+  if (cap > 4096.f && dtype != CRAFT_PREC_F32) return CRAFT_ERR_UNSUPPORTED;
+  if (cap > 0.f && !(fabsf(scale) / cap <= 1e30f)) return CRAFT_ERR_ARG;
   for (int i = 0; i < 6; ++i)
     if (shape[i] <= 0 || shape[i] >= (1l << 29)) return CRAFT_ERR_UNSUPPORTED;
   const long size = dtype == CRAFT_PREC_F32 ? 4 : 2, step = 16 / size;
@@ -91,6 +95,7 @@ int craft_attention_fwd(const void* q, const void* k, const void* v, const long*
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   p.q = q; p.k = k; p.v = v; p.out = out; p.lse = lse; p.rest = out_rest;
   if (splits) {
+    if ((long)p.Nq * (p.H / p.Hk) > 1l << 20) return CRAFT_ERR_UNSUPPORTED;
     p.splits = splits;
     if (splits > 1) {
       const long rows = (long)p.B * p.Hk * p.Nq * (p.H / p.Hk) * splits;

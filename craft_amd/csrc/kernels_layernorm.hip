@@ -3,11 +3,10 @@
 //   y = xn w + b,  xn = (x - mean) rstd;      dx = rstd (g - mean(g) - xn mean(g xn)) with g = dy w,   dw = sum_rows dy xn,   db = sum_rows dy
 //
 // HBM-bound: x is read once forward (and the row held in registers for its two statistics, mean first, then the squares about it, in fp32), x and dy once
-// backward.  A row belongs to TPR threads (16 of a wave, a wave, up to 16 waves), with one vector
-// each up to 1024 vectors.
+// backward.  A row belongs to TPR threads (16 of a wave, a wave, up to 16 waves), with one vector each up to 1024 vectors.
 // The weight's and the bias' gradients are summed on the way: a thread owns the same columns of every row it meets, so its sums stay in registers over the
 // block's whole share of the rows; the row groups of a block are joined in LDS, the blocks by k_layer_norm_sum -- each in a fixed order, no atomics.
-// Vectors are 16 bytes at any alignment (unaligned loads and stores are native): an odd width costs its last vector element by element, nothing else.
+// Vectors are 16 bytes at any alignment (unaligned loads and stores are native): an odd width moves its last vector back (LnCols).
 #include <type_traits>
 #include "launch.hpp"
 #include "../../include/craft_hip.h"
@@ -31,7 +30,7 @@ template <typename T> struct LnVec { static constexpr int N = 16 / sizeof(T); };
 
 // A thread's vector j holds columns base .. base + N - 1 of the row, of which those below `lo` belong to its neighbour: the last vector of a row whose
 // width is no multiple of N is moved back to end with the row, so that every load is one whole vector with no branch around it (a branch per vector made
-// the loads of a row wait for one another: 28 us instead of 9 for the gradients of 1441 rows of 1027).  A row narrower than a vector goes element by element.
+// the loads of a row wait for one another: 28 us instead of 11 for the gradients of 1441 rows of 1027).  A row narrower than a vector goes element by element.
 template <int N>
 struct LnCols {
   int base, lo;
@@ -290,7 +289,7 @@ __global__ __launch_bounds__(512) void k_layer_norm_sum(const float* part, int b
 template <typename T, typename W>
 static int layer_norm_run(const LayerNormParams& p, int blocks, void* dw, void* db, hipStream_t s) {
   constexpr int N = LnVec<T>::N;
-  auto go = [&](auto fwd, auto bwd, int tpr, int (*allow)(int)) {
+  auto go = [&](auto fwd, auto bwd, int tpr) {
     if (!p.dy) {
       const int th = tpr > 512 ? tpr : 512, rpb = th / tpr;
       const long most = (p.rows + rpb - 1) / rpb, full = th == 512 ? 768 : 256;      // what the card holds at once (72 registers)
@@ -300,8 +299,7 @@ static int layer_norm_run(const LayerNormParams& p, int blocks, void* dw, void* 
     const int rpb = 1024 / tpr;
     const long most = (p.rows + rpb - 1) / rpb;
     const int grid = most < blocks ? (int)most : blocks;
-    const size_t lds = p.part && rpb > 1 ? (size_t)2 * p.C * 4 : 0;
-    if (lds > 48 * 1024) if (const int rc = allow(2 * 8192 * 4)) return rc;      // (rows of up to 8192 share a block)
+    const size_t lds = p.part && rpb > 1 ? (size_t)2 * p.C * 4 : 0;          // (32 KB at most: wider rows have a block of their own)
     hipLaunchKernelGGL(bwd, dim3((unsigned)grid), dim3(1024), lds, s, p);
     HIP_CHECK_RET(hipGetLastError());
     if (p.part) hipLaunchKernelGGL(k_layer_norm_sum<W>, dim3((unsigned)((2 * p.C + 31) / 32)), dim3(512), 0, s, p.part, grid, p.C, (W*)dw, (W*)db);
@@ -309,8 +307,7 @@ static int layer_norm_run(const LayerNormParams& p, int blocks, void* dw, void* 
   };
   const int nv = (p.C + N - 1) / N;                    // vectors of a row
   const bool tail = p.C % N != 0;
-#define LN_GO(TPR, NV) go(k_layer_norm_fwd<T, W, TPR, NV, (TPR > 512 ? TPR : 512)>, tail ? k_layer_norm_bwd<T, W, TPR, NV, true> : k_layer_norm_bwd<T, W, TPR, NV, false>, TPR, \
-                          tail ? allow_lds<k_layer_norm_bwd<T, W, TPR, NV, true>> : allow_lds<k_layer_norm_bwd<T, W, TPR, NV, false>>)
+#define LN_GO(TPR, NV) go(k_layer_norm_fwd<T, W, TPR, NV, (TPR > 512 ? TPR : 512)>, tail ? k_layer_norm_bwd<T, W, TPR, NV, true> : k_layer_norm_bwd<T, W, TPR, NV, false>, TPR)
   if (nv <= 16) return LN_GO(16, 1);
   if (nv <= 64) return LN_GO(64, 1);
   if (nv <= 128) return LN_GO(128, 1);

@@ -742,9 +742,21 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
 def layer_norm_bwd(x: torch.Tensor, weight: Optional[torch.Tensor], bias_type: Optional[torch.dtype], dy: torch.Tensor, mean: torch.Tensor,
                    rstd: torch.Tensor, need=(True, True, True)):
     """(dx, dweight, dbias) of ``layer_norm`` from its saved row statistics; ``need`` leaves gradients out."""
+    wt = weight.dtype if weight is not None else bias_type or x.dtype
+    rows = x.numel() // max(x.shape[-1], 1) if x.dim() else 0
+    if dy.shape != x.shape or wt not in (x.dtype, torch.float32):
+        raise hip.CraftHipError(f"layer_norm_bwd: dy {tuple(dy.shape)} of rows {tuple(x.shape)}, weights of {wt}")
+    for t in (mean, rstd):
+        if t.numel() != rows or t.dtype != torch.float32 or not t.is_contiguous():
+            raise hip.CraftHipError(f"layer_norm_bwd: mean and rstd must be {rows} contiguous fp32 numbers")
+    _check_layer_norm(x, weight, None, 0.0)
+    _on_device(x, dy, mean, rstd)
+    return _layer_norm_bwd(x, weight, wt, dy, mean, rstd, need)
+
+
+def _layer_norm_bwd(x, weight, wt, dy, mean, rstd, need):
     C = x.shape[-1]
     rows = x.numel() // C
-    wt = weight.dtype if weight is not None else bias_type or x.dtype
     new = lambda want, shape, t: torch.empty(shape, device=x.device, dtype=t) if want else None      # noqa: E731
     dx, dw, db = new(need[0], x.shape, x.dtype), new(need[1], (C,), wt), new(need[2], (C,), wt)
     if not rows:
@@ -794,8 +806,8 @@ def _newton_schulz_coeffs(steps, coeffs):
 def orthogonalize(mats: Sequence[torch.Tensor], steps: int = 5, coeffs=NEWTON_SCHULZ, eps: float = 1e-7, out: Optional[Sequence[torch.Tensor]] = None):
     """Every matrix of the list with its singular values moved towards 1: X = G / (|G|_F + eps), then ``steps`` times X <- a X + (b A + c A A) X with
     A = X X^T from the smaller side.  ``coeffs``: (a, b, c), or one triple a step.  fp32 / fp16 / bf16 matrices of any strides, the smaller side up to
-    32768; fp32-class arithmetic whatever the type, one rounding at the end.  The whole list shares its launches.  ``out`` (may be ``mats``): where the
-    results go.  ``train.FlatMuon`` is the optimizer that uses it."""
+    32768; fp32-class arithmetic whatever the type, one rounding at the end.  The whole list shares its launches.  ``out`` (may be ``mats``, and
+    must not overlap another matrix of it): where the results go.  ``train.FlatMuon`` is the optimizer that uses it."""
     rows = _newton_schulz_coeffs(steps, coeffs)
     scales = _newton_schulz_scales(rows)
     if not 0 <= eps < float("inf"):
@@ -805,6 +817,13 @@ def orthogonalize(mats: Sequence[torch.Tensor], steps: int = 5, coeffs=NEWTON_SC
         out = list(out)
         if len(out) != len(mats):
             raise hip.CraftHipError("orthogonalize: out must be a list of the matrices' shapes, types and devices")
+        # a long list is worked off in parts: a result must not lie where another matrix, or another result, does
+        where = {}
+        for i, o in enumerate(out):
+            if o.numel() and where.setdefault(o.data_ptr(), i) != i:
+                raise hip.CraftHipError("orthogonalize: two results in one place")
+        if any(g.numel() and where.get(g.data_ptr(), i) != i for i, g in enumerate(mats)):
+            raise hip.CraftHipError("orthogonalize: a result in the place of another matrix")
     res, groups, device = [], {}, None
     for i, g in enumerate(mats):                      # (a list of a model's matrices: a microsecond here is fifty)
         shape, code = g.shape, DTYPE_CODE.get(g.dtype)
@@ -889,9 +908,13 @@ class AttentionPlan:
             raise err(f"attention: a head width that is a multiple of 8, up to 128, not {D}")
         if not 0 <= float(cap) <= 1e30:
             raise err("attention: cap must be positive, or 0 for none")
+        if cap > 4096 and q.dtype != torch.float32:
+            raise err("attention: a cap of 4096 at most in 16-bit types (scores would be off by cap 2^-22)")
         scale = D ** -0.5 if scale is None else float(scale)
         if not abs(scale) <= 1e30:
             raise err("attention: scale must be finite")
+        if cap and not abs(scale) / cap <= 1e30:
+            raise err("attention: scale / cap must not pass 1e30")
         if prefix is not None and not causal:
             raise err("attention: a prefix opens a causal mask: pass causal=True")
         if slopes is not None and (slopes.shape != (H,) or slopes.dtype != torch.float32):
@@ -976,16 +999,19 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optio
     q [B, Nq, H, D]; k, v [B, Nk, Hk, D] of the same type (fp32, fp16, bf16), H a multiple of Hk (query head h reads key head h // (H / Hk)), D a multiple
     of 8 up to 128; any strides (views the kernels cannot read in place are copied).  Query i stands at position i + Nk - Nq: new tokens at the end of a
     cache.  scale: 1 / sqrt(D) by default; cap 0: none; slopes [H] fp32.  ``causal``: keys up to the query's position, and with ``prefix`` [B] int32 also
-    the first prefix[b] keys.  ``docs`` [B, Nq] (and ``docs_k`` [B, Nk]) int32: only keys of the query's document; a negative document is padding, which
+    the first prefix[b] keys (a hidden key still counts as 0 times its v, which has to be finite).  ``docs`` [B, Nq] (and ``docs_k`` [B, Nk]) int32: only keys of the query's document; a negative document is padding, which
     nothing sees and whose rows of q, k, v may hold anything.  A query that sees nothing gives zeros.  Softmax sums and products accumulate in fp32;
     16-bit types round the probabilities to their own type for the product with v.  ``flash_attention`` and ``attn_probs`` are the model's own forms over
-    an image's tokens; the differentiable form is ``autograd.attention``."""
+    an image's tokens; the differentiable form is ``autograd.attention``.  ``out`` may be q, and must not overlap k or v."""
     with torch.no_grad():
         plan = AttentionPlan(q, k, v, scale, cap, slopes, causal, prefix, docs, docs_k)
         if out is None:
             out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or _strided(out) is not out:
+        elif (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or _strided(out) is not out
+              or any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride()))):
             raise hip.CraftHipError("attention: out must be of q's shape, type and device, with 16-byte aligned rows")
+        elif out.numel() and out.data_ptr() in (k.data_ptr(), v.data_ptr()):
+            raise hip.CraftHipError("attention: out must not be k's or v's memory, which other blocks still read")
         if out.numel() and not k.shape[1]:
             return out.zero_()
         if out.numel():

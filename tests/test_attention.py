@@ -67,6 +67,8 @@ def test_reference_gradients_are_autograds():
     (dict(k=torch.zeros(1, 4, 2, 16, dtype=torch.float16)), "one type"),
     (dict(q=torch.zeros(1, 4, 2, 16).double(), k=torch.zeros(1, 4, 2, 16).double(), v=torch.zeros(1, 4, 2, 16).double()), "one type"),
     (dict(cap=-1.0), "cap"), (dict(cap=float("nan")), "cap"), (dict(cap=float("inf")), "cap"),
+    (dict(cap=1e-38), "scale / cap"), (dict(cap=1e-20, scale=1e15), "scale / cap"),
+    (dict(q=torch.zeros(1, 4, 2, 16).half(), k=torch.zeros(1, 4, 2, 16).half(), v=torch.zeros(1, 4, 2, 16).half(), cap=4097.0), "4096"),
     (dict(scale=float("inf")), "scale"), (dict(scale=float("nan")), "scale"),
     (dict(prefix=torch.zeros(1, dtype=torch.int32)), "causal=True"),
     (dict(prefix=torch.zeros(2, dtype=torch.int32), causal=True), "prefix must"),
@@ -116,6 +118,7 @@ def test_entry_points_check_their_arguments():
     assert fwd(with_(7, 36)) == ALIGN and fwd(with_(10, -16)) == ALIGN and fwd(with_(10, 1 << 23)) == UNSUPPORTED
     assert fwd(q=buf + 8) == ALIGN and fwd(k=None) == ALIGN and fwd(out=buf + 2) == ALIGN
     assert fwd(dtype=3) == ARG and fwd(cap=-1.0) == ARG and fwd(cap=float("nan")) == ARG and fwd(scale=float("nan")) == ARG
+    assert fwd(dtype=2, cap=4097.0) == UNSUPPORTED and fwd(dtype=2, cap=1e-38) == ARG and fwd(with_(1, 1 << 21), splits=1) == UNSUPPORTED
     assert fwd(docs=(buf, None)) == ARG and fwd(docs=(buf, buf)) == ARG                      # (no workspace for the ranges)
     assert fwd(prefix=buf) == ARG and fwd(splits=-1) == ARG and fwd(splits=2) == ARG and fwd(splits=1, lse=buf) == ARG and fwd(splits=1, rest=buf) == ARG and fwd(rest=buf + 8) == ARG
     shape5 = (ctypes.c_long * 21)(*(good + [128, 32, 16]))
@@ -337,3 +340,67 @@ def test_other_stream_and_captured(device):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(a, ops.attention(q, k, v, docs=docs)) and torch.equal(b, ops.attention(one, k, v, causal=True))
+
+
+@gpu
+@pytest.mark.parametrize("t, cap", [("fp16", 4096.0), ("bf16", 4096.0), ("fp32", 1e6), ("fp32", 1e-3), ("bf16", 1e-3)])
+def test_largest_and_smallest_caps(device, t, cap):
+    """A cap far above every score changes none of them (16-bit types: by cap 2^-22 = 2^-10 of a power of two at most, an eighth of a bf16 rounding and
+    half of an fp16 one of each probability); one far below leaves their signs."""
+    from craft_amd import ops
+    q, k, v, _ = make(t, 1, 70, 70, 2, 2, 32)
+    a, b = ops.attention(q, k, v, cap=cap).double().cpu(), attention64(q, k, v, cap=cap)[0][0]
+    eps = {"fp16": 2.0 ** -11, "bf16": 2.0 ** -8, "fp32": 2.0 ** -21}[t]
+    # the probabilities are off by their rounding and twice the scores' error (their own and the sum's), the result by that of sum p |v|, and rounded once
+    size = attention64(q, k, v.abs(), cap=cap)[0][0]
+    score = 2.0 ** -10 if t != "fp32" else 2.0 ** -19          # fp32: products of 32 terms of unit size times 3, and two roundings of scores up to 30
+    assert ((a - b).abs() <= (2 * eps + 2 * score) * size + 2.0 ** -25).all()
+
+
+@gpu
+def test_out_in_place_of_q_and_refused(device):
+    from craft_amd import ops
+    from craft_amd.hip import CraftHipError
+    for nq in (150, 1):                                        # (blocks of queries, and single tokens whose keys are split)
+        q, k, v, _ = make("bf16", 2, nq, 700, 4, 2, 64)
+        want = ops.attention(q, k, v, causal=True)
+        assert ops.attention(q, k, v, causal=True, out=q) is q and torch.equal(q, want)
+    q, k, v, _ = make("bf16", 1, 40, 40, 2, 2, 64)
+    for out in (k, v, torch.empty(1, 40, 1, 64, device="cuda", dtype=q.dtype).expand(1, 40, 2, 64)):
+        with pytest.raises(CraftHipError, match="out must"):
+            ops.attention(q, k, v, out=out)
+
+
+@gpu
+def test_without_gradients_is_the_serving_form(device):
+    """autograd.attention and layer_norm under no_grad give the bits of ops'."""
+    from craft_amd import autograd, ops
+    q, k, v, _ = make("bf16", 2, 1, 500, 4, 2, 64)
+    with torch.no_grad():
+        assert torch.equal(autograd.attention(q, k, v, causal=True), ops.attention(q, k, v, causal=True))
+        x = torch.randn(5, 70, device="cuda")
+        assert torch.equal(autograd.layer_norm(x), ops.layer_norm(x))
+
+
+@gpu
+def test_two_streams_at_once(device):
+    """Calls that run beside each other share nothing: each has its own workspace."""
+    from craft_amd import autograd
+    a, b = (make("bf16", 1, 300, 300, 4, 2, 64, seed=s) for s in (1, 2))
+    docs = doc_ids(1, 300, 3, 9)
+
+    def run(x):
+        leaves = [y.clone().requires_grad_() for y in x[:3]]
+        o = autograd.attention(*leaves, causal=True, cap=20.0, docs=docs)
+        return [o, *torch.autograd.grad(o, leaves, x[3])]
+    want = [run(a), run(b)]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    torch.cuda.synchronize()
+    for _ in range(4):
+        got = []
+        for s, x in zip(streams, (a, b)):
+            with torch.cuda.stream(s):
+                got.append(run(x))
+        torch.cuda.synchronize()
+        for w, g in zip(want, got):
+            assert all(torch.equal(m, n) for m, n in zip(w, g))

@@ -203,3 +203,28 @@ def test_same_bits_and_captured(device):
         torch.cuda.synchronize()
         y2, mean2, rstd2 = ops._layer_norm(x, w, b, 1e-5, None, True)
         assert torch.equal(y, y2) and all(torch.equal(p, q) for p, q in zip(grads, ops.layer_norm_bwd(x, w, b.dtype, a, mean2, rstd2)))
+
+
+@pytest.mark.parametrize("change, says", [
+    (dict(dy=torch.zeros(3, 4)), "dy"), (dict(dy=torch.zeros(2, 5)), "dy"), (dict(mean=torch.zeros(1)), "mean and rstd"),
+    (dict(rstd=torch.zeros(2).double()), "mean and rstd"), (dict(mean=torch.zeros(4)[::2]), "mean and rstd"), (dict(weight=torch.zeros(3)), "weight must"),
+    (dict(bias_type=torch.float16), "dy"), (dict(), "device tensors")])
+def test_backward_refusals(change, says):
+    from craft_amd import ops
+    from craft_amd.hip import CraftHipError
+    args = dict(x=torch.zeros(2, 4), weight=None, bias_type=None, dy=torch.zeros(2, 4), mean=torch.zeros(2), rstd=torch.zeros(2))
+    args.update(change)
+    with pytest.raises(CraftHipError, match=says):
+        ops.layer_norm_bwd(**args)
+
+
+@gpu
+@pytest.mark.parametrize("rows, C", [(5, 7), (70, 46), (300, 257), (17, 1027), (600, 4100)])
+def test_in_place(device, rows, C):
+    from craft_amd import ops
+    x = torch.randn(rows, C, generator=torch.Generator().manual_seed(1)).bfloat16().cuda()
+    want = ops.layer_norm(x)
+    assert ops.layer_norm(x, out=x) is x and torch.equal(x, want)
+    # rows that are one row in memory
+    one = x[:1].expand(rows, C)
+    assert torch.equal(ops.layer_norm(one), ops.layer_norm(one.contiguous()))

@@ -295,3 +295,17 @@ def test_trainer_with_muon(device):
     sd = opt.state_dict()
     opt.load_state_dict(sd)
     assert len(sd["state"]) == len(opt.params) - len(opt.unused_index)
+
+
+def test_results_in_one_place_are_refused():
+    from craft_amd import ops
+    from craft_amd.hip import CraftHipError
+    a, b = torch.zeros(4, 4), torch.zeros(4, 4)
+    with pytest.raises(CraftHipError, match="two results"):
+        ops.orthogonalize([a, b], out=[a, a])
+    with pytest.raises(CraftHipError, match="two results"):
+        ops.orthogonalize([a, a], out=[a, a])
+    with pytest.raises(CraftHipError, match="another matrix"):
+        ops.orthogonalize([a, b], out=[b, a])
+    with pytest.raises(CraftHipError, match="device tensors"):             # (the same matrix twice, results of their own: fine)
+        ops.orthogonalize([a, a])
