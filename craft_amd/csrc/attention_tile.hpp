@@ -13,10 +13,26 @@
 // the transposing reads (ds_read_b64_tr_b16) of a tile are free of bank conflicts.  They are filled by LDS-DMA: the copy writes LDS linearly, so the
 // swizzle is applied to the global addresses of the lanes.
 #pragma once
+#include <atomic>
 #include <type_traits>
 #include "launch.hpp"
 
 namespace craft {
+
+// Dynamic LDS above 64 KB has to be allowed once per kernel and device (hipFuncSetAttribute takes as long as a launch).  The flags only remember that it
+// was done: any thread may set them again.
+template <auto Kernel>
+inline int allow_lds(int bytes) {
+  static std::atomic<unsigned> done{0};
+  int dev = 0;
+  if (const hipError_t e = hipGetDevice(&dev)) return (int)e;
+  if (dev < 32 && (done.load(std::memory_order_relaxed) >> dev & 1)) return 0;
+  if (const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes)) return (int)e;
+  if (dev < 32) done.fetch_or(1u << dev, std::memory_order_relaxed);
+  return 0;
+}
+
+template <auto Kernel> struct KernelTag { static constexpr auto value = Kernel; };
 
 #define CRAFT_LDS __attribute__((address_space(3)))
 typedef __fp16 at_fp16x4 __attribute__((__vector_size__(4 * sizeof(__fp16))));

@@ -1,7 +1,6 @@
 // Host-visible parameter blocks and launcher prototypes shared by the .hip translation units and the
 // C-ABI layer (craft_hip.hip).  Nothing here is part of the public ABI (see include/craft_hip.h).
 #pragma once
-#include <atomic>
 #include "common.hpp"
 #include "gemm_engine.hpp"
 
@@ -11,21 +10,6 @@
 #define CRAFT_ERR_UNSUPPORTED 10003
 
 namespace craft {
-
-// Dynamic LDS above 64 KB has to be allowed once per kernel and device (hipFuncSetAttribute takes as long as a launch).  The flags only remember that it
-// was done: any thread may set them again.
-template <auto Kernel>
-inline int allow_lds(int bytes) {
-  static std::atomic<unsigned> done{0};
-  int dev = 0;
-  if (const hipError_t e = hipGetDevice(&dev)) return (int)e;
-  if (dev < 32 && (done.load(std::memory_order_relaxed) >> dev & 1)) return 0;
-  if (const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(Kernel), hipFuncAttributeMaxDynamicSharedMemorySize, bytes)) return (int)e;
-  if (dev < 32) done.fetch_or(1u << dev, std::memory_order_relaxed);
-  return 0;
-}
-
-template <auto Kernel> struct KernelTag { static constexpr auto value = Kernel; };
 
 // Developer A/B overrides from the environment, read ONCE when the library is loaded (never in a launch path):
 // CRAFT_HALO_BN (64 | 128), CRAFT_NO_C64, CRAFT_WF_DYNAMIC_TAPS.  Everything a caller may legitimately vary per call is an
