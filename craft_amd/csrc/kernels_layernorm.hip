@@ -7,6 +7,9 @@
 // The weight's and the bias' gradients are summed on the way: a thread owns the same columns of every row it meets, so its sums stay in registers over the
 // block's whole share of the rows; the row groups of a block are joined in LDS, the blocks by k_layer_norm_sum -- each in a fixed order, no atomics.
 // Vectors are 16 bytes at any alignment (unaligned loads and stores are native): an odd width moves its last vector back (LnCols).
+//
+// 16384 rows of 4096 bf16: forward 52 us (5.2 TB/s), backward 81 us (5.0 TB/s), the sum over the blocks 4 us; a copy of 256 MiB moves 5.5 TB/s, one of
+// 2 GiB 4.9.  28672 rows of 256 fp32: 12 us (4.8 TB/s).  1441 rows of 1027 fp16: 6 + 11 + 4 us, latency.
 #include <type_traits>
 #include "launch.hpp"
 #include "../../include/craft_hip.h"

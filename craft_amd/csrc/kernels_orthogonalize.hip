@@ -4,15 +4,20 @@
 //   steps times:  A = X X^T,   B = b A + c A^2,   X <- a X + B X
 //
 // Each step is three products whose sizes differ from matrix to matrix, and each needs the one before it: three launches a step for the WHOLE list, a
-// block per output tile of any matrix.  A and A^2 are symmetric: only their lower
-// tiles are computed, and written twice.
+// block per output tile of any matrix.  A and A^2 are symmetric: only their lower tiles are computed, and written twice.
 //
 // Arithmetic: fp32-class.  Every operand is two fp16 planes hi + lo of its value times a power of two (22 bits and more: the scales bring the largest
 // possible entry, which the spectrum bounds, just below fp16's largest number, so that lo keeps its bits), every product three MFMAs with fp32 sums.  The
 // planes take the four bytes of an fp32 value.  The norm is summed in fp64: its error would scale the whole result.
 //
 // All operands are read along their rows: X (rows of n) for X X^T, A for A^2, and B with X^T (rows of m) for B X; the last product's epilogue writes both X
-// and X^T.  X^T is kept twice (blocks of one strip read it whole while others write).  Rows and columns are padded to 64 (128) with zeros, which the products keep.
+// and X^T.  X^T is kept twice (blocks of one strip read it whole while others write).
+//
+// One 2048 x 8192 matrix: 1.86 ms, of which B X five times 202 us (three fp16 products: 1.02 PF/s, 73 % of a large library product's 1.39), X X^T 114 us
+// and 14 us for the sum of its shares, B 34 + 18 us.  The 53 matrices of the CRAFT model (64 x 147 .. 1024 x 256): 310 us in 18 launches, bound by each launch's
+// own latency (its operations are 33 us): X X^T 22 us, B 7 us, B X 26 us a step.  One 256 x 256: 106 us, 18 launches of 4 .. 8 us.
+//
+// Rows and columns are padded to 64 (128) with zeros, which the products keep.
 #include "attention_tile.hpp"
 #include "../../include/craft_hip.h"
 

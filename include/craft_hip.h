@@ -669,6 +669,7 @@ int craft_layer_norm_bwd(const void* x, long ldx, const void* dy, long lddy, con
  *   cap 0: no cap;  slopes: [H] fp32, NULL: no bias.
  * shape: 18 host longs B, Nq, Nk, H, Hk, D, then the (batch, token, head) strides in elements of q, k, v, out.  H % Hk == 0 (query head h reads key head
  * h / (H / Hk)), D % 8 == 0, D <= 128, strides multiples of 16 bytes, pointers 16-byte aligned, the last axis contiguous.
+ * cap: 0 (none) or positive, at most 4096 for 16-bit types, |scale| / cap at most 1e30.
  * splits 0: blocks of 128 queries.  For the backward pass they leave the log2-sums in lse ([B][H][Nq]; fp32: [B][H][Nq][2] with their rounding's rest; +inf
  * where nothing is seen) and, 16-bit types, the rest of out's rounding in out_rest (contiguous [B][Nq][H][D], 16-byte aligned); either may be NULL.
  * splits >= 1: for a few rows (Nq * H / Hk up to about 64): the keys split over so many blocks; no lse, no out_rest.
