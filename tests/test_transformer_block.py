@@ -118,3 +118,16 @@ def test_tokens_one_by_one(device):
             one = ops.attention(a, cache[0][:, :n + 1], cache[1][:, :n + 1], cap=5.0, slopes=slopes, causal=True)
             # fp32 on both sides: projections of one row and of many differ by their sums' order, 96 roundings of unit values
             assert (one - whole[:, n:n + 1]).abs().max() < 2e-5, n
+
+
+@gpu
+def test_the_documented_calls_run(device):
+    """The documented example (the integration guide's last section) as it stands: its single token gives its row of the whole attention."""
+    import os
+    import re
+    text = open(os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "INTEGRATION.md")).read()
+    ns = {}
+    exec(re.search(r"```python\n(.*?)```", text[text.index("## 4."):], flags=re.S).group(1), ns)      # noqa: S102 -- our own document
+    # fp32 on both sides, sums of at most 100 unit values in another order
+    assert (ns["one"] - ns["o"].detach()[:, 89:90]).abs().max() < 2e-5
+    assert torch.isfinite(ns["proj"].weight).all()
