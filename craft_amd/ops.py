@@ -877,12 +877,16 @@ def orthogonalize(mats: Sequence[torch.Tensor], steps: int = 5, coeffs=NEWTON_SC
 # ------------------------------------------------------------------------------------------------
 # attention with a cap, a distance bias and causal / prefix / document masks
 # ------------------------------------------------------------------------------------------------
-def _strided(t: torch.Tensor) -> torch.Tensor:
-    """t itself where the kernels can read it in place: contiguous head width, 16-byte steps, rows less than 16 MiB apart; else a copy."""
+def _in_place(t: torch.Tensor) -> bool:
+    """The kernels can read t where it lies: contiguous head width, 16-byte steps from a 16-byte address, rows less than 16 MiB apart."""
     step = 16 // t.element_size()
-    ok = (t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or (s >= 0 and s % step == 0) for n, s in zip(t.shape[:3], t.stride()))
-          and (t.shape[1] == 1 or t.stride(1) * t.element_size() < 1 << 24))
-    return t if ok else t.contiguous()
+    return (t.stride(3) == 1 and t.data_ptr() % 16 == 0 and all(n == 1 or (s >= 0 and s % step == 0) for n, s in zip(t.shape[:3], t.stride()))
+            and (t.shape[1] == 1 or t.stride(1) * t.element_size() < 1 << 24))
+
+
+def _strided(t: torch.Tensor) -> torch.Tensor:
+    """t itself where the kernels can read it in place, else a copy (a contiguous tensor at an odd address too, which ``contiguous()`` would hand back)."""
+    return t if _in_place(t) else t.clone(memory_format=torch.contiguous_format)
 
 
 def _strides(t: torch.Tensor):
@@ -1007,7 +1011,7 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optio
         plan = AttentionPlan(q, k, v, scale, cap, slopes, causal, prefix, docs, docs_k)
         if out is None:
             out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        elif (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or _strided(out) is not out
+        elif (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not _in_place(out)
               or any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride()))):
             raise hip.CraftHipError("attention: out must be of q's shape, type and device, with 16-byte aligned rows")
         elif out.numel() and out.data_ptr() in (k.data_ptr(), v.data_ptr()):

@@ -404,3 +404,40 @@ def test_two_streams_at_once(device):
         torch.cuda.synchronize()
         for w, g in zip(want, got):
             assert all(torch.equal(m, n) for m, n in zip(w, g))
+
+
+def offset(x, by=1):
+    """x's values, contiguous, at an address that no 16-byte load fits."""
+    flat = torch.empty(x.numel() + by, device=x.device, dtype=x.dtype)
+    t = flat[by:].view(x.shape)
+    t.copy_(x)
+    return t
+
+
+@pytest.mark.parametrize("t", list(TYPES))
+def test_contiguous_but_misaligned_is_copied(t):
+    """A slice of a flat buffer is contiguous wherever it starts: contiguous() hands it back as it is."""
+    from craft_amd import ops
+    x = make(t, 2, 5, 5, 2, 2, 16, device="cpu")[0]
+    y = offset(x)
+    assert y.is_contiguous() and y.data_ptr() % 16
+    z = ops._strided(y)
+    assert z.data_ptr() % 16 == 0 and torch.equal(z, x)
+    a = offset(x, 16)                                                      # (32 or 64 bytes on: nothing to copy)
+    assert ops._strided(a) is a
+
+
+@gpu
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("nq", [1, 50])
+def test_misaligned_inputs_and_gradients(device, t, nq):
+    from craft_amd import autograd, ops
+    from craft_amd.hip import CraftHipError
+    q, k, v, go = make(t, 2, nq, 50, 4, 2, 40)
+    res, tol = attention64(q, k, v, go, causal=True)
+    q, k, v = (offset(x).requires_grad_() for x in (q, k, v))
+    o = autograd.attention(q, k, v, causal=True)
+    check([o, *torch.autograd.grad(o, (q, k, v), offset(go))], res, tol)
+    check([ops.attention(q, k, v, causal=True)], res[:1], tol[:1])
+    with pytest.raises(CraftHipError, match="out must"):
+        ops.attention(q, k, v, out=offset(go))
