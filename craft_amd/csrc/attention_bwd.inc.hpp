@@ -434,6 +434,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP == 32 ? 2 : 1)) void k_a
     head = headn;
     buf ^= 1;
   }
+  if constexpr (S::VL) wait_copies();                     // (where no tile was walked nothing else has waited for V's copy)
   if (jw + (lane & 31) < p.Nk) {
     typedef T t4 __attribute__((ext_vector_type(4)));
     const long row = (((long)b * p.Nk + key) * heads + hx) * p.D;

@@ -441,3 +441,48 @@ def test_misaligned_inputs_and_gradients(device, t, nq):
     check([ops.attention(q, k, v, causal=True)], res[:1], tol[:1])
     with pytest.raises(CraftHipError, match="out must"):
         ops.attention(q, k, v, out=offset(go))
+
+
+WIDTHS = [32, 72, 128]                                                     # (64 is every other test's; 72 and 128: V in LDS, 32-row tiles, columns behind D)
+
+
+@gpu
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("D", WIDTHS)
+@pytest.mark.parametrize("causal", [False, True])
+def test_documents_at_every_width(device, t, D, causal):
+    """Whole 128-key blocks of padding, which no query tile meets, among them."""
+    both(t, 2, 650, 650, 4, 2, D, causal=causal, docs=doc_ids(2, 650, 5, 270), cap=8.0 if causal else 0.0, slopes=None if causal else slopes_of(4))
+    both(t, 1, 300, 300, 2, 2, D, causal=causal, docs=doc_ids(1, 300, 60, 1))
+
+
+@gpu
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("D", WIDTHS)
+def test_prefix_at_every_width(device, t, D):
+    for nq, nk, prefix in ((300, 300, [130, 0]), (140, 20, [3, 0]), (70, 400, [1, 395])):
+        both(t, 2, nq, nk, 4, 2, D, causal=True, prefix=torch.tensor(prefix, dtype=torch.int32, device="cuda"))
+
+
+@gpu
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("D", WIDTHS)
+def test_padding_may_hold_anything_at_every_width(device, t, D):
+    """As test_padding_may_hold_anything, with padding in front, in the middle and over whole tiles and blocks, queries and keys apart."""
+    from craft_amd import autograd, ops
+    nq, nk = 330, 410
+    q, k, v, go = make(t, 2, nq, nk, 4, 2, D)
+    dq, dk = doc_ids(2, nq, 3, 140), doc_ids(2, nk, 3, 150)
+    dq[1], dk[1] = dq[1].roll(37), dk[1].roll(70)
+    dq[0, 50:53], dk[0, 20:90] = -7, -2147483648
+    res, tol = attention64(q, k, v, go, docs=dq, docs_k=dk, causal=True)
+    bad = torch.tensor([math.nan, math.inf, -math.inf], device="cuda").to(q.dtype)
+    for x, d in ((q, dq), (go, dq), (k, dk), (v, dk)):
+        m = (d < 0)[:, :, None, None].expand(x.shape)
+        x[m] = bad[torch.arange(int(m.sum()), device="cuda") % 3]
+    q, k, v = (x.requires_grad_() for x in (q, k, v))
+    o = autograd.attention(q, k, v, docs=dq, docs_k=dk, causal=True)
+    grads = torch.autograd.grad(o, (q, k, v), go)
+    check([o, *grads], res, tol)
+    check([ops.attention(q, k, v, docs=dq, docs_k=dk, causal=True)], res[:1], tol[:1])
+    assert not grads[0][dq < 0].any() and not grads[1][dk < 0].any() and not grads[2][dk < 0].any() and not o[dq < 0].any()
