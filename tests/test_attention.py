@@ -486,3 +486,27 @@ def test_padding_may_hold_anything_at_every_width(device, t, D):
     check([o, *grads], res, tol)
     check([ops.attention(q, k, v, docs=dq, docs_k=dk, causal=True)], res[:1], tol[:1])
     assert not grads[0][dq < 0].any() and not grads[1][dk < 0].any() and not grads[2][dk < 0].any() and not o[dq < 0].any()
+
+
+@gpu
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("B, nq, nk, H, Hk, D, how", [
+    (64, 100, 100, 16, 8, 64, {}), (43, 150, 260, 12, 4, 128, dict(causal=True, cap=6.0, slopes=True)), (43, 150, 260, 12, 4, 40, dict(docs=True)),
+    (43, 70, 260, 8, 4, 128, dict(docs=True, causal=True, slopes=True)), (86, 40, 330, 6, 2, 24, dict(causal=True, prefix=True, slopes=True))])
+def test_one_block_for_a_group_of_heads(device, t, B, nq, nk, H, Hk, D, how):
+    """Batches that fill the card with one block for each key head: it walks over the query heads of its group, each with its slope and log-sums."""
+    from craft_amd import autograd
+    assert B * Hk * ((nk + 127) // 128) >= 512 and H > Hk
+    how = dict(how)
+    if how.get("slopes"):
+        how["slopes"] = slopes_of(H)
+    if how.get("prefix"):
+        how["prefix"] = torch.arange(B, dtype=torch.int32, device="cuda") * 4
+    if how.pop("docs", False):
+        d = doc_ids(B, nk, 5, 130)
+        how.update(docs=d[:, :nq].contiguous(), docs_k=d)
+    q, k, v, go = make(t, B, nq, nk, H, Hk, D)
+    res, tol = attention64(q, k, v, go, **how)
+    q, k, v = (x.requires_grad_() for x in (q, k, v))
+    o = autograd.attention(q, k, v, **how)
+    check([o, *torch.autograd.grad(o, (q, k, v), go)], res, tol)

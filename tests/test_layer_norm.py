@@ -228,3 +228,60 @@ def test_in_place(device, rows, C):
     # rows that are one row in memory
     one = x[:1].expand(rows, C)
     assert torch.equal(ops.layer_norm(one), ops.layer_norm(one.contiguous()))
+
+
+def norm64_deep(x, w, b, dy, eps=1e-5):
+    """norm64 with the depth of the kernels' sums in place of their length, so that one lost row shows.  A row: at most 4 vectors of 8 values in a thread, 6 steps
+    over a wave, 16 waves: 54 roundings, 64 here.  A weight's gradient: the rows of a group, the groups of a block (a row has 16, 64, 128, ... 1024 threads of its
+    1024: the fewest that hold its 16-byte vectors), 16 + 16 blocks."""
+    e, C, R = 2.0 ** -24, x.shape[-1], x.shape[0]
+    vectors = -(-C * x.element_size() // 16)
+    groups = 1024 // next((n for n in (16, 64, 128, 256, 512) if vectors <= n), 1024)
+    row, col = 64, -(-R // (256 * groups)) + groups + 32
+    xd, dyd, wd, bd = (v.detach().cpu().double() for v in (x, dy, w, b))
+    xd = xd.requires_grad_()
+    wl, bl = wd.clone().requires_grad_(), bd.clone().requires_grad_()
+    y = torch.nn.functional.layer_norm(xd, (C,), wl, bl, eps)
+    dx, dw, db = torch.autograd.grad(y, (xd, wl, bl), dyd)
+    y, xd = y.detach(), xd.detach()
+    mean = xd.mean(-1, keepdim=True)
+    rstd = ((xd - mean).square().mean(-1, keepdim=True) + eps).rsqrt()
+    xn = (xd - mean) * rstd
+    em = row * e * xd.abs().mean(-1, keepdim=True)
+    en = rstd * (em + e * xd.abs()) + xn.abs() * (row * e + rstd ** 2 * em ** 2)
+    u = lambda v: torch.finfo(v.dtype).eps / 2                             # noqa: E731
+    ty = wd.abs() * en + u(x) * y.abs() + 4 * e * (y.abs() + bd.abs())
+    g = dyd * wd
+    m0, m1 = g.mean(-1, keepdim=True), (g * xn).mean(-1, keepdim=True)
+    e0 = row * e * g.abs().mean(-1, keepdim=True)
+    e1 = row * e * (g * xn).abs().mean(-1, keepdim=True) + (g.abs() * en).mean(-1, keepdim=True)
+    tx = rstd * (e0 + xn.abs() * e1 + en * m1.abs() + 8 * e * (g.abs() + m0.abs() + (xn * m1).abs())) + dx.abs() * row * e + u(x) * dx.abs()
+    tw = (dyd.abs() * en).sum(0) + col * e * (dyd * xn).abs().sum(0) + u(w) * dw.abs()
+    tb = col * e * dyd.abs().sum(0) + u(b) * db.abs()
+    return (y, dx, dw, db), (ty, tx, tw, tb), dyd * xn
+
+
+# rows so many that every group of threads meets at least three (256 blocks of 1024 / TPR groups), and an odd number of them
+MANY = [(50021, 24), (13001, 257), (13001, 136), (6501, 520), (3333, 1027), (1701, 2056), (901, 4100), (901, 8192), (781, 16384)]
+
+
+@pytest.mark.parametrize("rows, C", [(50021, 24), (901, 4100)])
+def test_many_rows_bound_shows_a_lost_row(rows, C):
+    """The oracle's bounds on the weights' gradients are below what one row brings, in most columns."""
+    x, w, b, dy = make("bf16", rows, C, device="cpu")
+    _, tol, term = norm64_deep(x, w, b, dy)
+    assert (term[-1].abs() > tol[2]).double().mean() > 0.5 and (dy[-1].double().abs() > tol[3]).double().mean() > 0.5
+
+
+@gpu
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("rows, C", MANY)
+def test_many_rows(device, t, rows, C):
+    """The walk over rows: the next row's prefetch, the alternating buffers of its sums, the weights' gradients held over all of them."""
+    from craft_amd import autograd, ops
+    x, w, b, dy = make(t, rows, C)
+    want, tol, _ = norm64_deep(x, w, b, dy)
+    check([ops.layer_norm(x, w, b)], want, tol)
+    x, w, b = (v.requires_grad_() for v in (x, w, b))
+    y = autograd.layer_norm(x, w, b)
+    check([y, *torch.autograd.grad(y, (x, w, b), dy)], want, tol)
