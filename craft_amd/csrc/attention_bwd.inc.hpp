@@ -37,6 +37,60 @@ __global__ __launch_bounds__(256) void k_attention_delta(AttentionParams p, floa
   if ((threadIdx.x & 15) == 0) delta[(b * p.H + head) * p.Nq + i] = -s;
 }
 
+// The same for fp16, which also needs the largest norms for its powers of two (score_exponent): a block per (batch, key head, slice), whose
+// share of the queries of the head's group and of its keys it reads, 8 or 16 lanes to a row.  Padding's rows do not count.  All loads of a row stand in front of
+// its sums (one behind the other they took twice the time).
+template <typename T>
+__global__ __launch_bounds__(256) void k_attention_delta_scaled(AttentionParams p, float* delta) {
+  typedef typename AtFrag<T>::type frag_t;
+  __shared__ float2 red[32];
+  const int bk = blockIdx.x / p.slices, slice = blockIdx.x - bk * p.slices, b = bk / p.Hk, kvh = bk - b * p.Hk, G = p.H / p.Hk;
+  const int shift = p.D > 64 ? 4 : 3, groups = 256 >> shift, sub = threadIdx.x >> shift, c = 8 * (threadIdx.x & ((1 << shift) - 1));
+  const bool in = c < p.D;
+  const int i0 = (int)((long)p.Nq * slice / p.slices), j0 = (int)((long)p.Nk * slice / p.slices);
+  const long nq = ((long)p.Nq * (slice + 1) / p.slices - i0) * G, nk = (long)p.Nk * (slice + 1) / p.slices - j0;
+  float go2 = 0.f, v2 = 0.f;
+  for (long r = sub; r < max(nq, nk); r += groups) {                       // (whole groups of lanes)
+    const bool isq = r < nq, isk = r < nk;
+    const int i = i0 + (int)(r / G), head = kvh * G + (int)(r % G);
+    const long row = ((long)b * p.Nq + i) * p.H + head;
+    frag_t o, g, t, v;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) o[j] = g[j] = t[j] = v[j] = (T)0.f;
+    int dq = 0, dk = 0;
+    if (isq) {
+      if (in) {
+        o = *reinterpret_cast<const frag_t*>(reinterpret_cast<const T*>(p.o) + b * p.o_b + i * p.o_n + head * p.o_h + c);
+        g = *reinterpret_cast<const frag_t*>(reinterpret_cast<const T*>(p.go) + b * p.go_b + i * p.go_n + head * p.go_h + c);
+        if (p.o_rest) t = *reinterpret_cast<const frag_t*>(reinterpret_cast<const T*>(p.o_rest) + row * p.D + c);
+      }
+      if (p.docq) dq = p.docq[(long)b * p.Nq + i];
+    }
+    if (isk) {
+      if (in) v = *reinterpret_cast<const frag_t*>(reinterpret_cast<const T*>(p.v) + b * p.v_b + (j0 + r) * p.v_n + kvh * p.v_h + c);
+      if (p.dock) dk = p.dock[(long)b * p.Nk + j0 + r];
+    }
+    float s = 0.f, n = 0.f, m = 0.f;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      s += (float)o[j] * (float)g[j];
+      s += (float)t[j] * (float)g[j];
+      n += (float)g[j] * (float)g[j];
+      m += (float)v[j] * (float)v[j];
+    }
+    for (int k = 1 << (shift - 1); k > 0; k >>= 1) { s += __shfl_xor(s, k); n += __shfl_xor(n, k); m += __shfl_xor(m, k); }
+    if (isq && c == 0) delta[((long)b * p.H + head) * p.Nq + i] = -s;
+    if (n < INFINITY && dq >= 0) go2 = fmaxf(go2, n);
+    if (m < INFINITY && dk >= 0) v2 = fmaxf(v2, m);
+  }
+  if (c == 0) red[sub] = make_float2(go2, v2);
+  __syncthreads();
+  if (threadIdx.x == 0) {
+    for (int k = 1; k < groups; ++k) { go2 = fmaxf(go2, red[k].x); v2 = fmaxf(v2, red[k].y); }
+    p.top[(long)bk * p.slices + slice] = make_float2(go2, v2);
+  }
+}
+
 template <typename T, int DP> struct BwdShape {
   static constexpr int TR = sizeof(T) == 2 && DP < 128 ? 64 : 32;         // rows of a tile (128 columns in 64-row tiles: registers spill)
   static constexpr int TILE = TR * DP * (int)sizeof(T);
@@ -85,6 +139,18 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP < 128 ? 2 : 1)) void k_a
   load_own<T, DP>(reinterpret_cast<const T*>(p.go) + b * p.go_b + (long)i * p.go_n + head * p.go_h, p.D, h, gf);
   const float* lp = p.lse + ((long)bh * p.Nq + i) * at_lw<T>();
   float row[3] = {lp[0], p.delta[(long)bh * p.Nq + i], at_lw<T>() == 2 ? lp[1] : 0.f};
+  int ex = 0;
+  if constexpr (std::is_same<T, _Float16>::value) {
+    const float v2 = largest_rows(p, b * p.Hk + kvh, lane).y;
+    float n = 0.f;
+#pragma unroll
+    for (int ks = 0; ks < DP / 16; ++ks)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) n += (float)gf[ks][j] * (float)gf[ks][j];
+    n += at_other_half(n);
+    ex = score_exponent(n < INFINITY ? n : 0.f, v2);
+    row[0] -= (float)ex;
+  }
   arrived(qf);
   arrived(gf);
   arrived(row);
@@ -213,6 +279,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP < 128 ? 2 : 1)) void k_a
   }
   if (i0 + wave * 32 + (lane & 31) < p.Nq) {
     T* row = reinterpret_cast<T*>(p.dq) + (((long)b * p.Nq + i) * p.H + head) * p.D;
+    const float scale = __builtin_ldexpf(p.scale, -ex);
     typedef T t4 __attribute__((ext_vector_type(4)));
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
@@ -222,7 +289,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP < 128 ? 2 : 1)) void k_a
         if (c < p.D) {
           t4 w;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) w[j] = (T)(dq[d][4 * g + j] * p.scale);
+          for (int j = 0; j < 4; ++j) w[j] = (T)(dq[d][4 * g + j] * scale);
           *reinterpret_cast<t4*>(row + c) = w;
         }
       }
@@ -235,6 +302,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP == 32 ? 2 : 1)) void k_a
   typedef DkvShape<T, DP> S;
   typedef typename AtFrag<T>::type frag_t;
   constexpr int TQ = S::TR, NB = TQ / 32;
+  constexpr bool F16 = std::is_same<T, _Float16>::value;
   extern __shared__ __align__(512) unsigned char lds[];
   const unsigned lds0 = (unsigned)(size_t)(CRAFT_LDS unsigned char*)lds;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), h = lane >> 5;
@@ -253,6 +321,12 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP == 32 ? 2 : 1)) void k_a
 
   frag_t kf[DP / 16], vf[S::VL ? 1 : DP / 16];
   load_own<T, DP>(reinterpret_cast<const T*>(p.k) + b * p.k_b + (long)key * p.k_n + kvh * p.k_h, p.D, h, kf);
+  int ex = 0;                                   // fp16 (behind the keys' loads): probabilities times 2^15, gradients of scores times 2^ex
+  if constexpr (F16) {
+    const float2 top = largest_rows(p, b * p.Hk + kvh, lane);
+    ex = __builtin_amdgcn_readfirstlane(score_exponent(top.x, top.y));
+  }
+  const float xp = F16 ? 0x1p15f : 1.f, xs = F16 ? __builtin_ldexpf(1.f, ex) : 1.f;
   const int nchunk = p.D * (int)sizeof(T) / 16;
   const unsigned VTr = row_addr<T, DP>(lds0 + (unsigned)(S::V + wave * 32 * at_rowb<T, DP>()), lane);
   if constexpr (S::VL) {
@@ -420,7 +494,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP == 32 ? 2 : 1)) void k_a
         }
 #pragma unroll
         for (int s2 = 0; s2 < 2; ++s2) {
-          const frag_t pf = at_pack<T>(x, s2), sf = at_pack<T>(y, s2);
+          const frag_t pf = at_pack<T>(x, s2, xp), sf = at_pack<T>(y, s2, xs);
 #pragma unroll
           for (int d = 0; d < DP / 32; ++d) {
             at_mma(col_read<T, DP>(Qc, 32 * ib + 16 * s2, d, S::TILE), pf, dv[d]);
@@ -438,6 +512,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP == 32 ? 2 : 1)) void k_a
   if (jw + (lane & 31) < p.Nk) {
     typedef T t4 __attribute__((ext_vector_type(4)));
     const long row = (((long)b * p.Nk + key) * heads + hx) * p.D;
+    const float sk = __builtin_ldexpf(p.scale, -ex), sv = 1.f / xp;
 #pragma unroll
     for (int d = 0; d < DP / 32; ++d)
 #pragma unroll
@@ -447,13 +522,13 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP == 32 ? 2 : 1)) void k_a
         if (p.part_k) {
           f32x4 wk, wv;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) { wk[j] = dk[d][4 * g + j] * p.scale; wv[j] = dv[d][4 * g + j]; }
+          for (int j = 0; j < 4; ++j) { wk[j] = dk[d][4 * g + j] * sk; wv[j] = dv[d][4 * g + j] * sv; }
           *reinterpret_cast<f32x4*>(p.part_k + row + c) = wk;
           *reinterpret_cast<f32x4*>(p.part_v + row + c) = wv;
         } else {
           t4 wk, wv;
 #pragma unroll
-          for (int j = 0; j < 4; ++j) { wk[j] = (T)(dk[d][4 * g + j] * p.scale); wv[j] = (T)dv[d][4 * g + j]; }
+          for (int j = 0; j < 4; ++j) { wk[j] = (T)(dk[d][4 * g + j] * sk); wv[j] = (T)(dv[d][4 * g + j] * sv); }
           *reinterpret_cast<t4*>(reinterpret_cast<T*>(p.dk) + row + c) = wk;
           *reinterpret_cast<t4*>(reinterpret_cast<T*>(p.dv) + row + c) = wv;
         }
@@ -487,8 +562,12 @@ int attention_bwd_launch(const AttentionParams& p, hipStream_t s) {
   typedef BwdShape<T, DP> S;
   const long rows = (long)p.B * p.Nq * p.H;
   const long bq = (long)p.B * p.H * ((p.Nq + 127) / 128), bk = (long)p.B * (p.part_k ? p.H : p.Hk) * ((p.Nk + 127) / 128);
+  if ((long)p.B * p.Hk * p.slices > 0x7fffffffL) return CRAFT_ERR_UNSUPPORTED;
   if (bq > 0x7fffffffL || bk > 0x7fffffffL || (rows + 15) / 16 > 0x7fffffffL) return CRAFT_ERR_UNSUPPORTED;
-  hipLaunchKernelGGL(k_attention_delta<T>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, p, const_cast<float*>(p.delta));
+  if constexpr (std::is_same<T, _Float16>::value)
+    hipLaunchKernelGGL(k_attention_delta_scaled<T>, dim3((unsigned)(p.B * p.Hk * p.slices)), dim3(256), 0, s, p, const_cast<float*>(p.delta));
+  else
+    hipLaunchKernelGGL(k_attention_delta<T>, dim3((unsigned)((rows + 15) / 16)), dim3(256), 0, s, p, const_cast<float*>(p.delta));
   HIP_CHECK_RET(hipGetLastError());
   auto go = [&](auto tag, long blocks, int bytes) {
     constexpr auto kernel = decltype(tag)::value;

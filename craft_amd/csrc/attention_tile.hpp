@@ -60,7 +60,33 @@ struct AttentionParams {
   float *part_o, *part_ml;                     // token kernel: partial results of the splits
   int splits;
   float *part_k, *part_v;                      // backward: per query head partial key / value gradients (null: written directly)
+  float2* top;                                 // backward, fp16: [B * Hk][slices] the largest |go_i|^2 and |v_j|^2 (see score_exponent)
+  int slices;
 };
+
+// fp16's second products.  An operand in fp16 keeps its bits between 2^-14 and 2^16 only: the probabilities of a long row, and the gradients of scores
+// where the loss' own are small, would lose them or vanish; large gradients of scores would overflow though dq and dk fit.  Both are carried times a
+// power of two, which the fp32 results lose again: 2^15 for probabilities (at most 1), 2^E for gradients of scores, which are at most
+// |go_i| (|v_j| + |o_i|) <= 2 max|go| max|v| < 2^(15 - E).  The gradient of q has its own query's |go_i| and so its own E; those of k and v have one for a
+// key head (its query heads share the sums).  Norms that are not finite do not count: their rows give inf or NaN at any scale.
+// (|go| = 1e-4, 2048 tokens: dk was off by 2.7e-3 without, where rounding the result costs 3e-4.)
+__device__ __forceinline__ int score_exponent(float go2, float v2) {
+  const float b = 2.f * sqrtf(go2) * sqrtf(v2);
+  return 15 - __builtin_amdgcn_frexp_expf(b < INFINITY ? b : 1.f);
+}
+// largest of the slices, by a wave; four loads on their way at a time
+__device__ __forceinline__ float2 largest_rows(const AttentionParams& p, int bk, int lane) {
+  const float2* top = p.top + (long)bk * p.slices;
+  float2 m = make_float2(0.f, 0.f);
+  for (int i = lane; i - lane < p.slices; i += 256) {
+    float2 t[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) t[u] = top[min(i + 64 * u, p.slices - 1)];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) { m.x = fmaxf(m.x, t[u].x); m.y = fmaxf(m.y, t[u].y); }
+  }
+  return make_float2(wave_max(m.x), wave_max(m.y));
+}
 
 template <typename T> struct AtFrag { typedef f32x8 type; };
 template <> struct AtFrag<_Float16> { typedef f16x8 type; };
@@ -153,12 +179,23 @@ __device__ __forceinline__ typename AtFrag<T>::type col_read(unsigned addr, int 
 }
 
 // 8 accumulator values (registers 8 s .. 8 s + 7) as a B operand.  16-bit types: the probabilities (at most 2^8 before normalisation) and score
-// gradients are rounded to the tensors' type here, once, to nearest; their sums are taken in fp32 before the rounding.
+// gradients are rounded to the tensors' type here, once, to nearest; their sums are taken in fp32 before the rounding.  That is one product in place of two
+// or three (a value in two 16-bit planes), and it is what makes the results err more than fp32 products rounded once at the end: outputs 2.8e-4 against 2.1e-4
+// (fp16) and 2.0e-3 against 1.7e-3 (bf16), dq and dk 3.5e-4 against 2.1e-4 and 2.6e-3 against 1.7e-3.
 template <typename T>
 __device__ __forceinline__ typename AtFrag<T>::type at_pack(const f32x16& x, int s) {
   typename AtFrag<T>::type v;
 #pragma unroll
   for (int j = 0; j < 8; ++j) v[j] = (T)x[8 * s + j];
+  return v;
+}
+// times a power of two (fp16: the product and its conversion are one instruction)
+template <typename T>
+__device__ __forceinline__ typename AtFrag<T>::type at_pack(const f32x16& x, int s, float f) {
+  if constexpr (!std::is_same<T, _Float16>::value) return at_pack<T>(x, s);
+  typename AtFrag<T>::type v;
+#pragma unroll
+  for (int j = 0; j < 8; ++j) v[j] = (T)(x[8 * s + j] * f);
   return v;
 }
 

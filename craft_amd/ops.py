@@ -988,7 +988,7 @@ class AttentionPlan:
         dk, dv = torch.empty(2, B, Nk, Hk, D, device=self.device, dtype=self.q.dtype)
         # key / value gradients of shared heads: one block walks over the group's heads, unless that leaves compute units without a block
         split_group = int(H > Hk and B * Hk * ((Nk + 127) // 128) < 512)
-        nbytes = self.range_bytes() + (4 * B * H * Nq + 15) // 16 * 16 + split_group * 8 * B * Nk * H * D
+        nbytes = self.range_bytes() + (4 * B * H * Nq + 15) // 16 * 16 + (8192 * B * Hk if self.code == hip.PREC_F16 else 0) + split_group * 8 * B * Nk * H * D
         with _on(self.device):
             call("craft_attention_bwd", self.q, self.k, self.v, out, rest, lse, go, self.shape(out, go), *self.masks(), self.scale, self.cap, self.causal, self.code,
                  split_group, dq, dk, dv, self.new(nbytes), nbytes)

@@ -510,3 +510,109 @@ def test_one_block_for_a_group_of_heads(device, t, B, nq, nk, H, Hk, D, how):
     q, k, v = (x.requires_grad_() for x in (q, k, v))
     o = autograd.attention(q, k, v, **how)
     check([o, *torch.autograd.grad(o, (q, k, v), go)], res, tol)
+
+
+def unavoidable(exact, t):
+    """What rounding the exact result to the type costs, in the mean."""
+    return (exact.to(t).double() - exact).norm().item()
+
+
+@gpu
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("D, size", [(64, 1.0), (64, 1e-3), (64, 1e-5), (128, 1e-4), (72, 1e-5), (32, 3000.0), (128, 3000.0)])
+def test_gradients_of_every_size(device, t, D, size):
+    """Gradients keep their bits whatever the size of the loss', in 16 bits too.  The bounds are those of gradients of unit size times the size (a power of two
+    near it), and half of fp16's smallest step for the last rounding; and in the mean: a rounding is off by its half step u / sqrt 3 at the worst, by 0.43 u over
+    all mantissas, so operands rounded once (incoherent, every term by itself) and a result rounded once are off by sqrt(1 + (0.577 / 0.43)^2) = 1.7 times what
+    rounding the result alone costs (fp32: the elements' bounds alone; its operands are not rounded)."""
+    from craft_amd import autograd
+    q, k, v, go = make(t, 1, 700, 700, 4, 2, D)
+    s = 2.0 ** round(math.log2(size))
+    how = dict(causal=True, slopes=slopes_of(4)) if D == 64 else dict(cap=20.0) if D == 128 else {}
+    go = (go.double() * s).to(go.dtype)                                    # (1e-5 in fp16: below its smallest normal number, rounded once more)
+    res, tol = attention64(q, k, v, go.double() / s, **how)
+    res, tol = [res[0]] + [r * s for r in res[1:]], [tol[0]] + [e * s + 2.0 ** -25 * (t == "fp16") for e in tol[1:]]
+    assert max(r.abs().max() for r in res) < 6e4
+    q, k, v = (x.requires_grad_() for x in (q, k, v))
+    o = autograd.attention(q, k, v, **how)
+    got = [o, *torch.autograd.grad(o, (q, k, v), go)]
+    check(got, res, tol)
+    for g, r, name in zip(got[1:], res[1:], ("dq", "dk", "dv")):
+        off, least = (g.cpu().double() - r).norm().item(), unavoidable(r, TYPES[t])
+        assert t == "fp32" or off <= 2.0 * least, (name, off / least)
+
+
+def two_keys_each(D, n=200, device="cuda"):
+    """Every query looks at two keys whose values differ widely: gradients of scores past fp16's largest number, of everything else within it."""
+    _, k, v, go = make("fp16", 1, n, n, 1, 1, D, device=device)
+    scale = 6.0 / (4 * D)
+    q = (4 * (k.float() + k.float().roll(1, 1))).half()
+    return q, k, (v.float() * 24 * (64 / D) ** 0.5).half(), (go.float() * 1000).half(), scale
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_two_keys_each(D):
+    q, k, v, go, scale = two_keys_each(D, device="cpu")
+    res, _ = attention64(q, k, v, go, scale=scale)
+    p = torch.softmax(scale * q.double()[0, :, 0] @ k.double()[0, :, 0].T, -1)
+    dp = go.double()[0, :, 0] @ v.double()[0, :, 0].T
+    ds = p * (dp - (p * dp).sum(-1, keepdim=True))
+    assert ds.abs().max() > 2 * 65504 and max(r.abs().max() for r in res) < 6e4
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_score_gradients_past_the_largest_fp16(device, D):
+    from craft_amd import autograd
+    q, k, v, go, scale = two_keys_each(D)
+    res, tol = attention64(q, k, v, go, scale=scale)
+    q, k, v = (x.requires_grad_() for x in (q, k, v))
+    o = autograd.attention(q, k, v, scale=scale)
+    check([o, *torch.autograd.grad(o, (q, k, v), go)], res, tol)
+
+
+@gpu
+@pytest.mark.parametrize("D", [64, 128])
+def test_small_probabilities_keep_their_bits(device, D):
+    """Flat rows of 20000 keys: probabilities of 5e-5, below fp16's smallest normal number, and score gradients of 1e-8."""
+    from craft_amd import autograd
+    q, k, v, go = make("fp16", 1, 130, 20000, 1, 1, D, spread=0.05)
+    go = go * 1e-3
+    s = 2.0 ** -10
+    res, tol = attention64(q, k, v, go.double() / s)
+    res, tol = [res[0]] + [r * s for r in res[1:]], [tol[0]] + [e * s + 2.0 ** -25 for e in tol[1:]]
+    q, k, v = (x.requires_grad_() for x in (q, k, v))
+    o = autograd.attention(q, k, v)
+    got = [o, *torch.autograd.grad(o, (q, k, v), go)]
+    check(got, res, tol)
+    for g, r, name in zip(got[1:], res[1:], ("dq", "dk", "dv")):
+        off, least = (g.cpu().double() - r).norm().item(), unavoidable(r, torch.float16)
+        assert off <= 2.0 * least, (name, off / least)
+
+
+@gpu
+@pytest.mark.parametrize("t", list(TYPES))
+def test_infinite_gradients_show(device, t):
+    """An overflow of the loss reaches every gradient that depends on it, where a loss scale looks for it.  (Finite values are what the operator asks for:
+    nothing says where else it goes.)"""
+    from craft_amd import autograd
+    q, k, v, go = make(t, 1, 300, 300, 4, 2, 64)
+    for bad in (math.inf, math.nan):
+        go[0, 130, 1, 3] = bad
+        a = [x.clone().requires_grad_() for x in (q, k, v)]
+        dq, dk, dv = torch.autograd.grad(autograd.attention(*a), a, go)
+        assert not torch.isfinite(dq[0, 130, 1]).any() and not torch.isfinite(dk[0, :, 0]).any() and not torch.isfinite(dv[0, :, 0, 3]).any()
+        assert torch.isfinite(dq[0, :130]).all()
+
+
+def test_gradients_workspace_is_checked():
+    """fp16 asks for the room of its powers of two; the other types do not."""
+    import ctypes
+
+    from craft_amd import hip
+    lib, buf = hip.load(), 4096
+    shape = (ctypes.c_long * 21)(*([2, 5, 4, 6, 3, 16] + [128, 32, 16] * 5))
+    bwd = lambda dtype, n, group=0: lib.craft_attention_bwd(buf, buf, buf, buf, None, buf, buf, shape, None, None, None, None, 1.0, 0.0, 0, dtype, group, buf, buf, buf, buf, n, None)  # noqa: E731
+    row, part = 240, 2 * 2 * 4 * 6 * 16 * 4
+    assert bwd(2, row + 6 * 8192 - 1) == 10001 and bwd(2, row + 6 * 8192 + part - 1, 1) == 10001
+    assert bwd(1, row - 1) == 10001 and bwd(0, row + part - 1, 1) == 10001
