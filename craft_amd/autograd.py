@@ -1184,6 +1184,10 @@ def sequence_loss(flow_preds, flow_gt, valid, gamma: float = 0.8, max_flow: floa
 # ------------------------------------------------------------------------------------------------------------------
 # LayerNorm with weights; attention with a cap, a distance bias and causal / prefix / document masks
 # ------------------------------------------------------------------------------------------------------------------
+def _wants_gradient(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
 class LayerNorm(Function):
     """ops.layer_norm with its gradients; keeps x and the two row statistics."""
 
@@ -1203,7 +1207,7 @@ class LayerNorm(Function):
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:
     """Differentiable ``ops.layer_norm`` (gradients of x, weight and bias; the weight's and bias' sums over the rows in fp32, in a fixed order)."""
-    if not torch.is_grad_enabled():
+    if not _wants_gradient(x, weight, bias):
         return ops.layer_norm(x, weight, bias, eps)
     return LayerNorm.apply(x, weight, bias, eps)
 
@@ -1234,7 +1238,8 @@ class Attention(Function):
             return (torch.zeros_like(q), torch.zeros_like(k), torch.zeros_like(v), *none)
         scale, cap, causal = ctx.how
         with torch.no_grad():
-            return (*ops.AttentionPlan(q, k, v, scale, cap, slopes, causal, prefix, docs, docs_k).backward(out, lse, rest, go), *none)
+            plan = ops.AttentionPlan(q, k, v, scale, cap, slopes, causal, prefix, docs, docs_k)
+            return (*plan.backward(out, lse, rest, go, ctx.needs_input_grad[:3]), *none)
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optional[float] = None, cap: float = 0.0, slopes: Optional[torch.Tensor] = None,
@@ -1244,6 +1249,6 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optio
     the cap have none.  The scores are computed again in the backward pass; no N x N tensor is kept."""
     if slopes is not None and slopes.requires_grad:
         raise hip.CraftHipError("attention: slopes have no gradient here")
-    if not torch.is_grad_enabled():                                        # (a few query rows: the single-token kernel, which keeps no log-sums)
+    if not _wants_gradient(q, k, v):                                       # (a few query rows: the single-token kernel, which keeps no log-sums)
         return ops.attention(q, k, v, scale=scale, cap=cap, slopes=slopes, causal=causal, prefix=prefix, docs=docs, docs_k=docs_k)
     return Attention.apply(q, k, v, scale, cap, slopes, causal, prefix, docs, docs_k)

@@ -575,10 +575,12 @@ int attention_bwd_launch(const AttentionParams& p, hipStream_t s) {
     hipLaunchKernelGGL(kernel, dim3((unsigned)blocks), dim3(256), bytes, s, p);
     return (int)hipGetLastError();
   };
-  int rc;
-  if (p.cap > 0.f) rc = p.slopes ? go(KernelTag<k_attention_dkv<T, DP, true, true>>(), bk, DkvShape<T, DP>::LDS) : go(KernelTag<k_attention_dkv<T, DP, true, false>>(), bk, DkvShape<T, DP>::LDS);
-  else rc = p.slopes ? go(KernelTag<k_attention_dkv<T, DP, false, true>>(), bk, DkvShape<T, DP>::LDS) : go(KernelTag<k_attention_dkv<T, DP, false, false>>(), bk, DkvShape<T, DP>::LDS);
-  if (rc) return rc;
+  if (p.dk) {
+    int rc;
+    if (p.cap > 0.f) rc = p.slopes ? go(KernelTag<k_attention_dkv<T, DP, true, true>>(), bk, DkvShape<T, DP>::LDS) : go(KernelTag<k_attention_dkv<T, DP, true, false>>(), bk, DkvShape<T, DP>::LDS);
+    else rc = p.slopes ? go(KernelTag<k_attention_dkv<T, DP, false, true>>(), bk, DkvShape<T, DP>::LDS) : go(KernelTag<k_attention_dkv<T, DP, false, false>>(), bk, DkvShape<T, DP>::LDS);
+    if (rc) return rc;
+  }
   if (p.part_k) {
     const long n4 = (long)p.B * p.Nk * p.Hk * (p.D / 4);
     if ((n4 + 255) / 256 > 0x7fffffffL) return CRAFT_ERR_UNSUPPORTED;
@@ -586,6 +588,7 @@ int attention_bwd_launch(const AttentionParams& p, hipStream_t s) {
                        reinterpret_cast<T*>(p.dv), n4, p.H / p.Hk, p.D / 4);
     HIP_CHECK_RET(hipGetLastError());
   }
+  if (!p.dq) return 0;
   if (p.cap > 0.f) return p.slopes ? go(KernelTag<k_attention_dq<T, DP, true, true>>(), bq, S::LDS) : go(KernelTag<k_attention_dq<T, DP, true, false>>(), bq, S::LDS);
   return p.slopes ? go(KernelTag<k_attention_dq<T, DP, false, true>>(), bq, S::LDS) : go(KernelTag<k_attention_dq<T, DP, false, false>>(), bq, S::LDS);
 }

@@ -117,7 +117,9 @@ int craft_attention_bwd(const void* q, const void* k, const void* v, const void*
   AttentionParams p;
   const int rc = fill(p, shape, 5, slopes, prefix, doc_q, doc_k, scale, cap, causal, dtype);
   if (rc) return rc;
-  if (!aligned(q) || !aligned(k) || !aligned(v) || !aligned(out) || !aligned(grad_out) || !aligned(dq) || !aligned(dk) || !aligned(dv)) return CRAFT_ERR_ALIGN;
+  if (!aligned(q) || !aligned(k) || !aligned(v) || !aligned(out) || !aligned(grad_out)) return CRAFT_ERR_ALIGN;
+  if ((dq && !aligned(dq)) || (dk && !aligned(dk)) || (dv && !aligned(dv))) return CRAFT_ERR_ALIGN;
+  if ((dk == nullptr) != (dv == nullptr) || (split_group && !dk)) return CRAFT_ERR_ARG;
   if (!lse || (reinterpret_cast<uintptr_t>(out_rest) & 15)) return CRAFT_ERR_ARG;
   const long ranges = range_bytes(p), delta = ((long)p.B * p.H * p.Nq * 4 + 15) / 16 * 16, part = split_group ? (long)p.B * p.Nk * p.H * p.D * 4 : 0;
   // fp16: a key head's rows are cut into slices for the largest norms, 16 rows each, 1024 slices at most, which a wave reads 64 at a time
@@ -125,6 +127,7 @@ int craft_attention_bwd(const void* q, const void* k, const void* v, const void*
   const long rows = (long)p.Nq * (p.H / p.Hk) > p.Nk ? (long)p.Nq * (p.H / p.Hk) : p.Nk, slices = rows >= 16384 ? 1024 : (rows + 1023) / 1024 * 64;
   const long more = f16 ? 8192l * p.B * p.Hk : 0;
   if (!aligned(ws) || ws_bytes < ranges + delta + more + 2 * part) return CRAFT_ERR_ARG;
+  if (!dq && !dk) return 0;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);
   p.q = q; p.k = k; p.v = v; p.o = out; p.o_rest = out_rest; p.go = grad_out; p.lse = const_cast<float*>(lse); p.dq = dq; p.dk = dk; p.dv = dv;
   char* w = reinterpret_cast<char*>(ws) + ranges;

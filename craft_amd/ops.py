@@ -981,18 +981,19 @@ class AttentionPlan:
             return torch.empty(B, H, Nq, 2, device=self.device, dtype=torch.float32), None
         return torch.empty(B, H, Nq, device=self.device, dtype=torch.float32), torch.empty(B, Nq, H, D, device=self.device, dtype=self.q.dtype)
 
-    def backward(self, out: torch.Tensor, lse: torch.Tensor, rest: Optional[torch.Tensor], go: torch.Tensor):
+    def backward(self, out: torch.Tensor, lse: torch.Tensor, rest: Optional[torch.Tensor], go: torch.Tensor, need=(True, True, True)):
+        """(dq, dk, dv); ``need`` leaves dq out, or dk and dv (one kernel makes both) where neither is wanted."""
         B, Nq, Nk, H, Hk, D = self.dims
         go = _strided(go.to(self.q.dtype))
-        dq = torch.empty(B, Nq, H, D, device=self.device, dtype=self.q.dtype)
-        dk, dv = torch.empty(2, B, Nk, Hk, D, device=self.device, dtype=self.q.dtype)
+        dq = torch.empty(B, Nq, H, D, device=self.device, dtype=self.q.dtype) if need[0] else None
+        dk, dv = torch.empty(2, B, Nk, Hk, D, device=self.device, dtype=self.q.dtype) if need[1] or need[2] else (None, None)
         # key / value gradients of shared heads: one block walks over the group's heads, unless that leaves compute units without a block
-        split_group = int(H > Hk and B * Hk * ((Nk + 127) // 128) < 512)
+        split_group = int(dk is not None and H > Hk and B * Hk * ((Nk + 127) // 128) < 512)
         nbytes = self.range_bytes() + (4 * B * H * Nq + 15) // 16 * 16 + (8192 * B * Hk if self.code == hip.PREC_F16 else 0) + split_group * 8 * B * Nk * H * D
         with _on(self.device):
             call("craft_attention_bwd", self.q, self.k, self.v, out, rest, lse, go, self.shape(out, go), *self.masks(), self.scale, self.cap, self.causal, self.code,
                  split_group, dq, dk, dv, self.new(nbytes), nbytes)
-        return dq, dk, dv
+        return dq, dk if need[1] else None, dv if need[2] else None
 
 
 def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optional[float] = None, cap: float = 0.0, slopes: Optional[torch.Tensor] = None,

@@ -678,6 +678,7 @@ int craft_attention_fwd(const void* q, const void* k, const void* v, const long*
                         const int* doc_k, float scale, float cap, int causal, int dtype, int splits, void* out, float* lse, void* out_rest, void* ws,
                         long ws_bytes, void* stream);
 /* gradients of q [B][Nq][H][D], k and v [B][Nk][Hk][D], contiguous.  out_rest may be NULL (the gradients are then off by out's rounding too).  shape: 21 host longs, as above with the strides of grad_out last.
+ * dq may be NULL, and dk and dv together: what is not asked for is not computed.
  * split_group 1: a block per query head for the key / value gradients and a sum over the heads of a group behind it (more blocks, fp32 partial results).
  * ws (16-byte aligned): the documents' ranges as above, then B * H * Nq floats rounded up to 16 bytes, for CRAFT_PREC_F16 8192 * B * Hk bytes, then
  * with split_group 2 * B * Nk * H * D floats.

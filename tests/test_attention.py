@@ -616,3 +616,57 @@ def test_gradients_workspace_is_checked():
     row, part = 240, 2 * 2 * 4 * 6 * 16 * 4
     assert bwd(2, row + 6 * 8192 - 1) == 10001 and bwd(2, row + 6 * 8192 + part - 1, 1) == 10001
     assert bwd(1, row - 1) == 10001 and bwd(0, row + part - 1, 1) == 10001
+
+
+def calls_of(monkeypatch):
+    """The names and arguments of the package's calls into the library from here on."""
+    from craft_amd import ops
+    seen, call = [], ops.call
+    monkeypatch.setattr(ops, "call", lambda name, *a: (seen.append((name, a)), call(name, *a))[1])
+    return seen
+
+
+@pytest.mark.parametrize("training", [False, True])
+def test_inputs_without_gradients_take_the_serving_form(monkeypatch, training):
+    """Gradients enabled and nothing that needs one: what a server that forgets no_grad calls."""
+    from craft_amd import autograd, ops
+    took = []
+    for name in ("attention", "layer_norm"):
+        monkeypatch.setattr(ops, name, lambda *a, n=name, **k: took.append(n))
+    for cls in (autograd.Attention, autograd.LayerNorm):
+        monkeypatch.setattr(cls, "apply", lambda *a, n=cls.__name__: took.append(n))
+    x, w = torch.zeros(1, 4, 2, 16), torch.zeros(16, requires_grad=training)
+    with torch.enable_grad():
+        autograd.attention(x, x, x.clone().requires_grad_(training))
+        autograd.layer_norm(x, None, w)
+    assert took == (["Attention", "LayerNorm"] if training else ["attention", "layer_norm"])
+
+
+@gpu
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("H, Hk", [(4, 4), (4, 2)])
+def test_only_the_gradients_asked_for(device, monkeypatch, t, H, Hk):
+    """The same bits as all of them, and the others' kernels are not launched."""
+    from craft_amd import autograd
+    q, k, v, go = make(t, 2, 150, 150, H, Hk, 64)
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    want = torch.autograd.grad(autograd.attention(*leaves, causal=True), leaves, go)
+    seen = calls_of(monkeypatch)
+    for some in ((0,), (1,), (2,), (0, 2), (1, 2)):
+        xs = [x.clone().requires_grad_(n in some) for n, x in enumerate((q, k, v))]
+        got = torch.autograd.grad(autograd.attention(*xs, causal=True), [xs[n] for n in some], go)
+        assert all(torch.equal(g, want[n]) for g, n in zip(got, some))
+        name, args = seen[-1]
+        assert name == "craft_attention_bwd" and [a is not None for a in args[17:20]] == [0 in some, some != (0,), some != (0,)]
+
+
+def test_gradients_entry_point_takes_what_is_asked_for():
+    import ctypes
+
+    from craft_amd import hip
+    lib, buf = hip.load(), 4096
+    shape = (ctypes.c_long * 21)(*([1, 4, 4, 2, 2, 16] + [128, 32, 16] * 5))
+    bwd = lambda dq, dk, dv, group=0: lib.craft_attention_bwd(buf, buf, buf, buf, None, buf, buf, shape, None, None, None, None, 1.0, 0.0, 0, 1, group, dq, dk, dv, buf, 1 << 20, None)  # noqa: E731
+    assert bwd(None, None, None) == 0                                      # (nothing asked for: nothing launched)
+    assert bwd(buf, None, buf) == 10001 and bwd(buf, buf, None) == 10001 and bwd(buf, None, None, 1) == 10001
+    assert bwd(buf + 8, None, None) == 10002 and bwd(None, buf, buf + 8) == 10002
