@@ -344,21 +344,22 @@ class FlatMuon(FlatAdamW):
         buf = momentum buf + g;   u = g + momentum buf (Nesterov) or buf;   p = (1 - lr wd) p - lr s O(u),   s = match_rms sqrt(max(rows, cols))
 
     for every parameter that is a matrix of at least ``matrix_min`` rows and columns once its trailing axes are flattened (a convolution's
-    [cout, cin KH KW]); AdamW for the others (biases, norms, position tables, one-channel heads).  An orthogonal matrix of r rows and c columns has entries of
+    [cout, cin KH KW]); AdamW for the others (biases, norms, one-channel heads) and for ``tables``: parameters of any shape whose entries are looked up one
+    by one and multiply nothing (``position_tables`` of a model; the shape does not tell them from a matrix).  An orthogonal matrix of r rows and c columns has entries of
     rms 1 / sqrt(max(r, c)): s brings them to ``match_rms``, about that of an AdamW update, so that one learning rate serves both.  The momentum of a
     matrix lives in its range of ``exp_avg``; its range of ``exp_avg_sq`` is not used.  Every data-parallel rank orthogonalises the same summed
     gradient with the same bits (no atomics)."""
 
     def __init__(self, params: Iterable[torch.nn.Parameter], lr: float = 1e-3, betas=(0.9, 0.999), eps: float = 1e-8, weight_decay: float = 1e-2,
                  unused: Iterable[torch.nn.Parameter] = (), momentum: float = 0.95, nesterov: bool = True, ns_steps: int = 5, matrix_min: int = 16,
-                 match_rms: float = 0.2):
+                 match_rms: float = 0.2, tables: Iterable[torch.nn.Parameter] = ()):
         super().__init__(params, lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, unused=unused)
         if not 0 <= momentum < 1:
             raise ValueError("FlatMuon: momentum must be in [0, 1)")
         self.momentum, self.nesterov, self.ns_steps, self.match_rms = momentum, nesterov, ns_steps, match_rms
-        skip = set(self.unused_index)
+        skip, table_ids = set(self.unused_index), {id(p) for p in tables}
         self.matrix_index = [i for i, p in enumerate(self.params)
-                             if i not in skip and p.dim() >= 2 and min(p.shape[0], p.numel() // max(1, p.shape[0])) >= matrix_min]
+                             if i not in skip and id(p) not in table_ids and p.dim() >= 2 and min(p.shape[0], p.numel() // max(1, p.shape[0])) >= matrix_min]
         matrices = set(self.matrix_index)
         self.adam_segments, start = [], 0
         for i, (p, off) in enumerate(zip(self.params, self.offsets)):      # FlatAdamW.segments without the matrices' ranges
@@ -440,6 +441,14 @@ def unused_parameters(model: torch.nn.Module) -> List[torch.nn.Parameter]:
     return out
 
 
+def position_tables(model: torch.nn.Module) -> List[torch.nn.Parameter]:
+    """Parameters that are looked up by position: the positional-bias tables of the transformers (setrans.py:690-708) and embeddings (gma.py:12-13).
+    FlatMuon leaves them to AdamW."""
+    from .setrans import SlidingPosBiases2D
+    return ([m.biases for m in model.modules() if isinstance(m, SlidingPosBiases2D)] +
+            [m.weight for m in model.modules() if isinstance(m, torch.nn.Embedding)])
+
+
 OPTIMIZERS = {"adamw": FlatAdamW, "muon": FlatMuon}
 
 
@@ -448,7 +457,8 @@ def fetch_optimizer(model: torch.nn.Module, lr: float, wdecay: float, epsilon: f
     linear anneal, no momentum cycling).  ``optimizer="muon"``: FlatMuon under the same schedule."""
     if optimizer not in OPTIMIZERS:
         raise ValueError(f"optimizer {optimizer!r}: one of {', '.join(OPTIMIZERS)}")
-    opt = OPTIMIZERS[optimizer](model.parameters(), lr=lr, weight_decay=wdecay, eps=epsilon, unused=unused_parameters(model))
+    more = {"tables": position_tables(model)} if optimizer == "muon" else {}
+    opt = OPTIMIZERS[optimizer](model.parameters(), lr=lr, weight_decay=wdecay, eps=epsilon, unused=unused_parameters(model), **more)
     return opt, OneCycleLR(lr, num_steps + 100, pct_start=0.05)
 
 

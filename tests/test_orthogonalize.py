@@ -309,3 +309,24 @@ def test_results_in_one_place_are_refused():
         ops.orthogonalize([a, b], out=[b, a])
     with pytest.raises(CraftHipError, match="device tensors"):             # (the same matrix twice, results of their own: fine)
         ops.orthogonalize([a, a])
+
+
+@pytest.mark.parametrize("over", [dict(pos_bias_radius=9), dict(pos_bias_radius=7), dict(use_setrans=False, position_and_content=True),
+                                  dict(use_setrans=False)])
+def test_position_tables_are_adamws(over):
+    """Tables of 16 rows and columns or more (a radius of 9: 19 x 19; relative positions: 319 x 128) are no matrices, whatever their shape."""
+    from craft_amd import CRAFT, default_args
+    from craft_amd.train import fetch_optimizer
+    model = CRAFT(default_args(**over))
+    opt, _ = fetch_optimizer(model, 1e-3, 1e-4, 1e-8, 10, "muon")
+    names = [k for k, _ in model.named_parameters()]
+    matrices = {names[i] for i in opt.matrix_index}
+    tables = {k for k in names if k.endswith("pos_coder.biases") or "rel_height" in k or "rel_width" in k}
+    assert tables and not tables & matrices
+    shapes = {k: (p.shape[0], p.numel() // p.shape[0]) for k, p in model.named_parameters() if p.dim() >= 2}
+    unused = {names[i] for i in opt.unused_index}
+    assert matrices == {k for k, v in shapes.items() if min(v) >= 16} - tables - unused
+    at = {names.index(k) for k in tables - unused}
+    for i in at:
+        assert any(a <= opt.offsets[i] and opt.offsets[i] + opt.params[i].numel() <= b for a, b in opt.adam_segments)
+        assert set(opt.state_dict()["state"][i]) == {"step", "exp_avg", "exp_avg_sq"}
