@@ -325,12 +325,18 @@ class FlatAdamW:
         return {"state": state, "param_groups": [group]}
 
     def load_state_dict(self, sd: Dict):
+        for i, p in enumerate(self.params):                    # (a state that does not fit is refused before any of it is taken over)
+            st = sd["state"].get(i)
+            if st is None:
+                continue
+            if "exp_avg" not in st:
+                raise ValueError(f"FlatAdamW: the state of parameter {i} is another optimizer's ({', '.join(map(str, st))})")
+            if any(st[k].numel() != p.numel() for k in ("exp_avg", "exp_avg_sq")):
+                raise ValueError(f"FlatAdamW: the state of parameter {i} is {tuple(st['exp_avg'].shape)}, the parameter {tuple(p.shape)}")
         for i, (p, off) in enumerate(zip(self.params, self.offsets)):
             n = p.numel()
             st = sd["state"].get(i)
             if st is not None:
-                if "exp_avg" not in st:
-                    raise ValueError(f"FlatAdamW: the state of parameter {i} is another optimizer's ({', '.join(map(str, st))})")
                 self.exp_avg[off:off + n].copy_(st["exp_avg"].reshape(-1))
                 self.exp_avg_sq[off:off + n].copy_(st["exp_avg_sq"].reshape(-1))
                 self.step_count = int(float(st["step"]))

@@ -330,3 +330,19 @@ def test_position_tables_are_adamws(over):
     for i in at:
         assert any(a <= opt.offsets[i] and opt.offsets[i] + opt.params[i].numel() <= b for a, b in opt.adam_segments)
         assert set(opt.state_dict()["state"][i]) == {"step", "exp_avg", "exp_avg_sq"}
+
+
+def test_a_state_that_does_not_fit_changes_nothing():
+    """Refused before any of it is taken over: the first parameters of these nets have states that either optimizer could read."""
+    from craft_amd.train import FlatAdamW, FlatMuon
+    nets = lambda width: torch.nn.Sequential(torch.nn.LayerNorm(40), torch.nn.Linear(40, width))     # noqa: E731
+    muon, adam = FlatMuon(nets(32).parameters(), lr=0.5), FlatAdamW(nets(32).parameters(), lr=0.25)
+    wide = FlatAdamW(nets(48).parameters(), lr=0.125)
+    for opt in (muon, adam, wide):
+        opt.exp_avg.fill_(opt.lr)
+        opt.step_count = 7
+    for opt, other, says in ((adam, muon, "another optimizer"), (muon, adam, "another optimizer"), (adam, wide, "the parameter")):
+        fresh = type(opt)(nets(32).parameters(), lr=3.0)
+        with pytest.raises(ValueError, match=says):
+            fresh.load_state_dict(other.state_dict())
+        assert not fresh.exp_avg.any() and not fresh.exp_avg_sq.any() and fresh.step_count == 0 and fresh.lr == 3.0
