@@ -166,12 +166,14 @@ __global__ __launch_bounds__(256) void k_ns_init(NsParams p) {
   if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = sum;
   __syncthreads();
   sum = (red[0] + red[1]) + (red[2] + red[3]);
-  const float f = (float)((double)p.s_x / (sqrt(sum) + (double)p.eps));
+  // the factor as a fraction and a power of two: it is past fp32's range for a norm below 1e-34 and no eps, and subnormal for one above 1e38
+  int e2;
+  const float f = (float)frexp((double)p.s_x / (sqrt(sum) + (double)p.eps), &e2);
   const bool flip = j.rows > j.cols;
   const int r0 = flip ? tj : ti, c0 = flip ? ti : tj;                    // the tile of G
   for (int e = threadIdx.x; e < 64 * 64; e += 256) {
     const int r = e >> 6, c = e & 63;
-    const float v = r0 + r < j.rows && c0 + c < j.cols ? ns_get(j.src, (long)(r0 + r) * j.ld_src + c0 + c, p.dtype) * f : 0.f;
+    const float v = r0 + r < j.rows && c0 + c < j.cols ? ldexpf(ns_get(j.src, (long)(r0 + r) * j.ld_src + c0 + c, p.dtype), e2) * f : 0.f;
     if (flip) t[c][r] = v; else t[r][c] = v;
   }
   __syncthreads();

@@ -806,7 +806,8 @@ def _newton_schulz_coeffs(steps, coeffs):
 def orthogonalize(mats: Sequence[torch.Tensor], steps: int = 5, coeffs=NEWTON_SCHULZ, eps: float = 1e-7, out: Optional[Sequence[torch.Tensor]] = None):
     """Every matrix of the list with its singular values moved towards 1: X = G / (|G|_F + eps), then ``steps`` times X <- a X + (b A + c A A) X with
     A = X X^T from the smaller side.  ``coeffs``: (a, b, c), or one triple a step.  fp32 / fp16 / bf16 matrices of any strides, the smaller side up to
-    32768; fp32-class arithmetic whatever the type, one rounding at the end.  The whole list shares its launches.  ``out`` (may be ``mats``, and
+    32768; fp32-class arithmetic whatever the type, one rounding at the end.  (Entries of X keep 2^-40 of |G|_F + eps: a matrix far below eps, whose result
+    is about as small, loses its small entries; without an eps a matrix of zeros gives NaN.)  The whole list shares its launches.  ``out`` (may be ``mats``, and
     must not overlap another matrix of it): where the results go.  ``train.FlatMuon`` is the optimizer that uses it."""
     rows = _newton_schulz_coeffs(steps, coeffs)
     scales = _newton_schulz_scales(rows)

@@ -346,3 +346,15 @@ def test_a_state_that_does_not_fit_changes_nothing():
         with pytest.raises(ValueError, match=says):
             fresh.load_state_dict(other.state_dict())
         assert not fresh.exp_avg.any() and not fresh.exp_avg_sq.any() and fresh.step_count == 0 and fresh.lr == 3.0
+
+
+@gpu
+@pytest.mark.parametrize("size", [1e-44, 1e-40, 1e-36, 1e-30, 1e30, 1e37])
+@pytest.mark.parametrize("shape", [(60, 200), (300, 280)])
+def test_norms_at_the_ends_of_fp32(device, size, shape):
+    """Without an eps a matrix of any size that is not zero has a direction; the factor to it does not fit fp32, nor does the norm of the largest."""
+    from craft_amd import ops
+    mats = [(g.double() * size).float() for g in grads([shape], size=1.0)]
+    assert mats[0].any() and mats[0].isfinite().all()
+    check(ops.orthogonalize(mats, eps=0.0), mats, eps=0.0)
+    assert ops.orthogonalize([torch.zeros(5, 9, device="cuda")], eps=0.0)[0].isnan().all()
