@@ -1193,16 +1193,25 @@ class LayerNorm(Function):
 
     @staticmethod
     def forward(ctx, x, weight, bias, eps):
-        y, mean, rstd = ops._layer_norm(x, weight, bias, eps, None, True)
-        ctx.save_for_backward(x, weight, mean, rstd)
+        y, stats = ops._layer_norm_fwd(x, weight, bias, eps, None, True)
+        ctx.save_for_backward(x, weight, stats)
         ctx.weight_type = weight.dtype if weight is not None else bias.dtype if bias is not None else x.dtype
         return y
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, dy):
-        x, weight, mean, rstd = ctx.saved_tensors
-        return (*ops._layer_norm_bwd(x, weight, ctx.weight_type, dy, mean, rstd, ctx.needs_input_grad[:3]), None)
+        if torch.is_grad_enabled():                           # (create_graph: a second derivative raises)
+            return _layer_norm_grads_once(ctx, dy)
+        return _layer_norm_grads(ctx, dy)
+
+
+def _layer_norm_grads(ctx, dy):
+    x, weight, stats = ctx.saved_tensors
+    mean = stats.data_ptr()
+    return (*ops._layer_norm_bwd(x, weight, ctx.weight_type, dy, mean, mean + stats.nbytes // 2, ctx.needs_input_grad), None)
+
+
+_layer_norm_grads_once = torch.autograd.function.once_differentiable(_layer_norm_grads)
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5) -> torch.Tensor:

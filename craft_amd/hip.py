@@ -325,11 +325,13 @@ def _debug_note(name, args, conv):
 
 
 _PLAIN = frozenset((int, float, type(None), bool))
+_TENSORS = frozenset((torch.Tensor, torch.nn.Parameter))
 
 
 def call(name: str, *args):
     lib = load()
-    conv = [a if type(a) in _PLAIN else _ptr(a) if isinstance(a, torch.Tensor) else a for a in args]      # (isinstance of Tensor is slow on numbers)
+    # (isinstance of Tensor asks its metaclass: slow)
+    conv = [a if (t := type(a)) in _PLAIN else _ptr(a) if t in _TENSORS or isinstance(a, torch.Tensor) else a for a in args]
     if _DEBUG_PATH:
         _debug_note(name, args, conv)
     rc = getattr(lib, name)(*conv, _stream())

@@ -677,8 +677,10 @@ _NOTHING = contextlib.nullcontext()
 def _norm_rows(x: torch.Tensor):
     """(x as rows of one stride, the stride): x itself where its leading axes are one run of rows, else a copy."""
     C = x.shape[-1]
+    if x.is_contiguous():
+        return x, C
     if x.dim() == 1:
-        return (x, C) if x.stride(0) == 1 or C == 1 else (x.contiguous(), C)
+        return x.contiguous(), C
     if x.stride(-1) == 1 or C == 1:
         lead = [(n, st) for n, st in zip(x.shape[:-1], x.stride()[:-1]) if n != 1]
         if not lead:
@@ -709,25 +711,34 @@ def _check_layer_norm(x, weight, bias, eps):
 
 
 def _layer_norm(x, weight, bias, eps, out, stats: bool):
+    """(out, mean, rstd): the rows' statistics with ``stats``, else None"""
+    y, both = _layer_norm_fwd(x, weight, bias, eps, out, stats)
+    return (y, *both) if stats else (y, None, None)
+
+
+def _layer_norm_fwd(x, weight, bias, eps, out, keep: bool):
+    """(out, the rows' means and reciprocal deviations [2, rows] or None)"""
     wt = _check_layer_norm(x, weight, bias, eps)
     C = x.shape[-1]
     rows = x.numel() // C
     if out is None:
-        out = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    elif out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
-        raise hip.CraftHipError("layer_norm: out must be of x's shape, type and device")
-    y, ldy = _norm_rows(out)
-    if y.data_ptr() != out.data_ptr() or (rows > 1 and ldy < C):
-        raise hip.CraftHipError("layer_norm: out must be one run of rows with contiguous channels")
-    mean = rstd = None
-    if stats:
-        mean, rstd = torch.empty(2, rows, device=x.device, dtype=torch.float32)
+        out, ldy = x.new_empty(x.shape), C
+    else:
+        if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
+            raise hip.CraftHipError("layer_norm: out must be of x's shape, type and device")
+        y, ldy = _norm_rows(out)
+        if y.data_ptr() != out.data_ptr() or (rows > 1 and ldy < C):
+            raise hip.CraftHipError("layer_norm: out must be one run of rows with contiguous channels")
+        ldy = ldy if rows > 1 else C
+    # (a small call is as fast as its host: one tensor for both statistics, whose halves go by their addresses)
+    stats = x.new_empty((2, rows), dtype=torch.float32) if keep else None
     if rows:
         xr, ldx = _norm_rows(x)
-        w, b = (None if t is None else t.contiguous() for t in (weight, bias))
+        mean = stats.data_ptr() if keep else None
         with _on(x.device):
-            call("craft_layer_norm_fwd", xr, ldx, w, b, rows, C, float(eps), DTYPE_CODE[x.dtype], DTYPE_CODE[wt], y, ldy if rows > 1 else C, mean, rstd)
-    return out, mean, rstd
+            call("craft_layer_norm_fwd", xr, ldx, None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous(), rows, C,
+                 float(eps), DTYPE_CODE[x.dtype], DTYPE_CODE[wt], out, ldy, mean, mean + 4 * rows if keep else None)
+    return out, stats
 
 
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
@@ -736,7 +747,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     Statistics in fp32, the result rounded once to x's type.  ``tokens_norm`` is the weightless fp32 form of the model's tokens; the differentiable
     form is ``autograd.layer_norm``."""
     with torch.no_grad():
-        return _layer_norm(x, weight, bias, eps, out, False)[0]
+        return _layer_norm_fwd(x, weight, bias, eps, out, False)[0]
 
 
 def layer_norm_bwd(x: torch.Tensor, weight: Optional[torch.Tensor], bias_type: Optional[torch.dtype], dy: torch.Tensor, mean: torch.Tensor,
@@ -751,21 +762,26 @@ def layer_norm_bwd(x: torch.Tensor, weight: Optional[torch.Tensor], bias_type: O
             raise hip.CraftHipError(f"layer_norm_bwd: mean and rstd must be {rows} contiguous fp32 numbers")
     _check_layer_norm(x, weight, None, 0.0)
     _on_device(x, dy, mean, rstd)
-    return _layer_norm_bwd(x, weight, wt, dy, mean, rstd, need)
+    return _layer_norm_bwd(x, weight, wt, dy, mean.data_ptr(), rstd.data_ptr(), need)
 
 
-def _layer_norm_bwd(x, weight, wt, dy, mean, rstd, need):
+def _layer_norm_bwd(x, weight, wt, dy, mean: int, rstd: int, need):
     C = x.shape[-1]
     rows = x.numel() // C
-    new = lambda want, shape, t: torch.empty(shape, device=x.device, dtype=t) if want else None      # noqa: E731
-    dx, dw, db = new(need[0], x.shape, x.dtype), new(need[1], (C,), wt), new(need[2], (C,), wt)
+    dx, dw, db = x.new_empty(x.shape) if need[0] else None, None, None
+    if need[1] and need[2]:
+        dw, db = x.new_empty((2, C), dtype=wt).unbind()
+    elif need[1]:
+        dw = x.new_empty(C, dtype=wt)
+    elif need[2]:
+        db = x.new_empty(C, dtype=wt)
     if not rows:
         return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
     xr, ldx = _norm_rows(x)
-    g, ldg = _norm_rows(dy.to(x.dtype))
+    g, ldg = _norm_rows(dy if dy.dtype == x.dtype else dy.to(x.dtype))
     # one block of 1024 threads for each compute unit (or fewer, where there are few rows): each leaves one partial sum of the weight's gradients
     blocks = min(rows, 256)
-    ws = torch.empty(blocks * 2 * C, device=x.device, dtype=torch.float32) if need[1] or need[2] else None
+    ws = x.new_empty(blocks * 2 * C, dtype=torch.float32) if need[1] or need[2] else None
     with _on(x.device):
         call("craft_layer_norm_bwd", xr, ldx, g, ldg if rows > 1 else C, None if weight is None else weight.contiguous(), mean, rstd, rows, C,
              DTYPE_CODE[x.dtype], DTYPE_CODE[wt], dx, C, dw, db, ws, blocks)

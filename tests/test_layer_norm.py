@@ -286,3 +286,34 @@ def test_many_rows(device, t, rows, C):
     x, w, b = (v.requires_grad_() for v in (x, w, b))
     y = autograd.layer_norm(x, w, b)
     check([y, *torch.autograd.grad(y, (x, w, b), dy)], want, tol)
+
+
+@gpu
+def test_second_derivatives_are_refused(device):
+    """The backward pass has none of its own: asked for (create_graph), its results raise when they are differentiated, and are right until then."""
+    from craft_amd import autograd
+    x, w, b, dy = make("fp32", 20, 70)
+    want, tol = norm64(x, w, b, dy)
+    leaves = [v.requires_grad_() for v in (x, w, b)]
+    y = autograd.layer_norm(*leaves)
+    got = torch.autograd.grad(y, leaves, dy.requires_grad_(), create_graph=True)        # (torch refuses where the incoming gradient has one)
+    check([y, *got], want, tol)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        got[0].sum().backward()
+
+
+@gpu
+def test_statistics_of_two_calls_and_saved_rows(device):
+    """Two passes in flight keep statistics of their own, in whichever order their gradients are taken, and no rows at all give zero gradients."""
+    from craft_amd import autograd
+    runs = []
+    for seed in (0, 1):
+        x, w, b, dy = make("fp16", 30 + seed, 130, seed)
+        want = norm64(x, w, b, dy)
+        leaves = [v.requires_grad_() for v in (x, w, b)]
+        runs.append((leaves, dy, want, autograd.layer_norm(*leaves)))
+    for leaves, dy, (want, tol), y in runs[::-1]:
+        check([y, *torch.autograd.grad(y, leaves, dy)], want, tol)
+    x, w = torch.zeros(0, 130, device="cuda", requires_grad=True), torch.ones(130, device="cuda", requires_grad=True)
+    gx, gw = torch.autograd.grad(autograd.layer_norm(x, w), (x, w), torch.zeros(0, 130, device="cuda"))
+    assert gx.shape == (0, 130) and not gw.any()
