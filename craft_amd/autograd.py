@@ -1185,7 +1185,11 @@ def sequence_loss(flow_preds, flow_gt, valid, gamma: float = 0.8, max_flow: floa
 # LayerNorm with weights; attention with a cap, a distance bias and causal / prefix / document masks
 # ------------------------------------------------------------------------------------------------------------------
 def _wants_gradient(*tensors) -> bool:
-    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
 
 
 class LayerNorm(Function):

@@ -691,23 +691,24 @@ def _norm_rows(x: torch.Tensor):
 
 
 def _check_layer_norm(x, weight, bias, eps):
-    if x.dtype not in DTYPE_CODE:
-        raise hip.CraftHipError(f"layer_norm: fp32, fp16 or bf16 rows, not {x.dtype}")
-    if x.dim() < 1 or not 1 <= x.shape[-1] <= LAYER_NORM_MAX_WIDTH:
-        raise hip.CraftHipError(f"layer_norm: a last axis of 1 .. {LAYER_NORM_MAX_WIDTH}, not {tuple(x.shape)}")
+    dtype, shape = x.dtype, x.shape
+    if dtype not in DTYPE_CODE:
+        raise hip.CraftHipError(f"layer_norm: fp32, fp16 or bf16 rows, not {dtype}")
+    if not shape or not 1 <= shape[-1] <= LAYER_NORM_MAX_WIDTH:
+        raise hip.CraftHipError(f"layer_norm: a last axis of 1 .. {LAYER_NORM_MAX_WIDTH}, not {tuple(shape)}")
     if not eps >= 0:
         raise hip.CraftHipError("layer_norm: eps must not be negative")
     wt = None
-    for t, name in ((weight, "weight"), (bias, "bias")):
+    for t in (weight, bias):
         if t is None:
             continue
-        if t.shape != x.shape[-1:] or t.dtype not in (x.dtype, torch.float32):
-            raise hip.CraftHipError(f"layer_norm: {name} must be [{x.shape[-1]}] of {x.dtype} or fp32, not {tuple(t.shape)} of {t.dtype}")
+        if t.shape != shape[-1:] or (t.dtype != dtype and t.dtype != torch.float32):
+            raise hip.CraftHipError(f"layer_norm: {'weight' if t is weight else 'bias'} must be [{shape[-1]}] of {dtype} or fp32, not {tuple(t.shape)} of {t.dtype}")
         if wt is not None and t.dtype != wt:
             raise hip.CraftHipError("layer_norm: weight and bias must have one type")
         wt = t.dtype
     _on_device(x, weight, bias)
-    return wt or x.dtype
+    return wt or dtype
 
 
 def _layer_norm(x, weight, bias, eps, out, stats: bool):
