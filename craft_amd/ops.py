@@ -976,13 +976,19 @@ class AttentionPlan:
         return self.slopes, self.prefix, self.docs, self.docs_k
 
     def splits(self) -> int:
-        """0: blocks of 128 queries.  A few query rows (the tokens times the query heads of a key head) take the single-token kernel, whose keys are
-        split over so many blocks: two for each compute unit in all, a split at least 256 keys."""
+        """0: blocks of 128 queries.  Otherwise the kernel of few rows (the tokens times the query heads of a key head, 32 to a block), whose keys are split
+        over so many blocks: two for each compute unit in all, a split at least 256 keys.
+
+        Up to 64 rows always (16 bf16 tokens of 32 / 8 heads of 128 against 32768 keys: 47 us, blocks of 128 queries 688; against 512 keys 26 and 22, the join's
+        launch).  More rows where the keys are long and their blocks few enough to be split in two: 64 such tokens 92 and 692 us, 256 of them 283 and 690.
+        One split, 512 blocks, is about even (512 tokens 500 and 692, 32 of a batch of 16 1246 and 1126), 1024 blocks are not (1048 and 717).  Long is 2048 keys (1024: 26 and 22 us), for fp32, whose blocks take
+        3.6 times as long for a key, 512 (26 and 43 us; 300 keys at width 64: 22 and 30).  Documents keep to the blocks, which pass over tiles of others."""
         B, Nq, Nk, H, Hk, D = self.dims
         rows = Nq * (H // Hk)
-        if rows > 64:
+        blocks = B * Hk * ((rows + 31) // 32)
+        if rows > 64 and (self.docs is not None or blocks > 256 or Nk < (512 if self.code == PREC_F32 else 2048)):
             return 0
-        return max(1, min(512 // (B * Hk * ((rows + 31) // 32)), (Nk + 255) // 256))
+        return max(1, min(512 // blocks, (Nk + 255) // 256))
 
     def forward(self, out: torch.Tensor, lse: Optional[torch.Tensor] = None, rest: Optional[torch.Tensor] = None):
         B, Nq, Nk, H, Hk, D = self.dims

@@ -672,7 +672,7 @@ int craft_layer_norm_bwd(const void* x, long ldx, const void* dy, long lddy, con
  * cap: 0 (none) or positive, at most 4096 for 16-bit types, |scale| / cap at most 1e30.
  * splits 0: blocks of 128 queries.  For the backward pass they leave the log2-sums in lse ([B][H][Nq]; fp32: [B][H][Nq][2] with their rounding's rest; +inf
  * where nothing is seen) and, 16-bit types, the rest of out's rounding in out_rest (contiguous [B][Nq][H][D], 16-byte aligned); either may be NULL.
- * splits >= 1: for a few rows (Nq * H / Hk up to about 64): the keys split over so many blocks; no lse, no out_rest.
+ * splits >= 1: for few rows (Nq * H / Hk, of which 32 share a block's read of the keys): the keys split over so many blocks; no lse, no out_rest.
  * ws (16-byte aligned): splits 0 with documents: 16 * B * (ceil(Nq / 32) + ceil(Nk / 32)) bytes;  splits > 1: B * Nq * H * splits * (D + 2) floats. */
 int craft_attention_fwd(const void* q, const void* k, const void* v, const long* shape, const float* slopes, const int* prefix, const int* doc_q,
                         const int* doc_k, float scale, float cap, int causal, int dtype, int splits, void* out, float* lse, void* out_rest, void* ws,

@@ -670,3 +670,38 @@ def test_gradients_entry_point_takes_what_is_asked_for():
     assert bwd(None, None, None) == 0                                      # (nothing asked for: nothing launched)
     assert bwd(buf, None, buf) == 10001 and bwd(buf, buf, None) == 10001 and bwd(buf, None, None, 1) == 10001
     assert bwd(buf + 8, None, None) == 10002 and bwd(None, buf, buf + 8) == 10002
+
+
+@pytest.mark.parametrize("dims, t, docs, want", [
+    ((1, 16, 32768, 32, 8, 128), "bf16", False, 32), ((1, 17, 32768, 32, 8, 128), "bf16", False, 21), ((1, 256, 32768, 32, 8, 128), "bf16", False, 2),
+    ((1, 257, 32768, 32, 8, 128), "bf16", False, 0), ((1, 17, 32768, 32, 8, 128), "bf16", True, 0), ((1, 16, 32768, 32, 8, 128), "bf16", True, 32),
+    ((1, 17, 2047, 32, 8, 128), "fp16", False, 0), ((1, 17, 2048, 32, 8, 128), "fp16", False, 8), ((1, 17, 511, 32, 8, 64), "fp32", False, 0),
+    ((1, 17, 512, 32, 8, 64), "fp32", False, 2), ((1, 1, 4096, 128, 1, 128), "bf16", False, 16), ((16, 1, 32768, 32, 8, 128), "bf16", False, 4),
+    ((700, 1, 10, 1, 1, 64), "fp32", False, 1), ((1, 1, 1, 1, 1, 8), "bf16", False, 1)])
+def test_which_kernel(dims, t, docs, want):
+    """Few rows, and more of them where the keys are long and split in two at least, take the kernel whose keys are split."""
+    from craft_amd import ops
+    plan = object.__new__(ops.AttentionPlan)
+    plan.dims, plan.code, plan.docs = dims, ops.DTYPE_CODE[TYPES[t]], torch.zeros(1) if docs else None
+    assert plan.splits() == want
+
+
+@gpu
+@pytest.mark.parametrize("t", list(TYPES))
+@pytest.mark.parametrize("shape, how", [
+    ((1, 17, 2100, 16, 4, 128), dict(causal=True)), ((1, 33, 2048, 8, 2, 64), dict(causal=True, cap=10.0)), ((2, 100, 3001, 6, 2, 72), dict(causal=True, slopes=True)),
+    ((1, 1, 2500, 128, 1, 64), dict(causal=True)), ((1, 130, 2050, 3, 3, 32), {}), ((3, 90, 2111, 2, 2, 40), dict(causal=True, prefix=[1990, 0, 2111])),
+    ((1, 2049, 2049, 1, 1, 64), dict(causal=True)), ((1, 2300, 2060, 2, 2, 24), dict(causal=True, cap=5.0, slopes=True))])
+def test_a_chunk_against_long_keys(device, t, shape, how):
+    """More than 64 rows with their keys split: whole prompts, rows that see nothing (more queries than keys), many heads on one key head."""
+    from craft_amd import ops
+    B, nq, nk, H, Hk, D = shape
+    how = dict(how)
+    if how.get("slopes"):
+        how["slopes"] = slopes_of(H)
+    if "prefix" in how:
+        how["prefix"] = torch.tensor(how["prefix"], dtype=torch.int32, device="cuda")
+    q, k, v, _ = make(t, *shape)
+    assert ops.AttentionPlan(q, k, v, None, 0.0, None, False, None, None, None).splits() >= 2 and nq * H // Hk > 64
+    res, tol = attention64(q, k, v, **how)
+    check([ops.attention(q, k, v, **how)], res, tol)
