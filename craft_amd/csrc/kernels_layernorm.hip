@@ -86,7 +86,7 @@ __device__ __forceinline__ void ln_sum(float (&s)[NS], float* red, int wave_in_r
 }
 
 // TH threads: TH / TPR rows at a time; a block walks over the rows blockIdx.x * RPB + group, + gridDim.x * RPB, ... and has the next row's vectors on
-// their way while this one is worked on.  Two blocks to a compute unit.
+// their way while this one is worked on.
 template <typename T, typename W, int TPR, int NV, int TH>
 __global__ __launch_bounds__(TH) void k_layer_norm_fwd(LayerNormParams p) {
   constexpr int N = LnVec<T>::N, RPB = TH / TPR, NW = TPR > 64 ? TPR / 64 : 1;
@@ -295,7 +295,10 @@ static int layer_norm_run(const LayerNormParams& p, int blocks, void* dw, void* 
   auto go = [&](auto fwd, auto bwd, int tpr) {
     if (!p.dy) {
       const int th = tpr > 512 ? tpr : 512, rpb = th / tpr;
-      const long most = (p.rows + rpb - 1) / rpb, full = th == 512 ? 768 : 256;      // what the card holds at once (72 registers)
+      // what the card holds at once: three blocks of 512 threads to a compute unit (up to 74 registers), two of 1024 of one fp32 vector each (48 registers; us,
+      // 16384 rows of 4096: 107, one block 143), one of those of 16 bits or more vectors (68 .. 128; 8192 rows of 8192 bf16: 68 with one, 66 with two).
+      // 16384 rows of 1024 bf16 with 256 / 512 / 768 / 1024 / 2048 blocks: 25 / 17 / 15 / 17 / 18; of 4096: 87 / 58 / 50 / 58 / 54.
+      const long most = (p.rows + rpb - 1) / rpb, full = th == 512 ? 768 : sizeof(T) == 4 && p.C <= 4096 ? 512 : 256;
       hipLaunchKernelGGL(fwd, dim3((unsigned)(most < full ? most : full)), dim3(th), 0, s, p);
       return (int)hipGetLastError();
     }
