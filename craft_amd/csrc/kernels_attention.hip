@@ -122,10 +122,10 @@ int craft_attention_bwd(const void* q, const void* k, const void* v, const void*
   if ((dk == nullptr) != (dv == nullptr) || (split_group && !dk)) return CRAFT_ERR_ARG;
   if (!lse || (reinterpret_cast<uintptr_t>(out_rest) & 15)) return CRAFT_ERR_ARG;
   const long ranges = range_bytes(p), delta = ((long)p.B * p.H * p.Nq * 4 + 15) / 16 * 16, part = split_group ? (long)p.B * p.Nk * p.H * p.D * 4 : 0;
-  // fp16: a key head's rows are cut into slices for the largest norms, 16 rows each, 1024 slices at most, which a wave reads 64 at a time
+  // fp16: a key head's rows are cut into slices for the largest norms: as many rows as a block has groups of lanes, 1024 slices at most (a wave reads them all)
   const bool f16 = dtype == CRAFT_PREC_F16;
-  const long rows = (long)p.Nq * (p.H / p.Hk) > p.Nk ? (long)p.Nq * (p.H / p.Hk) : p.Nk, slices = rows >= 16384 ? 1024 : (rows + 1023) / 1024 * 64;
-  const long more = f16 ? 8192l * p.B * p.Hk : 0;
+  const long rows = (long)p.Nq * (p.H / p.Hk) > p.Nk ? (long)p.Nq * (p.H / p.Hk) : p.Nk, each = p.D > 64 ? 16 : 32;
+  const long slices = (rows + each - 1) / each < 1024 ? (rows + each - 1) / each : 1024, more = f16 ? (8 * slices * p.B * p.Hk + 15) / 16 * 16 : 0;
   if (!aligned(ws) || ws_bytes < ranges + delta + more + 2 * part) return CRAFT_ERR_ARG;
   if (!dq && !dk) return 0;
   const hipStream_t s = reinterpret_cast<hipStream_t>(stream);

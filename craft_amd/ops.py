@@ -1011,9 +1011,15 @@ class AttentionPlan:
         go = _strided(go.to(self.q.dtype))
         dq = torch.empty(B, Nq, H, D, device=self.device, dtype=self.q.dtype) if need[0] else None
         dk, dv = torch.empty(2, B, Nk, Hk, D, device=self.device, dtype=self.q.dtype) if need[1] or need[2] else (None, None)
-        # key / value gradients of shared heads: one block walks over the group's heads, unless that leaves compute units without a block
+        # key / value gradients of shared heads: one block walks over the group's heads, unless that leaves compute units without one of the two blocks they
+        # hold.  (A block for each query head and a sum against it, us, causal, 2048 tokens, 4 key heads: 16 heads of 128 in bf16, 64 / 256 / 384 / 512 / 768 blocks:
+        # 129 / 216 / 324 / 426 / 655 against 417 / 434 / 447 / 465 / 534; fp16 and fp32 of 64 cross at the same place; without a mask it lies at 384.)
         split_group = int(dk is not None and H > Hk and B * Hk * ((Nk + 127) // 128) < 512)
-        nbytes = self.range_bytes() + (4 * B * H * Nq + 15) // 16 * 16 + (8192 * B * Hk if self.code == hip.PREC_F16 else 0) + split_group * 8 * B * Nk * H * D
+        up = lambda n: (n + 15) // 16 * 16                                 # noqa: E731
+        nbytes = self.range_bytes() + up(4 * B * H * Nq) + split_group * 8 * B * Nk * H * D
+        if self.code == hip.PREC_F16:                                      # (the largest norms, for the gradients' powers of two)
+            each = 16 if D > 64 else 32
+            nbytes += up(8 * B * Hk * min(1024, (max(Nq * (H // Hk), Nk) + each - 1) // each))
         with _on(self.device):
             call("craft_attention_bwd", self.q, self.k, self.v, out, rest, lse, go, self.shape(out, go), *self.masks(), self.scale, self.cap, self.causal, self.code,
                  split_group, dq, dk, dv, self.new(nbytes), nbytes)

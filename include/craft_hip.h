@@ -680,8 +680,8 @@ int craft_attention_fwd(const void* q, const void* k, const void* v, const long*
 /* gradients of q [B][Nq][H][D], k and v [B][Nk][Hk][D], contiguous.  out_rest may be NULL (the gradients are then off by out's rounding too).  shape: 21 host longs, as above with the strides of grad_out last.
  * dq may be NULL, and dk and dv together: what is not asked for is not computed.
  * split_group 1: a block per query head for the key / value gradients and a sum over the heads of a group behind it (more blocks, fp32 partial results).
- * ws (16-byte aligned): the documents' ranges as above, then B * H * Nq floats rounded up to 16 bytes, for CRAFT_PREC_F16 8192 * B * Hk bytes, then
- * with split_group 2 * B * Nk * H * D floats.
+ * ws (16-byte aligned): the documents' ranges as above, then B * H * Nq floats rounded up to 16 bytes, for CRAFT_PREC_F16
+ * 2 * B * Hk * min(1024, ceil(max(Nq * H / Hk, Nk) / (D > 64 ? 16 : 32))) floats rounded up likewise, then with split_group 2 * B * Nk * H * D floats.
  * The result does not depend on the order in which blocks run. */
 int craft_attention_bwd(const void* q, const void* k, const void* v, const void* out, const void* out_rest, const float* lse, const void* grad_out, const long* shape,
                         const float* slopes, const int* prefix, const int* doc_q, const int* doc_k, float scale, float cap, int causal, int dtype,
