@@ -690,6 +690,40 @@ def _norm_rows(x: torch.Tensor):
     return x.contiguous(), C
 
 
+def _owns_its_elements(t: torch.Tensor) -> bool:
+    """No two elements of t lie in one place."""
+    extent = 1
+    for st, n in sorted(zip(t.stride(), t.shape)):
+        if n > 1:
+            if st < extent:
+                return False
+            extent += (n - 1) * st
+    return True
+
+
+def _pieces(t: torch.Tensor):
+    """(address, bytes that lie together, steps in bytes from one such piece to another, bytes from the first to behind the last)"""
+    run, steps, extent, size = 1, [], 1, t.element_size()
+    for st, n in sorted(zip(t.stride(), t.shape)):
+        if n > 1 and st:
+            extent += (n - 1) * st
+            if st == run and not steps:
+                run *= n
+            else:
+                steps.append(st * size)
+    return t.data_ptr(), run * size, steps, extent * size
+
+
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """No element of a is one of b's: their ranges do not meet, or their pieces lie beside one another in every common step (slices of one projection)."""
+    pa, ra, sa, ea = _pieces(a)
+    pb, rb, sb, eb = _pieces(b)
+    if pa + ea <= pb or pb + eb <= pa:
+        return True
+    step = math.gcd(*sa, *sb)
+    return step > 0 and ra <= (pb - pa) % step <= step - rb
+
+
 def _check_layer_norm(x, weight, bias, eps):
     dtype, shape = x.dtype, x.shape
     if dtype not in DTYPE_CODE:
@@ -722,7 +756,8 @@ def _layer_norm_fwd(x, weight, bias, eps, out, keep: bool):
     wt = _check_layer_norm(x, weight, bias, eps)
     C = x.shape[-1]
     rows = x.numel() // C
-    if out is None:
+    given = out is not None
+    if not given:
         out, ldy = x.new_empty(x.shape), C
     else:
         if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device:
@@ -735,6 +770,8 @@ def _layer_norm_fwd(x, weight, bias, eps, out, keep: bool):
     stats = x.new_empty((2, rows), dtype=torch.float32) if keep else None
     if rows:
         xr, ldx = _norm_rows(x)
+        if given and not (y.data_ptr() == xr.data_ptr() and (ldy == ldx or rows == 1)) and not _apart(y, xr):
+            raise hip.CraftHipError("layer_norm: out may be x itself, and must not overlap it otherwise")
         mean = stats.data_ptr() if keep else None
         with _on(x.device):
             call("craft_layer_norm_fwd", xr, ldx, None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous(), rows, C,
@@ -745,7 +782,7 @@ def _layer_norm_fwd(x, weight, bias, eps, out, keep: bool):
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """LayerNorm over the last axis (width up to 16384) of fp32 / fp16 / bf16 rows; weight and bias [C] of the rows' type or fp32, each optional.
-    Statistics in fp32, the result rounded once to x's type.  ``tokens_norm`` is the weightless fp32 form of the model's tokens; the differentiable
+    Statistics in fp32, the result rounded once to x's type.  ``out`` may be x, and must not overlap it otherwise.  ``tokens_norm`` is the weightless fp32 form of the model's tokens; the differentiable
     form is ``autograd.layer_norm``."""
     with torch.no_grad():
         return _layer_norm_fwd(x, weight, bias, eps, out, False)[0]
@@ -1042,11 +1079,13 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optio
         plan = AttentionPlan(q, k, v, scale, cap, slopes, causal, prefix, docs, docs_k)
         if out is None:
             out = torch.empty(q.shape, device=q.device, dtype=q.dtype)
-        elif (out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not _in_place(out)
-              or any(n > 1 and s == 0 for n, s in zip(out.shape, out.stride()))):
-            raise hip.CraftHipError("attention: out must be of q's shape, type and device, with 16-byte aligned rows")
-        elif out.numel() and out.data_ptr() in (k.data_ptr(), v.data_ptr()):
-            raise hip.CraftHipError("attention: out must not be k's or v's memory, which other blocks still read")
+        elif out.shape != q.shape or out.dtype != q.dtype or out.device != q.device or not _in_place(out) or not _owns_its_elements(out):
+            raise hip.CraftHipError("attention: out must be of q's shape, type and device, with 16-byte aligned rows of its own")
+        elif out.numel():
+            is_q = out.data_ptr() == plan.q.data_ptr() and _strides(out) == _strides(plan.q)
+            for t, name in ((plan.q, "q"), (plan.k, "k"), (plan.v, "v")):
+                if t.numel() and not (name == "q" and is_q) and not _apart(out, t):
+                    raise hip.CraftHipError(f"attention: out must not share memory with {name}, which other blocks still read (it may be q itself)")
         if out.numel() and not k.shape[1]:
             return out.zero_()
         if out.numel():

@@ -726,3 +726,82 @@ def test_norms_of_many_and_long_rows(device, B, n, H, Hk, D):
         assert torch.isfinite(g).all(), name
         off, least = (g.double() - w.double()).norm().item(), unavoidable(w.double(), torch.float16)
         assert off <= least + 2.0 ** -11 * w.double().norm().item(), (name, off / least)
+
+
+def test_memory_that_is_shared_or_not():
+    from craft_amd import ops
+    flat = torch.zeros(4096)
+    at = lambda o, shape, strides: torch.as_strided(flat, shape, strides, o)                  # noqa: E731
+    a, b, c = torch.zeros(2, 5, 3, 4, 8).unbind(2)
+    assert ops._apart(a, b) and ops._apart(b, a) and ops._apart(a, c) and not ops._apart(a, a)            # slices of one projection
+    a, b, c = torch.zeros(2, 5, 4, 3, 8).unbind(3)                                            # within a head
+    assert ops._apart(a, b) and ops._apart(c, a)
+    x = torch.zeros(3, 20, 2, 8)
+    assert ops._apart(x[:, :5], x[:, 5:9]) and not ops._apart(x[:, :5], x[:, 4:9]) and ops._apart(x[:1], x[1:2]) and not ops._apart(x[:2], x[1:])
+    assert ops._apart(x[..., :4], x[..., 4:]) and not ops._apart(x[..., :5], x[..., 4:]) and ops._apart(flat[:10], flat[10:]) and not ops._apart(flat[:10], flat[9:])
+    assert not ops._apart(flat[:8].expand(6, 8), flat[:48].view(6, 8)) and not ops._apart(at(0, (4, 8), (10, 1)), at(6, (4, 8), (10, 1)))
+    # (against every element, over random pairs: what it calls apart is)
+    g = torch.Generator().manual_seed(0)
+    r = lambda hi: int(torch.randint(0, hi, (1,), generator=g))                               # noqa: E731
+    proven = 0
+    for _ in range(400):
+        t = [at(r(60), (1 + r(3), 1 + r(4), 1 + r(5)), (r(4) * 12, r(3) * 6, 1 + r(2))) for _ in range(2)]
+        places = [{o + i * s[0] + j * s[1] + k * s[2] for i in range(n[0]) for j in range(n[1]) for k in range(n[2])}
+                  for o, s, n in ((y.storage_offset(), y.stride(), y.shape) for y in t)]
+        if ops._apart(*t):
+            proven += 1
+            assert not places[0] & places[1]
+        for y, p in zip(t, places):
+            assert not ops._owns_its_elements(y) or len(p) == y.numel()
+    assert proven > 40
+
+
+@gpu
+@pytest.mark.parametrize("nq", [1, 40])
+def test_out_that_shares_memory(device, nq):
+    """q's own memory and slices beside q, k and v are written; what overlaps them is refused."""
+    from craft_amd import ops
+    from craft_amd.hip import CraftHipError
+    g = torch.Generator().manual_seed(4)
+    qkvo = torch.randn(2, 60, 4, 2, 64, generator=g).bfloat16().cuda()
+    q, k, v, o = qkvo.unbind(2)
+    want = ops.attention(q[:, :nq], k, v)
+    assert torch.equal(ops.attention(q[:, :nq], k, v, out=o[:, :nq]), want) and torch.equal(o[:, :nq], want)
+    later = q[:, nq:2 * nq] if 2 * nq <= 60 else q[:, :0]
+    assert later.numel() == 0 or torch.equal(ops.attention(q[:, :nq], k, v, out=later), want)
+    for bad in (k[:, :nq], v[:, :nq], v[:, 1:nq + 1], q[:, 1:nq + 1] if nq > 1 else k[:, 5:6], qkvo[:, :nq, 1:3].flatten(2, 3)[:, :, 1:3],
+                torch.as_strided(qkvo, (2, nq, 2, 64), (0, 512, 64, 1)), torch.as_strided(o.clone(), (2, nq, 2, 64), (8, 128, 64, 1))):
+        with pytest.raises(CraftHipError, match="out must"):
+            ops.attention(q[:, :nq], k, v, out=bad)
+    assert torch.equal(ops.attention(q[:, :nq], k, v, out=q[:, :nq]), want)
+
+
+@gpu
+@pytest.mark.parametrize("t", list(TYPES))
+def test_captured_gradients(device, t):
+    """A training step's forward and backward pass in a graph whose replays follow new inputs, eager steps between them; every replay against eager."""
+    from craft_amd import autograd
+    q, k, v, go = make(t, 2, 150, 150, 4, 2, 72)
+    docs = doc_ids(2, 150, 4, 30)
+    w = torch.ones(72, device="cuda").to(q.dtype)
+
+    def step(q, k, v, go, w):
+        leaves = [x.detach().requires_grad_() for x in (q, k, v, w)]
+        o = autograd.layer_norm(autograd.attention(*leaves[:3], docs=docs, causal=True, cap=20.0), leaves[3])
+        return [o, *torch.autograd.grad(o, leaves, go)]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(q, k, v, go, w)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step(q, k, v, go, w)
+    for seed in range(4):
+        for x, y in zip((q, k, v, go), make(t, 2, 150, 150, 4, 2, 72, seed=seed)):
+            x.copy_(y * (1 if seed < 2 else 1e-4))
+        docs.copy_(doc_ids(2, 150, 4, 30, seed=seed))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = step(q, k, v, go, w)
+        assert all(torch.equal(a, b) for a, b in zip(got, want))

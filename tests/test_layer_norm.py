@@ -317,3 +317,19 @@ def test_statistics_of_two_calls_and_saved_rows(device):
     x, w = torch.zeros(0, 130, device="cuda", requires_grad=True), torch.ones(130, device="cuda", requires_grad=True)
     gx, gw = torch.autograd.grad(autograd.layer_norm(x, w), (x, w), torch.zeros(0, 130, device="cuda"))
     assert gx.shape == (0, 130) and not gw.any()
+
+
+@gpu
+def test_out_that_shares_memory(device):
+    """x itself and columns beside it are written; rows that others still read are refused."""
+    from craft_amd import ops
+    from craft_amd.hip import CraftHipError
+    buf = torch.randn(50, 300, device="cuda")
+    want = ops.layer_norm(buf[:, :130])
+    assert torch.equal(ops.layer_norm(buf[:, :130], out=buf[:, 130:260]), want)
+    for x, out in ((buf[:40, :100], buf[1:41, :100]), (buf[:, :100], buf[:, 50:150]), (buf[:1, :100].expand(40, 100), buf[:40, :100])):
+        with pytest.raises(CraftHipError, match="must not overlap"):
+            ops.layer_norm(x, out=out)
+    assert torch.equal(ops.layer_norm(buf[:, :130], out=buf[:, :130]), want)
+    one = buf[:1, 200:].clone()
+    assert torch.equal(ops.layer_norm(one, out=one), ops.layer_norm(buf[:1, 200:]))
