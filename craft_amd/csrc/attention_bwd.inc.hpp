@@ -486,7 +486,7 @@ __global__ __launch_bounds__(256, (sizeof(T) == 2 || DP == 32 ? 2 : 1)) void k_a
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
               const int r = 4 * g + e, dr = e == 0 ? di.x : e == 1 ? di.y : e == 2 ? di.z : di.w;
-              const bool see = acc_row(r) >= need && acc_row(r) < room && (!docmask || (dr == mydoc && dr >= 0));
+              const bool see = (acc_row(r) >= need) & (acc_row(r) < room) & (!docmask | ((dr == mydoc) & (dr >= 0)));
               x[r] = see ? x[r] : 0.f;
               y[r] = see ? y[r] : 0.f;
             }
