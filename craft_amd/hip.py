@@ -329,9 +329,9 @@ _TENSORS = frozenset((torch.Tensor, torch.nn.Parameter))
 
 
 def call(name: str, *args):
-    lib = load()
+    lib = _lib or load()
     # (isinstance of Tensor asks its metaclass: slow)
-    conv = [a if (t := type(a)) in _PLAIN else _ptr(a) if t in _TENSORS or isinstance(a, torch.Tensor) else a for a in args]
+    conv = [a if (t := type(a)) in _PLAIN else a.data_ptr() if t in _TENSORS and a.is_cuda else _ptr(a) if isinstance(a, torch.Tensor) else a for a in args]
     if _DEBUG_PATH:
         _debug_note(name, args, conv)
     rc = getattr(lib, name)(*conv, _stream())
@@ -340,6 +340,14 @@ def call(name: str, *args):
         raise CraftHipError(f"{name} failed with code {rc}: {msg}")
     if _DEBUG_PATH:
         torch.cuda.synchronize()
+
+
+def call_on(device, name: str, *args):
+    """``call`` with ``device`` current."""
+    if device.index == torch._C._cuda_getDevice():
+        return call(name, *args)
+    with torch.cuda.device(device):
+        return call(name, *args)
 
 
 _CARRAY_TYPES = {}

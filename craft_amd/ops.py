@@ -773,9 +773,8 @@ def _layer_norm_fwd(x, weight, bias, eps, out, keep: bool):
         if given and not (y.data_ptr() == xr.data_ptr() and (ldy == ldx or rows == 1)) and not _apart(y, xr):
             raise hip.CraftHipError("layer_norm: out may be x itself, and must not overlap it otherwise")
         mean = stats.data_ptr() if keep else None
-        with _on(x.device):
-            call("craft_layer_norm_fwd", xr, ldx, None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous(), rows, C,
-                 float(eps), DTYPE_CODE[x.dtype], DTYPE_CODE[wt], out, ldy, mean, mean + 4 * rows if keep else None)
+        hip.call_on(x.device, "craft_layer_norm_fwd", xr, ldx, None if weight is None else weight.contiguous(), None if bias is None else bias.contiguous(),
+                    rows, C, float(eps), DTYPE_CODE[x.dtype], DTYPE_CODE[wt], out, ldy, mean, mean + 4 * rows if keep else None)
     return out, stats
 
 
@@ -806,23 +805,19 @@ def layer_norm_bwd(x: torch.Tensor, weight: Optional[torch.Tensor], bias_type: O
 def _layer_norm_bwd(x, weight, wt, dy, mean: int, rstd: int, need):
     C = x.shape[-1]
     rows = x.numel() // C
-    dx, dw, db = x.new_empty(x.shape) if need[0] else None, None, None
-    if need[1] and need[2]:
+    dx, dw, db, ws = x.new_empty(x.shape) if need[0] else None, None, None, None
+    # one block of 1024 threads for each compute unit (or fewer, where there are few rows): each leaves one partial sum of the weight's gradients
+    blocks = min(rows, 256)
+    if need[1] or need[2]:
         dw, db = x.new_empty((2, C), dtype=wt).unbind()
-    elif need[1]:
-        dw = x.new_empty(C, dtype=wt)
-    elif need[2]:
-        db = x.new_empty(C, dtype=wt)
+        ws = x.new_empty(blocks * 2 * C, dtype=torch.float32) if rows else None
+        dw, db = dw if need[1] else None, db if need[2] else None
     if not rows:
         return dx, None if dw is None else dw.zero_(), None if db is None else db.zero_()
     xr, ldx = _norm_rows(x)
     g, ldg = _norm_rows(dy if dy.dtype == x.dtype else dy.to(x.dtype))
-    # one block of 1024 threads for each compute unit (or fewer, where there are few rows): each leaves one partial sum of the weight's gradients
-    blocks = min(rows, 256)
-    ws = x.new_empty(blocks * 2 * C, dtype=torch.float32) if need[1] or need[2] else None
-    with _on(x.device):
-        call("craft_layer_norm_bwd", xr, ldx, g, ldg if rows > 1 else C, None if weight is None else weight.contiguous(), mean, rstd, rows, C,
-             DTYPE_CODE[x.dtype], DTYPE_CODE[wt], dx, C, dw, db, ws, blocks)
+    hip.call_on(x.device, "craft_layer_norm_bwd", xr, ldx, g, ldg if rows > 1 else C, None if weight is None else weight.contiguous(), mean, rstd, rows, C,
+                DTYPE_CODE[x.dtype], DTYPE_CODE[wt], dx, C, dw, db, ws, blocks)
     return dx, dw, db
 
 
