@@ -784,7 +784,7 @@ def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Opt
     Statistics in fp32, the result rounded once to x's type.  ``out`` may be x, and must not overlap it otherwise.  ``tokens_norm`` is the weightless fp32 form of the model's tokens; the differentiable
     form is ``autograd.layer_norm``."""
     with torch.no_grad():
-        return _layer_norm_fwd(x, weight, bias, eps, out, False)[0]
+        return _layer_norm(x, weight, bias, eps, out, False)[0]
 
 
 def layer_norm_bwd(x: torch.Tensor, weight: Optional[torch.Tensor], bias_type: Optional[torch.dtype], dy: torch.Tensor, mean: torch.Tensor,
