@@ -1259,7 +1259,9 @@ def attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, *, scale: Optio
               causal: bool = False, prefix: Optional[torch.Tensor] = None, docs: Optional[torch.Tensor] = None,
               docs_k: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Differentiable ``ops.attention``: gradients of q, k and v (those of shared key heads summed over the heads that read them); the masks, slopes and
-    the cap have none.  The scores are computed again in the backward pass; no N x N tensor is kept."""
+    the cap have none.  The scores are computed again in the backward pass; no N x N tensor is kept.  16-bit types round the probabilities and the scores'
+    gradients once to their own type for the products behind them: dq and dk are off by about 1.6 times what rounding the result alone costs, whatever the
+    size of the incoming gradient (fp16 carries both times powers of two)."""
     if slopes is not None and slopes.requires_grad:
         raise hip.CraftHipError("attention: slopes have no gradient here")
     if not _wants_gradient(q, k, v):                                       # (a few query rows: the single-token kernel, which keeps no log-sums)

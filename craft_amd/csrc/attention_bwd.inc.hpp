@@ -4,8 +4,10 @@
 // queries and walks over the keys, k_attention_dkv owns 128 keys and walks over the queries of every head that shares them.  Both recompute the scores.
 //
 // Bound by the same turns of vector and matrix instructions as the forward pass, with 18 instead of 14 D operations a pair (the scores and dp twice:
-// the price of one writer for each gradient).  Capped, causal, 4096 bf16 tokens x 32 heads of 128 on 8 key heads: dk, dv 380 us
-// (0.72 PF/s), dq 280 us (0.74 PF/s), the sum over the group 24 us, delta 18 us.  fp32, 2852 tokens x 8 heads of 64: 401 and 301 us, 83 TF/s of 154.
+// the price of one writer for each gradient).  Capped, causal, 4096 bf16 tokens x 32 heads of 128 on 8 key heads: dk, dv 368 us
+// (0.75 PF/s; matrix instructions 36 %, vector instructions 41 % of the SIMDs' cycles, the rest waits for LDS), dq 288 us (0.72 PF/s; 35 % and 48 %), the sum over
+// the group 24 us, delta 18 us.  fp32, 2852 tokens x 8 heads of 64: 396 and 300 us, 83 TF/s of 154 (55 % and 8 %).  fp16, 4 x 3001 tokens in documents of about
+// 400, 8 heads of 64: 89 and 51 us, delta and the largest norms 12 us: two of three SIMDs' cycles wait, tiles cut by documents' borders and their ranges read in the walk.
 #pragma once
 #include "attention_tile.hpp"
 

@@ -1,11 +1,11 @@
 // Forward attention: a block owns 128 queries of one head (4 waves x 32), walks over the keys in LDS tiles, and keeps the running maximum and sum
 // of the softmax, the query operand and the 32 x D output in registers.
 //
-// Bound by the vector instructions of the softmax, which take the SIMD in turns with the matrix instructions (exponentials and reciprocals run beside
-// them, multiplications and maxima do not), and at large sizes by the package's power (1.85 GHz).  8192 fp16 queries x 32 heads of 128, causal with a
-// prefix of 1900: 609 us, 0.95 PF/s, 68 % of what a large library product reaches; matrix units busy 52 % of the time.  With scores of the next tile
-// computed under the softmax of this one the same 628 us stood against 628 (and capped scores were slower): no slot is left to fill.  Capped, causal,
-// 4096 bf16 tokens x 32 heads of 128: 220 us.  fp32, 2852 tokens x 8 heads of 64: 242 us, 69 TF/s (the rate of an fp32 library product is 154).
+// Bound by the vector instructions of the softmax, which take the SIMD in turns with the matrix instructions, and at large sizes by the package's power.
+// 8192 fp16 queries x 32 heads of 128, causal with a prefix of 1900: 607 .. 626 us, 0.95 PF/s, 68 % of what a large library product reaches; counters: matrix
+// instructions 50 % of the SIMDs' cycles, vector instructions 44 %, at 1.5 .. 1.7 GHz.  With scores of the next tile computed under the softmax of this one the
+// same 628 us stood against 628 (and capped scores were slower).  Capped, causal, 4096 bf16 tokens x 32 heads of 128: 222 us (29 % and 54 %).  fp32, 2852 tokens
+// x 8 heads of 64: 242 us, 69 TF/s (the rate of an fp32 library product is 154): 45 % and 10 %, one wave to a SIMD waits for its own products.
 #pragma once
 #include "attention_tile.hpp"
 

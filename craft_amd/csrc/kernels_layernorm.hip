@@ -9,7 +9,9 @@
 // Vectors are 16 bytes at any alignment (unaligned loads and stores are native): an odd width moves its last vector back (LnCols).
 //
 // 16384 rows of 4096 bf16: forward 52 us (5.2 TB/s), backward 81 us (5.0 TB/s), the sum over the blocks 4 us; a copy of 256 MiB moves 5.5 TB/s, one of
-// 2 GiB 4.9.  28672 rows of 256 fp32: 12 us (4.8 TB/s).  1441 rows of 1027 fp16: 6 + 11 + 4 us, latency.
+// 2 GiB 4.9.  28672 rows of 256 fp32: 12 us (4.8 TB/s).  1441 rows of 1027 fp16: 6 + 11 + 4 us, latency.  Above 8192 columns the backward kernel's 1024 threads
+// keep 128 .. 448 bytes each in scratch (16-bit rows of an odd width from 4096 on 36): 4096 rows of 16384, forward and backward, bf16 322 us (2.1 TB/s), fp32 494 (2.7);
+// 8192 rows of 8192 take 163 (4.1 TB/s) and 272 us (4.9).
 #include <type_traits>
 #include "launch.hpp"
 #include "../../include/craft_hip.h"

@@ -14,8 +14,9 @@
 // and X^T.  X^T is kept twice (blocks of one strip read it whole while others write).
 //
 // One 2048 x 8192 matrix: 1.86 ms, of which B X five times 202 us (three fp16 products: 1.02 PF/s, 73 % of a large library product's 1.39), X X^T 114 us
-// and 14 us for the sum of its shares, B 34 + 18 us.  The 53 matrices of the CRAFT model (64 x 147 .. 1024 x 256): 310 us in 18 launches, bound by each launch's
-// own latency (its operations are 33 us): X X^T 22 us, B 7 us, B X 26 us a step.  One 256 x 256: 106 us, 18 launches of 4 .. 8 us.
+// and 14 us for the sum of its shares, B 34 + 18 us.  The 53 matrices of the CRAFT model (64 x 147 .. 1024 x 256): 306 .. 324 us in 18 launches (its operations
+// are 33 us).  B X 26 us a step: it moves 142 MB (a strip of X^T once for each 64 rows of tiles, the old X, X and X^T written), 5.4 TB/s.  X X^T 22 us: 192 blocks,
+// a tile's whole K in each, up to 20 steps of a wave one behind the other's loads.  B 7 us.  One 256 x 256: 106 us, 18 dependent launches of 4 .. 8 us.
 //
 // Rows and columns are padded to 64 (128) with zeros, which the products keep.
 #include "attention_tile.hpp"
