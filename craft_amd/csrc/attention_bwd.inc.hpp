@@ -41,7 +41,7 @@ __global__ __launch_bounds__(256) void k_attention_delta(AttentionParams p, floa
 
 // The same for fp16, which also needs the largest norms for its powers of two (score_exponent): a block per (batch, key head, slice), whose
 // share of the queries of the head's group and of its keys it reads, 8 or 16 lanes to a row.  Padding's rows do not count.  All loads of a row stand in front of
-// its sums (one behind the other they took twice the time).
+// its sums (one behind the other: 20 us instead of 16; as many slices as there are rows for: 12).
 template <typename T>
 __global__ __launch_bounds__(256) void k_attention_delta_scaled(AttentionParams p, float* delta) {
   typedef typename AtFrag<T>::type frag_t;

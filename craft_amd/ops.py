@@ -781,8 +781,8 @@ def _layer_norm_fwd(x, weight, bias, eps, out, keep: bool):
 def layer_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None, eps: float = 1e-5,
                out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """LayerNorm over the last axis (width up to 16384) of fp32 / fp16 / bf16 rows; weight and bias [C] of the rows' type or fp32, each optional.
-    Statistics in fp32, the result rounded once to x's type.  ``out`` may be x, and must not overlap it otherwise.  ``tokens_norm`` is the weightless fp32 form of the model's tokens; the differentiable
-    form is ``autograd.layer_norm``."""
+    Statistics in fp32, the result rounded once to x's type.  ``out`` may be x, and must not overlap it otherwise.  ``tokens_norm`` is the weightless fp32 form
+    of the model's tokens; the differentiable form is ``autograd.layer_norm``."""
     with torch.no_grad():
         return _layer_norm(x, weight, bias, eps, out, False)[0]
 
